@@ -38,6 +38,11 @@ enum {
 
 #define EXL3_MAX_SHARDS 4
 
+/* Scalar types, where an argument may have more than two. */
+#define EXL3_F16 0
+#define EXL3_BF16 1
+#define EXL3_F32 2
+
 /* The first EXL3_WORKSPACE_COUNTER_BYTES of every exl3_linear / exl3_gemm_rotated / exl3_moe_forward workspace hold
  * the split counters (one int per output column block).  They must be zero before the first call on a workspace;
  * every call leaves them zero again, so calls of any shapes may share one workspace (ordered on one stream).  The
@@ -301,6 +306,91 @@ int exl3_kv_decode_attention(const void* q, const void* k_cache, const void* v_c
                              const void* seq_lens, int batch, int num_q_heads, int num_kv_heads, int head_dim,
                              int page_size, int bits, float sm_scale, void* out, void* workspace,
                              size_t workspace_bytes, void* stream);
+
+/* ---- Around the quantized-KV attention of a decode or speculative step ----------------------------------------------
+ * No counterpart in the reference: its engines bring these steps themselves.  Token strides (ld_*) count elements from
+ * one token's heads to the next's, multiples of 8, so q, k and v may be columns of the fused linear's output; a token's
+ * heads are contiguous, and every tensor is 16-byte aligned.  Caches, page tables and seq_lens as
+ * exl3_kv_decode_attention has them. */
+
+/* q_out, k_out [tokens][heads][128] = the heads of q and k, each normalised over its 128 values with its weight,
+ *   y = x * rsqrt(mean(x^2) + eps) * w      (weights fp16 | bf16 | fp32 [128], w_type EXL3_F16 / _BF16 / _F32; both or
+ *                                            neither: NULL leaves the heads as they are),
+ * then rotated by their token's position (cos_sin NULL: not rotated): the pairs (i, i + rotary_dim / 2) of the first
+ * rotary_dim values (a multiple of 16, at most 128), or (2i, 2i + 1) when `interleaved`, by row positions[t] of cos_sin
+ * fp32 [max_pos][rotary_dim] = the cosines, then the sines.  positions int32 or int64 [tokens], clamped into the table.
+ * fp32 inside, one rounding; x fp16 | bf16, outputs fp16 | bf16 and contiguous.  An output may be its own input where both
+ * have one layout and type; otherwise they must not overlap. */
+int exl3_qk_norm_rope(const void* q, const void* k, int x_bf16, long long ld_q, long long ld_k, int tokens,
+                      int num_q_heads, int num_kv_heads, int head_dim, const void* q_weight, const void* k_weight,
+                      int w_type, float eps, const float* cos_sin, int max_pos, int rotary_dim, int interleaved,
+                      const void* positions, int positions_i64, void* q_out, void* k_out, int out_bf16, void* stream);
+
+/* Quantizes new keys and values into the cache, at positions seq_lens[b], seq_lens[b] + 1, ... of sequence b (seq_lens are
+ * the lengths before the call and are not changed).  k, v fp16 | bf16, `rows` token rows of num_kv_heads x 128.  Sequence
+ * b's rows are row_start[b] .. row_start[b + 1] - 1 (int32 [batch + 1]), or, with row_start NULL, rows_per_seq rows each
+ * (rows = batch * rows_per_seq).  Its new tokens are all of them, or those that row select[b][j] names, counted from the
+ * sequence's first (int32 [batch][max_new], e.g. accepted_nodes of exl3_verify_drafts); of them the first counts[b]
+ * (int32 [batch], NULL: all) and at most max_new.
+ * Per page, kv head and K or V: scale = the smallest fp16 not below max |x| / qmax over the new finite values (qmax 127 or
+ * 7), and not below the page's scale if it holds older tokens, whose codes are then rounded anew where it grew; code = x /
+ * scale to the nearest integer (ties to even), infinities to +-qmax, NaN to 0.  A value is off by at most scale / 2 when
+ * written, and by as much again for each time that its page's scale grows.
+ * Tokens past the table or selected outside their sequence's rows, and pages whose id is outside [0, num_pages), are not
+ * written; slots past the last token keep their codes.  No two sequences may append to one page. */
+int exl3_kv_append(const void* k, const void* v, int x_bf16, long long ld_k, long long ld_v, int rows,
+                   const int* row_start, int rows_per_seq, const int* select, const int* counts, int max_new,
+                   void* k_cache, void* v_cache, void* k_scale, void* v_scale, int num_pages, const int* page_table,
+                   int max_pages, const int* seq_lens, int batch, int num_kv_heads, int head_dim, int page_size,
+                   int bits, void* stream);
+
+/* Reads the cache back: k_out, v_out fp16 | bf16 [rows][num_kv_heads][128], row row_start[b] + i = code * scale of token
+ * starts[b] + i (starts int32 [batch], NULL: 0) of sequence b, for the rows below row_start[b + 1] (int32 [batch + 1],
+ * ascending) and the tokens below seq_lens[b]; other rows are left as they were.  Page ids outside [0, num_pages) are
+ * clamped. */
+int exl3_kv_gather(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale, int num_pages,
+                   const int* page_table, int max_pages, const int* seq_lens, const int* starts, const int* row_start,
+                   int batch, int rows, int num_kv_heads, int head_dim, int page_size, int bits, void* k_out,
+                   void* v_out, int out_bf16, void* stream);
+
+/* Workspace bytes of exl3_kv_tree_attention (fp32 partial states of split rows).  No zero-fill needed. */
+size_t exl3_kv_tree_workspace_bytes(int batch, int nodes, int num_q_heads, int num_kv_heads, int max_pages);
+/* Attention of `nodes` drafted tokens per sequence (1 to 64) over the cache and each other:
+ *   out[b][i][h] = softmax(sm_scale * q[b][i][h] . [K_b ; K'_b]^T) [V_b ; V'_b]
+ * with K_b, V_b the first seq_lens[b] cached tokens, which every node sees, and K'_b, V'_b the nodes' own keys and values
+ * (k_new, v_new fp16 [batch][nodes][num_kv_heads][128], token strides ld_k, ld_v), of which node i sees those whose bits
+ * tree_mask[b][i] sets (uint64 [batch][nodes], bit j: node j; its own bit too, as a rule; NULL: nodes 0 .. i).  q fp16
+ * [batch][nodes][num_q_heads][128] (token stride ld_q), out the same, contiguous.  num_nodes int32 [batch] (NULL: all):
+ * the nodes of a sequence from there on are neither read nor written.  A node that sees nothing gives zeros; what a node
+ * does not see does not reach it, infinities and NaN included.  Two launches; deterministic; calls that share a workspace
+ * must not overlap. */
+int exl3_kv_tree_attention(const void* q, long long ld_q, const void* k_new, const void* v_new, long long ld_k,
+                           long long ld_v, const void* tree_mask, int nodes, const int* num_nodes, const void* k_cache,
+                           const void* v_cache, const void* k_scale, const void* v_scale, int num_pages,
+                           const int* page_table, int max_pages, const int* seq_lens, int batch, int num_q_heads,
+                           int num_kv_heads, int head_dim, int page_size, int bits, float sm_scale, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of exl3_verify_drafts.  No zero-fill needed. */
+size_t exl3_verify_workspace_bytes(int batch, int vocab);
+/* Verification of drafted tokens: node 0 of a sequence is its last committed token, nodes 1 .. are drafts (1 to 64 nodes).
+ * target_probs fp32 [batch][nodes][vocab]: row i is the target's distribution after node i (rows sum to 1; entries that
+ * are not positive and finite count as 0); tokens int32 [batch][nodes] (node 0's is not read as a draft); parents int32
+ * [batch][nodes], 0 <= parent < node (a node with another parent is never reached; NULL: a chain, node i after i - 1);
+ * uniform fp32 [batch][nodes] in [0, 1); num_nodes int32 [batch] (NULL: all).
+ *   draft_probs fp32 [batch][nodes][vocab] (chains only), row i the distribution that node i + 1 was drawn from: node i is
+ *     accepted while p(t) > 0 and u[i] q(t) < p(t); the next token comes from max(p - q, 0) after a refusal, else from p.
+ *   draft_probs NULL: the children of the last accepted node in index order, each accepted when p(t) > 0 and
+ *     u[i] m < p(t), m = 1 less the p of its refused brothers; refused tokens are struck from p.
+ * Next token: the smallest v whose running sum of weights passes u[0] times their sum (from p itself where they sum to 0,
+ * and -1 where that does too).  Both rules emit tokens that are distributed as the target's.
+ * counts int32 [batch]: the accepted nodes, the root among them, which is also the number of tokens emitted (0 for a
+ * sequence without nodes); accepted_nodes int32 [batch][nodes]: 0, then the accepted drafts; out_tokens int32
+ * [batch][nodes]: their tokens, then the next one; both -1 past counts[b].  Two launches; calls that share a workspace
+ * must not overlap. */
+int exl3_verify_drafts(const float* target_probs, const float* draft_probs, const int* tokens, const int* parents,
+                       const float* uniform, const int* num_nodes, int batch, int nodes, int vocab, int* accepted_nodes,
+                       int* counts, int* out_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

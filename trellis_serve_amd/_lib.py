@@ -49,7 +49,7 @@ class Exl3MoeClass(ctypes.Structure):
                 ("K_gate_up", ctypes.c_int), ("K_down", ctypes.c_int)]
 
 
-_P, _I, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_P, _I, _SZ, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong, ctypes.c_float
 _SIGNATURES: dict[str, tuple] = {
     "exl3_abi_version": (_I, []),
     "exl3_last_error": (ctypes.c_char_p, []),
@@ -87,6 +87,16 @@ _SIGNATURES: dict[str, tuple] = {
     "exl3_kv_decode_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "exl3_kv_decode_attention": (_I, [_P, _P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, ctypes.c_float, _P,
                                       _P, _SZ, _P]),
+    "exl3_qk_norm_rope": (_I, [_P, _P, _I, _LL, _LL, _I, _I, _I, _I, _P, _P, _I, _F, _P, _I, _I, _I, _P, _I, _P, _P, _I,
+                               _P]),
+    "exl3_kv_append": (_I, [_P, _P, _I, _LL, _LL, _I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I,
+                            _I, _P]),
+    "exl3_kv_gather": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P]),
+    "exl3_kv_tree_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "exl3_kv_tree_attention": (_I, [_P, _LL, _P, _P, _LL, _LL, _P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I,
+                                    _I, _I, _I, _F, _P, _P, _SZ, _P]),
+    "exl3_verify_workspace_bytes": (_SZ, [_I, _I]),
+    "exl3_verify_drafts": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

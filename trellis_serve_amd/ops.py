@@ -732,3 +732,332 @@ def kv_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                                             out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(q.device)),
                "kv_decode_attention")
     return out
+
+
+# ---- Around the quantized-KV attention: what a decode or speculative step does between its linears and the cache.  The
+# reference has no counterpart of these (its engines bring them).  Their workspaces come from torch's allocator on the
+# current stream, call by call: calls on several streams and captured graphs never share one.  A caller that may not
+# allocate passes `workspace`; calls that share it must then be ordered.
+
+_HEAD_DIM = 128
+_HALVES = (torch.float16, torch.bfloat16)
+_WEIGHT_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _token_stride(t: torch.Tensor, name: str, dims: int, dtypes=_HALVES) -> int:
+    """Elements from one token's heads to the next's in t [..., heads, 128] (`dims` dimensions): columns of a wider row
+    are fine, a token's heads are contiguous."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    if len(shape) != dims or shape[-1] != _HEAD_DIM:
+        raise ValueError(f"{name} must be a {dims}-D tensor [..., heads, {_HEAD_DIM}], got {tuple(shape)}")
+    if stride[-1] != 1 or (shape[-2] > 1 and stride[-2] != _HEAD_DIM):
+        raise ValueError(f"{name}: a token's heads must be contiguous, got strides {stride}")
+    if dims == 3:
+        return stride[0] if shape[0] > 1 else shape[1] * _HEAD_DIM
+    if shape[0] > 1 and shape[1] > 1 and stride[0] != shape[1] * stride[1]:
+        raise ValueError(f"{name}: the sequences' tokens must lie at one stride, got strides {stride}")
+    return stride[1] if shape[1] > 1 else stride[0] if shape[0] > 1 else shape[2] * _HEAD_DIM
+
+
+def _check_int32(t: torch.Tensor | None, name: str, shape: tuple) -> None:
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int) -> tuple[int, int, int, int]:
+    """Checks a paged cache as kv_decode_attention takes it; returns (pages, kv heads, sequences, table width)."""
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or shape[2] != 16 or shape[3] != _HEAD_DIM * bits // 8:
+        raise ValueError(f"k_cache / v_cache must both be [P, Hkv, 16, {_HEAD_DIM * bits // 8}] at {bits} bits, got "
+                         f"{tuple(shape)} / {tuple(v_cache.shape)}")
+    if k_cache.element_size() != 1 or v_cache.element_size() != 1:
+        raise ValueError("caches must hold 1-byte codes (int8 / uint8)")
+    P, Hkv = shape[0], shape[1]
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float16 or tuple(t.shape) != (P, Hkv):
+            raise ValueError(f"{name} must be fp16 [{P}, {Hkv}]")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+        raise ValueError("page_table must be int32 [B, max_pages]")
+    B, max_pages = page_table.shape
+    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,):
+        raise ValueError(f"seq_lens must be int32 [{B}]")
+    for t in (k_cache, v_cache, k_scale, v_scale, page_table, seq_lens):
+        if not t.is_contiguous():
+            raise ValueError("caches, scales, page table and lengths must be contiguous")
+    return P, Hkv, B, max_pages
+
+
+def _one_device(device: torch.device, tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors must be on one device, got {t.device} and {device}")
+    if device.type != "cuda":
+        raise ValueError(f"Expected a cuda device, but got: {device}")
+
+
+def _call_workspace(workspace: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+    if workspace is None:
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    if not workspace.is_contiguous() or workspace.device != device:
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    return workspace
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 cos_sin: torch.Tensor | None, positions: torch.Tensor | None, eps: float = 1e-6,
+                 interleaved: bool = False, out_dtype: torch.dtype | None = None,
+                 out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The norm of every query and key head and its rotation by the token's position, in one launch.
+    q fp16|bf16 [T, Hq, 128], k [T, Hkv, 128], columns of the fused q/k/v linear's output or tensors of their own;
+    q_weight, k_weight fp16|bf16|fp32 [128] (both None: no norm); cos_sin fp32 [max_pos, rotary] holds the cosines and then
+    the sines of every position (rotary a multiple of 16 up to 128; None: no rotation), positions int32|int64 [T] (clamped
+    into the table).  Pairs are (i, i + rotary / 2), or (2i, 2i + 1) when `interleaved`.  fp32 inside; returns (q, k)
+    contiguous in `out_dtype` (q's by default; fp16 for the attention over the cache), in `out` if given (which may be q
+    and k themselves where those are contiguous and of one type)."""
+    ld_q, ld_k = _token_stride(q, "q", 3), _token_stride(k, "k", 3)
+    T, Hq, _ = q.shape
+    Hkv = k.shape[1]
+    if k.shape[0] != T or k.dtype != q.dtype:
+        raise ValueError(f"k must hold {T} tokens in {q.dtype}, got {k.shape[0]} in {k.dtype}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("both weights or neither")
+    w_type = 0
+    if q_weight is not None:
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w.dtype not in _WEIGHT_TYPE or tuple(w.shape) != (_HEAD_DIM,) or w.dtype != q_weight.dtype \
+                    or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [{_HEAD_DIM}] tensor, both of one type (fp16, bf16, fp32)")
+        w_type = _WEIGHT_TYPE[q_weight.dtype]
+    max_pos = rotary = 0
+    if cos_sin is not None:
+        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+            raise ValueError("cos_sin must be a contiguous fp32 [max_pos, rotary] tensor")
+        if positions is None or positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,) \
+                or not positions.is_contiguous():
+            raise ValueError(f"positions must be a contiguous int32/int64 [{T}] tensor")
+        max_pos, rotary = cos_sin.shape
+        if max_pos < 1 or rotary % 16 or not 16 <= rotary <= _HEAD_DIM:
+            raise ValueError(f"cos_sin {tuple(cos_sin.shape)}: rotary must be a multiple of 16 up to {_HEAD_DIM}")
+    elif q_weight is None:
+        raise ValueError("neither weights nor a rotation table")
+    if out is None:
+        out_dtype = out_dtype or q.dtype
+        if out_dtype not in _HALVES:
+            raise ValueError(f"out_dtype must be fp16 or bf16, got {out_dtype}")
+        q_out = torch.empty((T, Hq, _HEAD_DIM), dtype=out_dtype, device=q.device)
+        k_out = torch.empty((T, Hkv, _HEAD_DIM), dtype=out_dtype, device=q.device)
+    else:
+        q_out, k_out = out
+        _check_out(q_out, (T, Hq, _HEAD_DIM), q)
+        _check_out(k_out, (T, Hkv, _HEAD_DIM), q)
+        if q_out.dtype != k_out.dtype or out_dtype not in (None, q_out.dtype):
+            raise ValueError(f"outputs of one type, got {q_out.dtype}, {k_out.dtype}")
+        for x, o in ((q, q_out), (k, k_out)):
+            if x.data_ptr() == o.data_ptr() and (x.dtype != o.dtype or not x.is_contiguous()):
+                raise ValueError("an output may be its input only where both are contiguous and of one type")
+    device = q.device
+    _one_device(device, (k, q_weight, k_weight, cos_sin, positions, q_out, k_out))
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, None, (q_out, k_out))
+    _lib.check(_lib.load().exl3_qk_norm_rope(
+        q.data_ptr(), k.data_ptr(), int(q.dtype == torch.bfloat16), ld_q, ld_k, T, Hq, Hkv, _HEAD_DIM, _ptr(q_weight),
+        _ptr(k_weight), w_type, float(eps), _ptr(cos_sin), max_pos, rotary, int(interleaved),
+        _ptr(positions) if cos_sin is not None else None, int(positions is not None and positions.dtype == torch.int64),
+        q_out.data_ptr(), k_out.data_ptr(), int(q_out.dtype == torch.bfloat16), _stream(device)), "qk_norm_rope")
+    return q_out, k_out
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+              v_scale: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int,
+              row_start: torch.Tensor | None = None, max_new: int | None = None, select: torch.Tensor | None = None,
+              counts: torch.Tensor | None = None) -> None:
+    """Quantizes new keys and values into the paged cache (the layout of kv_decode_attention), at positions seq_lens[b],
+    seq_lens[b] + 1, ... of sequence b; seq_lens (the lengths before the call) are not changed.  k, v fp16|bf16, columns of
+    a wider row allowed:
+      [B, n, Hkv, 128]     n rows a sequence (with `counts` int32 [B]: the first counts[b] of them);
+      [B, Hkv, 128]        one a sequence;
+      [rows, Hkv, 128]     with row_start int32 [B + 1]: rows row_start[b] .. row_start[b + 1] - 1 are sequence b's
+                           (`max_new`: the most a sequence has, if known on the host; it sizes the launch).
+    select int32 [B, S]: token j of sequence b is its row select[b, j] (the accepted nodes of verify_drafts, with its
+    `counts`).  A page's scale covers its new tokens and what it held; older codes are rounded anew where it grows.  Tokens
+    past the table and pages outside the cache are not written; no two sequences may append to one page."""
+    P, Hkv, B, max_pages = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits)
+    dims = k.dim()
+    if dims not in (3, 4) or (dims == 4 and row_start is not None):
+        raise ValueError("k must be [B, n, Hkv, 128], [B, Hkv, 128], or [rows, Hkv, 128] with row_start")
+    ld_k, ld_v = _token_stride(k, "k", dims), _token_stride(v, "v", dims)
+    if v.shape != k.shape or v.dtype != k.dtype or k.shape[-2] != Hkv:
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, of {Hkv} heads")
+    rows = k.shape[0] * k.shape[1] if dims == 4 else k.shape[0]
+    per_seq = 0
+    if row_start is None:
+        if k.shape[0] != B:
+            raise ValueError(f"k holds {k.shape[0]} sequences, the page table {B}")
+        per_seq = k.shape[1] if dims == 4 else 1
+    _check_int32(row_start, "row_start", (B + 1,))
+    _check_int32(counts, "counts", (B,))
+    if select is not None:
+        if select.dim() != 2:
+            raise ValueError(f"select must be int32 [{B}, S]")
+        _check_int32(select, "select", (B, select.shape[1]))
+        max_new = select.shape[1]
+    elif max_new is None or row_start is None:
+        max_new = rows if row_start is not None else per_seq
+    if max_new < 0:
+        raise ValueError(f"max_new = {max_new}")
+    device = k.device
+    _one_device(device, (v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, select, counts))
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return kv_append(k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits, row_start, max_new,
+                             select, counts)
+    _lib.check(_lib.load().exl3_kv_append(
+        k.data_ptr(), v.data_ptr(), int(k.dtype == torch.bfloat16), ld_k, ld_v, rows, _ptr(row_start), per_seq,
+        _ptr(select), _ptr(counts), int(max_new), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), P, page_table.data_ptr(), max_pages, seq_lens.data_ptr(), B, Hkv, _HEAD_DIM, 16, int(bits),
+        _stream(device)), "kv_append")
+
+
+def kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+              page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int, row_start: torch.Tensor, rows: int,
+              starts: torch.Tensor | None = None, dtype: torch.dtype = torch.float16,
+              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Reads the paged cache back: (k, v) fp16|bf16 [rows, Hkv, 128] whose row row_start[b] + i is token starts[b] + i of
+    sequence b, for the rows below row_start[b + 1] (int32 [B + 1], ascending) and the tokens below seq_lens[b]; starts int32
+    [B] (None: 0).  Other rows are left as they were (in tensors made here: uninitialised).  Page ids outside the cache are
+    clamped."""
+    P, Hkv, B, max_pages = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits)
+    _check_int32(row_start, "row_start", (B + 1,))
+    _check_int32(starts, "starts", (B,))
+    shape, device = (int(rows), Hkv, _HEAD_DIM), k_cache.device
+    if out is None:
+        if dtype not in _HALVES or rows < 0:
+            raise ValueError(f"rows = {rows}; dtype must be fp16 or bf16, got {dtype}")
+        out = (torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
+    k_out, v_out = out
+    _check_out(k_out, shape, k_cache)
+    _check_out(v_out, shape, k_cache, (k_out.dtype,))
+    _one_device(device, (v_cache, k_scale, v_scale, page_table, seq_lens, row_start, starts))
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return kv_gather(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits, row_start, rows, starts,
+                             dtype, out)
+    _lib.check(_lib.load().exl3_kv_gather(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, page_table.data_ptr(),
+        max_pages, seq_lens.data_ptr(), _ptr(starts), row_start.data_ptr(), B, int(rows), Hkv, _HEAD_DIM, 16, int(bits),
+        k_out.data_ptr(), v_out.data_ptr(), int(k_out.dtype == torch.bfloat16), _stream(device)), "kv_gather")
+    return k_out, v_out
+
+
+def kv_tree_workspace_bytes(batch: int, nodes: int, num_q_heads: int, num_kv_heads: int, max_pages: int) -> int:
+    """Bytes of a `workspace` for kv_tree_attention at this shape."""
+    return _lib.load().exl3_kv_tree_workspace_bytes(batch, nodes, num_q_heads, num_kv_heads, max_pages)
+
+
+def kv_tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, tree_mask: torch.Tensor | None,
+                      k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                      page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int, sm_scale: float | None = None,
+                      num_nodes: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each sequence's drafted tokens over the paged quantized cache and over each other.  q fp16
+    [B, N, Hq, 128], k_new / v_new fp16 [B, N, Hkv, 128] (N <= 64; columns of the fused linear's output allowed): every node
+    sees the seq_lens[b] cached tokens, and node i those nodes j of its sequence with bit j of tree_mask[b, i] set (int64
+    [B, N]; its own too, as a rule; None: nodes 0 .. i, a chain or a prompt's chunk).  num_nodes int32 [B]: the nodes of a
+    sequence from there on are neither read nor written.  A node that sees nothing gives zeros.  Cache as
+    kv_decode_attention; returns fp16 [B, N, Hq, 128]."""
+    P, Hkv, B, max_pages = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits)
+    half = (torch.float16,)
+    ld_q, ld_k, ld_v = (_token_stride(q, "q", 4, half), _token_stride(k_new, "k_new", 4, half),
+                        _token_stride(v_new, "v_new", 4, half))
+    _, N, Hq, _ = q.shape
+    if q.shape[0] != B or k_new.shape != (B, N, Hkv, _HEAD_DIM) or v_new.shape != k_new.shape:
+        raise ValueError(f"q {tuple(q.shape)}, k_new {tuple(k_new.shape)} and v_new {tuple(v_new.shape)} do not match "
+                         f"{B} sequences and {Hkv} kv heads")
+    if not 1 <= N <= 64 or Hq % Hkv or not 1 <= Hq // Hkv <= 16:
+        raise ValueError(f"1 to 64 nodes and 1 to 16 query heads per kv head, got {N} nodes, heads {Hq} / {Hkv}")
+    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tuple(tree_mask.shape) != (B, N)
+                                  or not tree_mask.is_contiguous()):
+        raise ValueError(f"tree_mask must be a contiguous int64 [{B}, {N}] tensor")
+    _check_int32(num_nodes, "num_nodes", (B,))
+    device = q.device
+    if out is None:
+        out = torch.empty((B, N, Hq, _HEAD_DIM), dtype=torch.float16, device=device)
+    else:
+        _check_out(out, (B, N, Hq, _HEAD_DIM), q, half)
+    _one_device(device, (k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, num_nodes))
+    if sm_scale is None:
+        sm_scale = _HEAD_DIM ** -0.5
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return kv_tree_attention(q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table,
+                                     seq_lens, bits, sm_scale, num_nodes, out, workspace)
+    lib = _lib.load()
+    ws = _call_workspace(workspace, lib.exl3_kv_tree_workspace_bytes(B, N, Hq, Hkv, max_pages), device)
+    _lib.check(lib.exl3_kv_tree_attention(
+        q.data_ptr(), ld_q, k_new.data_ptr(), v_new.data_ptr(), ld_k, ld_v, _ptr(tree_mask), N, _ptr(num_nodes),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, page_table.data_ptr(),
+        max_pages, seq_lens.data_ptr(), B, Hq, Hkv, _HEAD_DIM, 16, int(bits), float(sm_scale), out.data_ptr(),
+        ws.data_ptr(), ws.numel() * ws.element_size(), _stream(device)), "kv_tree_attention")
+    return out
+
+
+def verify_workspace_bytes(batch: int, vocab: int) -> int:
+    """Bytes of a `workspace` for verify_drafts at this shape."""
+    return _lib.load().exl3_verify_workspace_bytes(batch, vocab)
+
+
+def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniform: torch.Tensor,
+                  parents: torch.Tensor | None = None, draft_probs: torch.Tensor | None = None,
+                  num_nodes: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stay, and the token after them, so that every emitted token is distributed as the target's.
+    Node 0 of a sequence is its last committed token, nodes 1 .. N - 1 are drafts (N <= 64).  target_probs fp32 [B, N, V]:
+    row i after node i; tokens int32|int64 [B, N]; uniform fp32 [B, N] in [0, 1): u[b, i] decides node i, u[b, 0] draws the
+    next token; parents int32|int64 [B, N], a node's parent before it (None: a chain); num_nodes int32 [B] (None: N each).
+      draft_probs fp32 [B, N, V] (chains): row i is what node i + 1 was drawn from; accepted while u q(t) < p(t), the next
+        token from max(p - q, 0) after a refusal;
+      None: candidates however chosen; brothers in order, accepted when u m < p(t) with m = 1 less their refused brothers'
+        p, refused tokens struck from p.
+    Returns (accepted_nodes [B, N]: 0, then the accepted drafts; counts [B]: how many of them, the root among them;
+    out_tokens [B, N]: the accepted drafts' tokens, then the next one), int32, -1 past counts[b].  accepted_nodes and counts
+    are what kv_append takes as `select` and `counts`."""
+    if target_probs.dtype != torch.float32 or target_probs.dim() != 3 or not target_probs.is_contiguous():
+        raise ValueError(f"target_probs must be a contiguous fp32 [B, N, V] tensor, got {target_probs.dtype} "
+                         f"{tuple(target_probs.shape)}")
+    B, N, V = target_probs.shape
+    if not 1 <= N <= 64 or V < 1:
+        raise ValueError(f"1 to 64 nodes and at least one token, got {N} nodes, {V} tokens")
+    for name, t in (("tokens", tokens), ("parents", parents)):
+        if t is not None and (t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B, N)):
+            raise ValueError(f"{name} must be int32/int64 [{B}, {N}], got {t.dtype} {tuple(t.shape)}")
+    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (B, N) or not uniform.is_contiguous():
+        raise ValueError(f"uniform must be a contiguous fp32 [{B}, {N}] tensor")
+    if draft_probs is not None:
+        if parents is not None:
+            raise ValueError("the draft's probabilities come with a chain (parents = None)")
+        if draft_probs.dtype != torch.float32 or draft_probs.shape != target_probs.shape \
+                or not draft_probs.is_contiguous():
+            raise ValueError(f"draft_probs must be a contiguous fp32 [{B}, {N}, {V}] tensor")
+    _check_int32(num_nodes, "num_nodes", (B,))
+    device = target_probs.device
+    _one_device(device, (tokens, uniform, parents, draft_probs, num_nodes))
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return verify_drafts(target_probs, tokens, uniform, parents, draft_probs, num_nodes, workspace)
+    tokens = tokens.to(torch.int32).contiguous()
+    parents = None if parents is None else parents.to(torch.int32).contiguous()
+    accepted, out_tokens = (torch.empty((B, N), dtype=torch.int32, device=device) for _ in range(2))
+    counts = torch.empty(B, dtype=torch.int32, device=device)
+    lib = _lib.load()
+    ws = _call_workspace(workspace, lib.exl3_verify_workspace_bytes(B, V), device)
+    _lib.check(lib.exl3_verify_drafts(
+        target_probs.data_ptr(), _ptr(draft_probs), tokens.data_ptr(), _ptr(parents), uniform.data_ptr(),
+        _ptr(num_nodes), B, N, V, accepted.data_ptr(), counts.data_ptr(), out_tokens.data_ptr(), ws.data_ptr(),
+        ws.numel() * ws.element_size(), _stream(device)), "verify_drafts")
+    return accepted, counts, out_tokens
