@@ -739,9 +739,13 @@ def kv_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
 # current stream, call by call: calls on several streams and captured graphs never share one.  A caller that may not
 # allocate passes `workspace`; calls that share it must then be ordered.
 
+# The checks are written for their cost: a call of 23 arguments takes 3.4 us, and each attribute read of a tensor 0.06.
+
 _HEAD_DIM = 128
 _HALVES = (torch.float16, torch.bfloat16)
+_FP16 = (torch.float16,)
 _WEIGHT_TYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_INTS = (torch.int32, torch.int64)
 
 
 def _token_stride(t: torch.Tensor, name: str, dims: int, dtypes=_HALVES) -> int:
@@ -752,59 +756,71 @@ def _token_stride(t: torch.Tensor, name: str, dims: int, dtypes=_HALVES) -> int:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
     if len(shape) != dims or shape[-1] != _HEAD_DIM:
         raise ValueError(f"{name} must be a {dims}-D tensor [..., heads, {_HEAD_DIM}], got {tuple(shape)}")
-    if stride[-1] != 1 or (shape[-2] > 1 and stride[-2] != _HEAD_DIM):
+    if stride[-1] != 1 or (stride[-2] != _HEAD_DIM and shape[-2] > 1):
         raise ValueError(f"{name}: a token's heads must be contiguous, got strides {stride}")
     if dims == 3:
         return stride[0] if shape[0] > 1 else shape[1] * _HEAD_DIM
-    if shape[0] > 1 and shape[1] > 1 and stride[0] != shape[1] * stride[1]:
+    B, n, heads, _ = shape
+    if n == 1:
+        return stride[0] if B > 1 else heads * _HEAD_DIM
+    if B > 1 and stride[0] != n * stride[1]:
         raise ValueError(f"{name}: the sequences' tokens must lie at one stride, got strides {stride}")
-    return stride[1] if shape[1] > 1 else stride[0] if shape[0] > 1 else shape[2] * _HEAD_DIM
+    return stride[1]
 
 
 def _check_int32(t: torch.Tensor | None, name: str, shape: tuple) -> None:
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+    if t is not None and (t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                  page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int) -> tuple[int, int, int, int]:
     """Checks a paged cache as kv_decode_attention takes it; returns (pages, kv heads, sequences, table width)."""
-    if bits not in (4, 8):
+    if bits != 8 and bits != 4:
         raise ValueError(f"bits must be 4 or 8, got {bits}")
     shape = k_cache.shape
-    if len(shape) != 4 or shape != v_cache.shape or shape[2] != 16 or shape[3] != _HEAD_DIM * bits // 8:
-        raise ValueError(f"k_cache / v_cache must both be [P, Hkv, 16, {_HEAD_DIM * bits // 8}] at {bits} bits, got "
+    if len(shape) != 4 or shape != v_cache.shape or shape[2] != 16 or shape[3] != 16 * bits:
+        raise ValueError(f"k_cache / v_cache must both be [P, Hkv, 16, {16 * bits}] at {bits} bits, got "
                          f"{tuple(shape)} / {tuple(v_cache.shape)}")
     if k_cache.element_size() != 1 or v_cache.element_size() != 1:
         raise ValueError("caches must hold 1-byte codes (int8 / uint8)")
     P, Hkv = shape[0], shape[1]
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float16 or tuple(t.shape) != (P, Hkv):
-            raise ValueError(f"{name} must be fp16 [{P}, {Hkv}]")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+    if k_scale.dtype != torch.float16 or k_scale.shape != (P, Hkv):
+        raise ValueError(f"k_scale must be fp16 [{P}, {Hkv}]")
+    if v_scale.dtype != torch.float16 or v_scale.shape != (P, Hkv):
+        raise ValueError(f"v_scale must be fp16 [{P}, {Hkv}]")
+    table = page_table.shape
+    if page_table.dtype != torch.int32 or len(table) != 2:
         raise ValueError("page_table must be int32 [B, max_pages]")
-    B, max_pages = page_table.shape
-    if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,):
+    B, max_pages = table
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,):
         raise ValueError(f"seq_lens must be int32 [{B}]")
-    for t in (k_cache, v_cache, k_scale, v_scale, page_table, seq_lens):
-        if not t.is_contiguous():
-            raise ValueError("caches, scales, page table and lengths must be contiguous")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+            and page_table.is_contiguous() and seq_lens.is_contiguous()):
+        raise ValueError("caches, scales, page table and lengths must be contiguous")
     return P, Hkv, B, max_pages
 
 
-def _one_device(device: torch.device, tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"all tensors must be on one device, got {t.device} and {device}")
-    if device.type != "cuda":
-        raise ValueError(f"Expected a cuda device, but got: {device}")
+def _cuda_index(first: torch.Tensor, *others) -> int:
+    """The index of the device that all tensors are on (None: no tensor)."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"all tensors must be on one device, got {t.device} and {first.device}")
+    if index < 0:
+        raise ValueError(f"Expected a cuda device, but got: {first.device}")
+    return index
 
 
-def _call_workspace(workspace: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+def _current(index: int) -> bool:
+    return torch._C._cuda_getDevice() == index
+
+
+def _call_workspace(workspace: torch.Tensor | None, nbytes: int, index: int) -> torch.Tensor:
     if workspace is None:
-        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-    if not workspace.is_contiguous() or workspace.device != device:
-        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=index)
+    if not workspace.is_contiguous() or workspace.get_device() != index:
+        raise ValueError(f"workspace must be a contiguous tensor on cuda:{index}")
     return workspace
 
 
@@ -821,55 +837,57 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     and k themselves where those are contiguous and of one type)."""
     ld_q, ld_k = _token_stride(q, "q", 3), _token_stride(k, "k", 3)
     T, Hq, _ = q.shape
-    Hkv = k.shape[1]
-    if k.shape[0] != T or k.dtype != q.dtype:
-        raise ValueError(f"k must hold {T} tokens in {q.dtype}, got {k.shape[0]} in {k.dtype}")
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("both weights or neither")
-    w_type = 0
-    if q_weight is not None:
+    Tk, Hkv, _ = k.shape
+    dtype = q.dtype
+    if Tk != T or k.dtype != dtype:
+        raise ValueError(f"k must hold {T} tokens in {dtype}, got {Tk} in {k.dtype}")
+    w_type = max_pos = rotary = wide = 0
+    wq = wk = cs = pos = None
+    if q_weight is not None and k_weight is not None:
+        w_dtype = q_weight.dtype
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w.dtype not in _WEIGHT_TYPE or tuple(w.shape) != (_HEAD_DIM,) or w.dtype != q_weight.dtype \
-                    or not w.is_contiguous():
+            if w.dtype != w_dtype or w_dtype not in _WEIGHT_TYPE or w.shape != (_HEAD_DIM,) or not w.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous [{_HEAD_DIM}] tensor, both of one type (fp16, bf16, fp32)")
-        w_type = _WEIGHT_TYPE[q_weight.dtype]
-    max_pos = rotary = 0
-    if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
-            raise ValueError("cos_sin must be a contiguous fp32 [max_pos, rotary] tensor")
-        if positions is None or positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,) \
-                or not positions.is_contiguous():
-            raise ValueError(f"positions must be a contiguous int32/int64 [{T}] tensor")
-        max_pos, rotary = cos_sin.shape
-        if max_pos < 1 or rotary % 16 or not 16 <= rotary <= _HEAD_DIM:
-            raise ValueError(f"cos_sin {tuple(cos_sin.shape)}: rotary must be a multiple of 16 up to {_HEAD_DIM}")
-    elif q_weight is None:
+        w_type, wq, wk = _WEIGHT_TYPE[w_dtype], q_weight.data_ptr(), k_weight.data_ptr()
+    elif q_weight is not None or k_weight is not None:
+        raise ValueError("both weights or neither")
+    elif cos_sin is None:
         raise ValueError("neither weights nor a rotation table")
+    if cos_sin is not None:
+        shape = cos_sin.shape
+        if cos_sin.dtype != torch.float32 or len(shape) != 2 or not cos_sin.is_contiguous():
+            raise ValueError("cos_sin must be a contiguous fp32 [max_pos, rotary] tensor")
+        if positions is None or positions.dtype not in _INTS or positions.shape != (T,) or not positions.is_contiguous():
+            raise ValueError(f"positions must be a contiguous int32/int64 [{T}] tensor")
+        max_pos, rotary = shape
+        if max_pos < 1 or rotary % 16 or not 16 <= rotary <= _HEAD_DIM:
+            raise ValueError(f"cos_sin {tuple(shape)}: rotary must be a multiple of 16 up to {_HEAD_DIM}")
+        cs, pos, wide = cos_sin.data_ptr(), positions.data_ptr(), int(positions.dtype == torch.int64)
     if out is None:
-        out_dtype = out_dtype or q.dtype
+        out_dtype = out_dtype or dtype
         if out_dtype not in _HALVES:
             raise ValueError(f"out_dtype must be fp16 or bf16, got {out_dtype}")
-        q_out = torch.empty((T, Hq, _HEAD_DIM), dtype=out_dtype, device=q.device)
-        k_out = torch.empty((T, Hkv, _HEAD_DIM), dtype=out_dtype, device=q.device)
     else:
         q_out, k_out = out
         _check_out(q_out, (T, Hq, _HEAD_DIM), q)
         _check_out(k_out, (T, Hkv, _HEAD_DIM), q)
         if q_out.dtype != k_out.dtype or out_dtype not in (None, q_out.dtype):
             raise ValueError(f"outputs of one type, got {q_out.dtype}, {k_out.dtype}")
+        out_dtype = q_out.dtype
         for x, o in ((q, q_out), (k, k_out)):
             if x.data_ptr() == o.data_ptr() and (x.dtype != o.dtype or not x.is_contiguous()):
                 raise ValueError("an output may be its input only where both are contiguous and of one type")
-    device = q.device
-    _one_device(device, (k, q_weight, k_weight, cos_sin, positions, q_out, k_out))
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, None, (q_out, k_out))
+    index = _cuda_index(q, k, q_weight, k_weight, cos_sin, positions if cos_sin is not None else None)
+    if not _current(index):
+        with torch.cuda.device(index):
+            return qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, out_dtype, out)
+    if out is None:
+        q_out = torch.empty((T, Hq, _HEAD_DIM), dtype=out_dtype, device=index)
+        k_out = torch.empty((T, Hkv, _HEAD_DIM), dtype=out_dtype, device=index)
     _lib.check(_lib.load().exl3_qk_norm_rope(
-        q.data_ptr(), k.data_ptr(), int(q.dtype == torch.bfloat16), ld_q, ld_k, T, Hq, Hkv, _HEAD_DIM, _ptr(q_weight),
-        _ptr(k_weight), w_type, float(eps), _ptr(cos_sin), max_pos, rotary, int(interleaved),
-        _ptr(positions) if cos_sin is not None else None, int(positions is not None and positions.dtype == torch.int64),
-        q_out.data_ptr(), k_out.data_ptr(), int(q_out.dtype == torch.bfloat16), _stream(device)), "qk_norm_rope")
+        q.data_ptr(), k.data_ptr(), dtype == torch.bfloat16, ld_q, ld_k, T, Hq, Hkv, _HEAD_DIM, wq, wk, w_type, eps, cs,
+        max_pos, rotary, interleaved, pos, wide, q_out.data_ptr(), k_out.data_ptr(), out_dtype == torch.bfloat16,
+        torch._C._cuda_getCurrentRawStream(index)), "qk_norm_rope")
     return q_out, k_out
 
 
@@ -888,40 +906,46 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     `counts`).  A page's scale covers its new tokens and what it held; older codes are rounded anew where it grows.  Tokens
     past the table and pages outside the cache are not written; no two sequences may append to one page."""
     P, Hkv, B, max_pages = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits)
-    dims = k.dim()
+    shape = k.shape
+    dims = len(shape)
     if dims not in (3, 4) or (dims == 4 and row_start is not None):
         raise ValueError("k must be [B, n, Hkv, 128], [B, Hkv, 128], or [rows, Hkv, 128] with row_start")
     ld_k, ld_v = _token_stride(k, "k", dims), _token_stride(v, "v", dims)
-    if v.shape != k.shape or v.dtype != k.dtype or k.shape[-2] != Hkv:
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be alike, of {Hkv} heads")
-    rows = k.shape[0] * k.shape[1] if dims == 4 else k.shape[0]
+    dtype = k.dtype
+    if v.shape != shape or v.dtype != dtype or shape[-2] != Hkv:
+        raise ValueError(f"k {tuple(shape)} {dtype} and v {tuple(v.shape)} {v.dtype} must be alike, of {Hkv} heads")
+    rows = shape[0] * shape[1] if dims == 4 else shape[0]
     per_seq = 0
+    starts = picks = limits = None
     if row_start is None:
-        if k.shape[0] != B:
-            raise ValueError(f"k holds {k.shape[0]} sequences, the page table {B}")
-        per_seq = k.shape[1] if dims == 4 else 1
-    _check_int32(row_start, "row_start", (B + 1,))
-    _check_int32(counts, "counts", (B,))
+        if shape[0] != B:
+            raise ValueError(f"k holds {shape[0]} sequences, the page table {B}")
+        per_seq = shape[1] if dims == 4 else 1
+    else:
+        _check_int32(row_start, "row_start", (B + 1,))
+        starts = row_start.data_ptr()
+    if counts is not None:
+        _check_int32(counts, "counts", (B,))
+        limits = counts.data_ptr()
     if select is not None:
         if select.dim() != 2:
             raise ValueError(f"select must be int32 [{B}, S]")
-        _check_int32(select, "select", (B, select.shape[1]))
         max_new = select.shape[1]
+        _check_int32(select, "select", (B, max_new))
+        picks = select.data_ptr()
     elif max_new is None or row_start is None:
         max_new = rows if row_start is not None else per_seq
     if max_new < 0:
         raise ValueError(f"max_new = {max_new}")
-    device = k.device
-    _one_device(device, (v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, select, counts))
-    if _elsewhere(device):
-        with torch.cuda.device(device):
+    index = _cuda_index(k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, select, counts)
+    if not _current(index):
+        with torch.cuda.device(index):
             return kv_append(k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits, row_start, max_new,
                              select, counts)
     _lib.check(_lib.load().exl3_kv_append(
-        k.data_ptr(), v.data_ptr(), int(k.dtype == torch.bfloat16), ld_k, ld_v, rows, _ptr(row_start), per_seq,
-        _ptr(select), _ptr(counts), int(max_new), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), P, page_table.data_ptr(), max_pages, seq_lens.data_ptr(), B, Hkv, _HEAD_DIM, 16, int(bits),
-        _stream(device)), "kv_append")
+        k.data_ptr(), v.data_ptr(), dtype == torch.bfloat16, ld_k, ld_v, rows, starts, per_seq, picks, limits, max_new,
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, page_table.data_ptr(), max_pages,
+        seq_lens.data_ptr(), B, Hkv, _HEAD_DIM, 16, bits, torch._C._cuda_getCurrentRawStream(index)), "kv_append")
 
 
 def kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -934,24 +958,31 @@ def kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tenso
     clamped."""
     P, Hkv, B, max_pages = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits)
     _check_int32(row_start, "row_start", (B + 1,))
-    _check_int32(starts, "starts", (B,))
-    shape, device = (int(rows), Hkv, _HEAD_DIM), k_cache.device
+    first = None
+    if starts is not None:
+        _check_int32(starts, "starts", (B,))
+        first = starts.data_ptr()
+    shape = (rows, Hkv, _HEAD_DIM)
     if out is None:
         if dtype not in _HALVES or rows < 0:
             raise ValueError(f"rows = {rows}; dtype must be fp16 or bf16, got {dtype}")
-        out = (torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device))
-    k_out, v_out = out
-    _check_out(k_out, shape, k_cache)
-    _check_out(v_out, shape, k_cache, (k_out.dtype,))
-    _one_device(device, (v_cache, k_scale, v_scale, page_table, seq_lens, row_start, starts))
-    if _elsewhere(device):
-        with torch.cuda.device(device):
+    else:
+        k_out, v_out = out
+        dtype = k_out.dtype
+        _check_out(k_out, shape, k_cache)
+        _check_out(v_out, shape, k_cache, (dtype,))
+    index = _cuda_index(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, starts)
+    if not _current(index):
+        with torch.cuda.device(index):
             return kv_gather(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits, row_start, rows, starts,
                              dtype, out)
+    if out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=index)
+        v_out = torch.empty(shape, dtype=dtype, device=index)
     _lib.check(_lib.load().exl3_kv_gather(
         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, page_table.data_ptr(),
-        max_pages, seq_lens.data_ptr(), _ptr(starts), row_start.data_ptr(), B, int(rows), Hkv, _HEAD_DIM, 16, int(bits),
-        k_out.data_ptr(), v_out.data_ptr(), int(k_out.dtype == torch.bfloat16), _stream(device)), "kv_gather")
+        max_pages, seq_lens.data_ptr(), first, row_start.data_ptr(), B, rows, Hkv, _HEAD_DIM, 16, bits, k_out.data_ptr(),
+        v_out.data_ptr(), dtype == torch.bfloat16, torch._C._cuda_getCurrentRawStream(index)), "kv_gather")
     return k_out, v_out
 
 
@@ -972,38 +1003,40 @@ def kv_tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     sequence from there on are neither read nor written.  A node that sees nothing gives zeros.  Cache as
     kv_decode_attention; returns fp16 [B, N, Hq, 128]."""
     P, Hkv, B, max_pages = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits)
-    half = (torch.float16,)
-    ld_q, ld_k, ld_v = (_token_stride(q, "q", 4, half), _token_stride(k_new, "k_new", 4, half),
-                        _token_stride(v_new, "v_new", 4, half))
-    _, N, Hq, _ = q.shape
-    if q.shape[0] != B or k_new.shape != (B, N, Hkv, _HEAD_DIM) or v_new.shape != k_new.shape:
+    ld_q, ld_k, ld_v = (_token_stride(q, "q", 4, _FP16), _token_stride(k_new, "k_new", 4, _FP16),
+                        _token_stride(v_new, "v_new", 4, _FP16))
+    Bq, N, Hq, _ = q.shape
+    if Bq != B or k_new.shape != (B, N, Hkv, _HEAD_DIM) or v_new.shape != k_new.shape:
         raise ValueError(f"q {tuple(q.shape)}, k_new {tuple(k_new.shape)} and v_new {tuple(v_new.shape)} do not match "
                          f"{B} sequences and {Hkv} kv heads")
     if not 1 <= N <= 64 or Hq % Hkv or not 1 <= Hq // Hkv <= 16:
         raise ValueError(f"1 to 64 nodes and 1 to 16 query heads per kv head, got {N} nodes, heads {Hq} / {Hkv}")
-    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tuple(tree_mask.shape) != (B, N)
-                                  or not tree_mask.is_contiguous()):
-        raise ValueError(f"tree_mask must be a contiguous int64 [{B}, {N}] tensor")
-    _check_int32(num_nodes, "num_nodes", (B,))
-    device = q.device
-    if out is None:
-        out = torch.empty((B, N, Hq, _HEAD_DIM), dtype=torch.float16, device=device)
-    else:
-        _check_out(out, (B, N, Hq, _HEAD_DIM), q, half)
-    _one_device(device, (k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, num_nodes))
+    mask = live = None
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.shape != (B, N) or not tree_mask.is_contiguous():
+            raise ValueError(f"tree_mask must be a contiguous int64 [{B}, {N}] tensor")
+        mask = tree_mask.data_ptr()
+    if num_nodes is not None:
+        _check_int32(num_nodes, "num_nodes", (B,))
+        live = num_nodes.data_ptr()
+    if out is not None:
+        _check_out(out, (B, N, Hq, _HEAD_DIM), q, _FP16)
+    index = _cuda_index(q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, num_nodes)
     if sm_scale is None:
         sm_scale = _HEAD_DIM ** -0.5
-    if _elsewhere(device):
-        with torch.cuda.device(device):
+    if not _current(index):
+        with torch.cuda.device(index):
             return kv_tree_attention(q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table,
                                      seq_lens, bits, sm_scale, num_nodes, out, workspace)
+    if out is None:
+        out = torch.empty((B, N, Hq, _HEAD_DIM), dtype=torch.float16, device=index)
     lib = _lib.load()
-    ws = _call_workspace(workspace, lib.exl3_kv_tree_workspace_bytes(B, N, Hq, Hkv, max_pages), device)
+    ws = _call_workspace(workspace, lib.exl3_kv_tree_workspace_bytes(B, N, Hq, Hkv, max_pages), index)
     _lib.check(lib.exl3_kv_tree_attention(
-        q.data_ptr(), ld_q, k_new.data_ptr(), v_new.data_ptr(), ld_k, ld_v, _ptr(tree_mask), N, _ptr(num_nodes),
-        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, page_table.data_ptr(),
-        max_pages, seq_lens.data_ptr(), B, Hq, Hkv, _HEAD_DIM, 16, int(bits), float(sm_scale), out.data_ptr(),
-        ws.data_ptr(), ws.numel() * ws.element_size(), _stream(device)), "kv_tree_attention")
+        q.data_ptr(), ld_q, k_new.data_ptr(), v_new.data_ptr(), ld_k, ld_v, mask, N, live, k_cache.data_ptr(),
+        v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P, page_table.data_ptr(), max_pages,
+        seq_lens.data_ptr(), B, Hq, Hkv, _HEAD_DIM, 16, bits, sm_scale, out.data_ptr(), ws.data_ptr(), ws.nbytes,
+        torch._C._cuda_getCurrentRawStream(index)), "kv_tree_attention")
     return out
 
 
@@ -1027,37 +1060,45 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniform: tor
     Returns (accepted_nodes [B, N]: 0, then the accepted drafts; counts [B]: how many of them, the root among them;
     out_tokens [B, N]: the accepted drafts' tokens, then the next one), int32, -1 past counts[b].  accepted_nodes and counts
     are what kv_append takes as `select` and `counts`."""
-    if target_probs.dtype != torch.float32 or target_probs.dim() != 3 or not target_probs.is_contiguous():
+    shape = target_probs.shape
+    if target_probs.dtype != torch.float32 or len(shape) != 3 or not target_probs.is_contiguous():
         raise ValueError(f"target_probs must be a contiguous fp32 [B, N, V] tensor, got {target_probs.dtype} "
-                         f"{tuple(target_probs.shape)}")
-    B, N, V = target_probs.shape
+                         f"{tuple(shape)}")
+    B, N, V = shape
     if not 1 <= N <= 64 or V < 1:
         raise ValueError(f"1 to 64 nodes and at least one token, got {N} nodes, {V} tokens")
     for name, t in (("tokens", tokens), ("parents", parents)):
-        if t is not None and (t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B, N)):
+        if t is not None and (t.dtype not in _INTS or t.shape != (B, N)):
             raise ValueError(f"{name} must be int32/int64 [{B}, {N}], got {t.dtype} {tuple(t.shape)}")
-    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (B, N) or not uniform.is_contiguous():
+    if uniform.dtype != torch.float32 or uniform.shape != (B, N) or not uniform.is_contiguous():
         raise ValueError(f"uniform must be a contiguous fp32 [{B}, {N}] tensor")
+    q = up = live = None
     if draft_probs is not None:
         if parents is not None:
             raise ValueError("the draft's probabilities come with a chain (parents = None)")
-        if draft_probs.dtype != torch.float32 or draft_probs.shape != target_probs.shape \
-                or not draft_probs.is_contiguous():
+        if draft_probs.dtype != torch.float32 or draft_probs.shape != shape or not draft_probs.is_contiguous():
             raise ValueError(f"draft_probs must be a contiguous fp32 [{B}, {N}, {V}] tensor")
-    _check_int32(num_nodes, "num_nodes", (B,))
-    device = target_probs.device
-    _one_device(device, (tokens, uniform, parents, draft_probs, num_nodes))
-    if _elsewhere(device):
-        with torch.cuda.device(device):
+        q = draft_probs.data_ptr()
+    if num_nodes is not None:
+        _check_int32(num_nodes, "num_nodes", (B,))
+        live = num_nodes.data_ptr()
+    index = _cuda_index(target_probs, tokens, uniform, parents, draft_probs, num_nodes)
+    if not _current(index):
+        with torch.cuda.device(index):
             return verify_drafts(target_probs, tokens, uniform, parents, draft_probs, num_nodes, workspace)
-    tokens = tokens.to(torch.int32).contiguous()
-    parents = None if parents is None else parents.to(torch.int32).contiguous()
-    accepted, out_tokens = (torch.empty((B, N), dtype=torch.int32, device=device) for _ in range(2))
-    counts = torch.empty(B, dtype=torch.int32, device=device)
+    if tokens.dtype != torch.int32 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int32).contiguous()
+    if parents is not None:
+        if parents.dtype != torch.int32 or not parents.is_contiguous():
+            parents = parents.to(torch.int32).contiguous()
+        up = parents.data_ptr()
+    accepted = torch.empty((B, N), dtype=torch.int32, device=index)
+    out_tokens = torch.empty((B, N), dtype=torch.int32, device=index)
+    counts = torch.empty(B, dtype=torch.int32, device=index)
     lib = _lib.load()
-    ws = _call_workspace(workspace, lib.exl3_verify_workspace_bytes(B, V), device)
+    ws = _call_workspace(workspace, lib.exl3_verify_workspace_bytes(B, V), index)
     _lib.check(lib.exl3_verify_drafts(
-        target_probs.data_ptr(), _ptr(draft_probs), tokens.data_ptr(), _ptr(parents), uniform.data_ptr(),
-        _ptr(num_nodes), B, N, V, accepted.data_ptr(), counts.data_ptr(), out_tokens.data_ptr(), ws.data_ptr(),
-        ws.numel() * ws.element_size(), _stream(device)), "verify_drafts")
+        target_probs.data_ptr(), q, tokens.data_ptr(), up, uniform.data_ptr(), live, B, N, V, accepted.data_ptr(),
+        counts.data_ptr(), out_tokens.data_ptr(), ws.data_ptr(), ws.nbytes,
+        torch._C._cuda_getCurrentRawStream(index)), "verify_drafts")
     return accepted, counts, out_tokens
