@@ -27,10 +27,9 @@ namespace exl3 {
 typedef float verify_f4_t __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any multiple of 4 bytes
 
 constexpr int kVerifyNodes = 64;     // a node per lane
-constexpr int kVerifyChunks = 64;    // most chunks of a row: a lane each in the pick
-constexpr int kMassThreads = 256;
-constexpr int kPickThreads = 1024;
-constexpr int kVerifyBlock = 4 * kPickThreads;  // chunk lengths are multiples of it
+constexpr int kVerifyPart = 1024;    // consecutive elements that one wave sums: 16 a lane
+constexpr int kMassWaves = 4;
+constexpr int kMassThreads = 64 * kMassWaves;
 
 struct VerifyEnd {
   unsigned long long struck;  // refused children of the last accepted node
@@ -44,9 +43,9 @@ struct VerifyArgs {
   const int *tokens, *parents;
   const float* uniform;
   const int* num_nodes;
-  int nodes, vocab, chunks, chunk_len;
+  int nodes, vocab, parts;
   int *accepted, *counts, *out_tokens;
-  double* mass;      // [batch][chunks][2]: the chunk's sum of w, and of p
+  double* mass;      // [batch][parts][2]: the part's sum of w, and of p
   VerifyEnd* end;    // [batch]
 };
 
@@ -110,13 +109,6 @@ __device__ __forceinline__ VerifyWalk verify_walk(const VerifyArgs& a, int b) {
   return w;
 }
 
-// p as a weight: finite positive values, anything else is 0
-__device__ __forceinline__ double verify_weight(float p) { return p > 0.f && p < __builtin_inff() ? (double)p : 0.0; }
-__device__ __forceinline__ double verify_rest(float p, float q) {
-  const double d = verify_weight(p) - (q > 0.f ? (double)q : 0.0);
-  return d > 0.0 ? d : 0.0;
-}
-
 // The struck tokens in [first, last), compacted into list by one wave; their number
 __device__ __forceinline__ int struck_in(unsigned long long struck, int token, int first, int last, int* list) {
   const int lane = threadIdx.x & 63;
@@ -126,70 +118,85 @@ __device__ __forceinline__ int struck_in(unsigned long long struck, int token, i
   return __builtin_popcountll(mask);
 }
 
-// Weights w[0..3] of elements v .. v+3 (0 past `last`), and their p
-__device__ __forceinline__ void verify_load(const float* p, const float* q, int v, int last, int nstruck,
-                                            const int* list, double w[4], double pw[4]) {
-  float pv[4] = {0.f, 0.f, 0.f, 0.f}, qv[4] = {0.f, 0.f, 0.f, 0.f};
-  if (v + 4 <= last) {
-    const verify_f4_t x = *reinterpret_cast<const verify_f4_t*>(p + v);
-#pragma unroll
-    for (int e = 0; e < 4; e++) pv[e] = x[e];
-    if (q) {
-      const verify_f4_t y = *reinterpret_cast<const verify_f4_t*>(q + v);
-#pragma unroll
-      for (int e = 0; e < 4; e++) qv[e] = y[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (v + e < last) {
-        pv[e] = p[v + e];
-        if (q) qv[e] = q[v + e];
-      }
-  }
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    pw[e] = verify_weight(pv[e]);
-    w[e] = q ? verify_rest(pv[e], qv[e]) : pw[e];
-  }
-  for (int i = 0; i < nstruck; i++) {
-    const int t = list[i] - v;
-#pragma unroll
-    for (int e = 0; e < 4; e++) w[e] = t == e ? 0.0 : w[e];
-  }
-}
+// A lane's 16 elements of a part of the row: v + STEP j + e (j, e < 4), 0 past `last`.  All loads are issued before
+// any of them is used; weights that are no finite positive number are 0.
+template <int STEP>
+struct VerifyRow {
+  float p[16], q[16];
 
-__device__ __forceinline__ double shfl_up_f64(double v, int by) {
+  __device__ __forceinline__ void load(const float* prow, const float* qrow, int v, bool whole, int last) {
+    get(prow, v, whole, last, p);
+    if (qrow) get(qrow, v, whole, last, q);
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      p[i] = p[i] > 0.f && p[i] < __builtin_inff() ? p[i] : 0.f;
+      q[i] = qrow && q[i] > 0.f ? q[i] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void strike(int v, int n, const int* list) {
+    for (int i = 0; i < n; i++) {
+      const int t = list[i] - v;
+#pragma unroll
+      for (int j = 0; j < 16; j++) p[j] = t == STEP * (j / 4) + (j & 3) ? 0.f : p[j];
+    }
+  }
+  __device__ __forceinline__ double rest(int i) const {
+    const double d = (double)p[i] - (double)q[i];
+    return d > 0.0 ? d : 0.0;
+  }
+
+ private:
+  __device__ __forceinline__ static void get(const float* row, int v, bool whole, int last, float x[16]) {
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const verify_f4_t r = *reinterpret_cast<const verify_f4_t*>(row + v + STEP * j);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[4 * j + e] = r[e];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        const int i = v + STEP * (j / 4) + (j & 3);
+        x[j] = i < last ? row[i] : 0.f;
+      }
+    }
+  }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v) {  // 0 where no lane feeds
   const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
-  const unsigned lo = __shfl_up((unsigned)u, by), hi = __shfl_up((unsigned)(u >> 32), by);
-  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
-}
-__device__ __forceinline__ double shfl_f64(double v, int from) {
-  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
-  const unsigned lo = __shfl((unsigned)u, from), hi = __shfl((unsigned)(u >> 32), from);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, ROWS, 0xF, ROWS == 0xF);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, ROWS, 0xF, ROWS == 0xF);
   return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 __device__ __forceinline__ double wave_scan_f64(double v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double o = shfl_up_f64(v, m);
-    v += lane >= m ? o : 0.0;
-  }
+  v += dpp_f64<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8: inside each row of 16
+  v += dpp_f64<0x112, 0xF>(v);
+  v += dpp_f64<0x114, 0xF>(v);
+  v += dpp_f64<0x118, 0xF>(v);
+  v += dpp_f64<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_f64<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ double lane_f64(double v, int from) {  // from: wave-uniform
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)u, from);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(u >> 32), from);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
 
-__global__ __launch_bounds__(kMassThreads) void verify_mass_kernel(const VerifyArgs a) {
+__global__ __launch_bounds__(kMassThreads) void verify_mass_kernel(const VerifyArgs a, int each) {
   __shared__ VerifyEnd end;
   __shared__ int list[kVerifyNodes], nlist;
-  __shared__ double sums[kMassThreads / 64][2];
-  const int b = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int first = chunk * a.chunk_len, last = min(first + a.chunk_len, a.vocab);
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part0 = blockIdx.x * kMassWaves * each, part1 = min(part0 + kMassWaves * each, a.parts);
   if (wave == 0) {
     const VerifyWalk w = verify_walk(a, b);
-    const int n = struck_in(w.end.struck, w.token, first, last, list);
+    const int n = struck_in(w.end.struck, w.token, part0 * kVerifyPart, min(part1 * kVerifyPart, a.vocab), list);
     if (lane == 0) end = w.end, nlist = n;
-    if (chunk == 0) {
+    if (blockIdx.x == 0) {
       const size_t at = (size_t)b * a.nodes;
       if (w.path >> lane & 1) {
         const int place = __builtin_popcountll(w.path & ((1ull << lane) - 1));
@@ -211,102 +218,109 @@ __global__ __launch_bounds__(kMassThreads) void verify_mass_kernel(const VerifyA
   if (e.count == 0) return;
   const size_t row = ((size_t)b * a.nodes + e.node) * a.vocab;
   const float *p = a.p + row, *q = e.residual ? a.q + row : nullptr;
-  double sw = 0.0, sp = 0.0;
-#pragma unroll 4
-  for (int v = first + 4 * threadIdx.x; v < last; v += 4 * kMassThreads) {
-    double w[4], pw[4];
-    verify_load(p, q, v, last, nlist, list, w, pw);
-    sw += (w[0] + w[1]) + (w[2] + w[3]);
-    sp += (pw[0] + pw[1]) + (pw[2] + pw[3]);
-  }
-  sw = wave_scan_f64(sw), sp = wave_scan_f64(sp);
-  if (lane == 63) sums[wave][0] = sw, sums[wave][1] = sp;
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double t = 0.0;
+  for (int part = part0 + wave; part < part1; part += kMassWaves) {
+    const int first = part * kVerifyPart, last = min(first + kVerifyPart, a.vocab);
+    VerifyRow<256> r;
+    r.load(p, q, first + 4 * lane, first + kVerifyPart <= last, last);
+    double sw = 0.0, sp = 0.0;
 #pragma unroll
-    for (int i = 0; i < kMassThreads / 64; i++) t += sums[i][threadIdx.x];
-    a.mass[((size_t)b * a.chunks + chunk) * 2 + threadIdx.x] = t;
+    for (int i = 0; i < 16; i++) sp += (double)r.p[i];
+    if (q) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) sw += r.rest(i);
+    } else if (nlist) {
+      r.strike(first + 4 * lane, nlist, list);
+#pragma unroll
+      for (int i = 0; i < 16; i++) sw += (double)r.p[i];
+    } else {
+      sw = sp;
+    }
+    sw = wave_scan_f64(sw), sp = wave_scan_f64(sp);
+    if (lane == 63) {
+      double* to = a.mass + ((size_t)b * a.parts + part) * 2;
+      to[0] = sw, to[1] = sp;
+    }
   }
 }
 
-__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(const VerifyArgs a) {
-  constexpr int WAVES = kPickThreads / 64;
-  __shared__ int list[kVerifyNodes], nlist, picked, fallback;
-  __shared__ double wave_sum[WAVES];
-  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// One wave per sequence: from the parts' sums, a run of parts per lane, to a run, to its part, to its element
+__global__ __launch_bounds__(64) void verify_pick_kernel(const VerifyArgs a) {
+  __shared__ int list[kVerifyNodes];
+  const int b = blockIdx.x, lane = threadIdx.x;
   const VerifyEnd e = a.end[b];
+  const float u = a.uniform[(size_t)b * a.nodes];
+  const int token = a.tokens[(size_t)b * a.nodes + min(lane, a.nodes - 1)];
   if (e.count == 0) return;
-  // every wave: the chunk that the threshold falls in
-  const double* mass = a.mass + (size_t)b * a.chunks * 2;
-  const double mw = lane < a.chunks ? mass[2 * lane] : 0.0, mp = lane < a.chunks ? mass[2 * lane + 1] : 0.0;
-  double run = wave_scan_f64(mw);
-  const bool plain = !(shfl_f64(run, 63) > 0.0);  // nothing left of w: the target's row as it is
-  const double mine = plain ? mp : mw;
-  if (plain) run = wave_scan_f64(mp);
-  const double total = shfl_f64(run, 63);
+  const double* mass = a.mass + (size_t)b * a.parts * 2;
+  const int run = (a.parts + 63) / 64, run0 = lane * run, run1 = min(run0 + run, a.parts);
+  double mw = 0.0, mp = 0.0;
+  for (int i = run0; i < run1; i++) mw += mass[2 * i], mp += mass[2 * i + 1];
+  double scan = wave_scan_f64(mw);
+  const bool plain = !(lane_f64(scan, 63) > 0.0);  // nothing left of w: the target's row as it is
+  double mine = plain ? mp : mw;
+  if (plain) scan = wave_scan_f64(mp);
+  const double total = lane_f64(scan, 63);
   int next = -1;
   if (total > 0.0) {
-    const float u = a.uniform[(size_t)b * a.nodes];
     const double bar = (u > 0.f ? (double)fminf(u, 1.f) : 0.0) * total;
-    unsigned long long over = __builtin_amdgcn_ballot_w64(run > bar);
-    if (!over) over = 1ull << (63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(mine > 0.0)));  // u = 1: the last
-    const int chunk = __builtin_ctzll(over);
-    double base = shfl_f64(run, max(chunk - 1, 0));
-    base = chunk > 0 ? base : 0.0;
-    const int first = chunk * a.chunk_len, last = min(first + a.chunk_len, a.vocab);
-    if (wave == 0) {
-      const int token = a.tokens[(size_t)b * a.nodes + min(lane, a.nodes - 1)];
-      const int n = struck_in(plain ? 0 : e.struck, token, first, last, list);
-      if (lane == 0) nlist = n, picked = 0x7FFFFFFF, fallback = -1;
+    // where the scan first passes the threshold; rounding may leave that to nobody, then it is the last with any weight
+    auto passes = [&](double scan, double mine) {
+      const unsigned long long over = __builtin_amdgcn_ballot_w64(scan > bar && mine > 0.0);
+      return over ? __builtin_ctzll(over) : 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(mine > 0.0) | 1);
+    };
+    int at = passes(scan, mine);
+    double base = at > 0 ? lane_f64(scan, at - 1) : 0.0;
+    const int from = at * run, to = min(from + run, a.parts);
+    int part = from;
+    for (int i0 = from; i0 < to; i0 += 64) {
+      const int i = i0 + lane;
+      mine = i < to ? mass[2 * i + plain] : 0.0;
+      if (!__builtin_amdgcn_ballot_w64(mine > 0.0)) continue;
+      scan = base + wave_scan_f64(mine);
+      const int l = passes(scan, mine);
+      part = i0 + l;
+      if (lane_f64(scan, l) > bar || i0 + 64 >= to) {
+        base = l > 0 ? lane_f64(scan, l - 1) : base;
+        break;
+      }
+      base = lane_f64(scan, 63);
     }
+    const int first = part * kVerifyPart, last = min(first + kVerifyPart, a.vocab);
+    const int n = struck_in(plain ? 0 : e.struck, token, first, last, list);
     __syncthreads();
     const size_t row = ((size_t)b * a.nodes + e.node) * a.vocab;
     const float *p = a.p + row, *q = e.residual && !plain ? a.q + row : nullptr;
-    for (int at = first; at < last; at += kVerifyBlock) {
-      const int v = at + 4 * threadIdx.x;
-      double w[4] = {0.0, 0.0, 0.0, 0.0}, pw[4];
-      if (v < last) verify_load(p, q, v, last, nlist, list, w, pw);
-      const double sum = (w[0] + w[1]) + (w[2] + w[3]);
-      const double scan = wave_scan_f64(sum);
-      if (lane == 63) wave_sum[wave] = scan;
-      __syncthreads();
-      double before = base;
+    const int v = first + 16 * lane;
+    VerifyRow<4> r;
+    r.load(p, q, v, first + kVerifyPart <= last, last);
+    r.strike(v, n, list);
+    double w[16], sum = 0.0;
 #pragma unroll
-      for (int i = 0; i < WAVES; i++) {
-        before += i < wave ? wave_sum[i] : 0.0;
-        base += wave_sum[i];
-      }
-      double c = before + (scan - sum);
-      int found = 0x7FFFFFFF, positive = -1;
+    for (int i = 0; i < 16; i++) w[i] = r.rest(i), sum += w[i];
+    scan = base + wave_scan_f64(sum);
+    double c = scan - sum;
+    int found = -1, positive = -1;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        c += w[i];
-        if (w[i] > 0.0) {
-          positive = v + i;
-          if (c > bar) found = min(found, v + i);
-        }
+    for (int i = 0; i < 16; i++) {
+      c += w[i];
+      if (w[i] > 0.0) {
+        positive = v + i;
+        if (c > bar && found < 0) found = v + i;
       }
-      if (found != 0x7FFFFFFF) atomicMin(&picked, found);
-      if (positive >= 0) atomicMax(&fallback, positive);
-      __syncthreads();
-      if (picked != 0x7FFFFFFF) break;
     }
-    next = picked != 0x7FFFFFFF ? picked : fallback;
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(found >= 0);
+    const unsigned long long any = __builtin_amdgcn_ballot_w64(positive >= 0);
+    if (hit)
+      next = __builtin_amdgcn_readlane(found, __builtin_ctzll(hit));
+    else if (any)
+      next = __builtin_amdgcn_readlane(positive, 63 - __builtin_clzll(any));
   }
-  if (threadIdx.x == 0) a.out_tokens[(size_t)b * a.nodes + e.count - 1] = next;
+  if (lane == 0) a.out_tokens[(size_t)b * a.nodes + e.count - 1] = next;
 }
 
-struct VerifyPlan {
-  int chunks, chunk_len;
-  size_t bytes;
-};
-static VerifyPlan verify_plan(int batch, int vocab) {
-  const int blocks = (vocab + kVerifyBlock - 1) / kVerifyBlock;
-  const int each = (blocks + kVerifyChunks - 1) / kVerifyChunks;
-  const int chunks = (blocks + each - 1) / each;
-  return VerifyPlan{chunks, each * kVerifyBlock,
-                    (size_t)batch * (chunks * 2 * sizeof(double) + sizeof(VerifyEnd))};
+static int verify_parts(int vocab) { return (vocab + kVerifyPart - 1) / kVerifyPart; }
+static size_t verify_bytes(int batch, int vocab) {
+  return (size_t)batch * (verify_parts(vocab) * 2 * sizeof(double) + sizeof(VerifyEnd));
 }
 
 }  // namespace exl3
@@ -315,7 +329,7 @@ using namespace exl3;
 
 extern "C" size_t exl3_verify_workspace_bytes(int batch, int vocab) {
   if (batch <= 0 || vocab <= 0 || vocab > (1 << 28)) return 0;
-  return verify_plan(batch, vocab).bytes;
+  return verify_bytes(batch, vocab);
 }
 
 extern "C" int exl3_verify_drafts(const float* target_probs, const float* draft_probs, const int* tokens,
@@ -329,16 +343,21 @@ extern "C" int exl3_verify_drafts(const float* target_probs, const float* draft_
   if (batch == 0) return EXL3_OK;
   EXL3_CHECK_ARG(target_probs && tokens && uniform && accepted_nodes && counts && out_tokens,
                  "exl3_verify_drafts: null pointer");
-  const VerifyPlan plan = verify_plan(batch, vocab);
-  EXL3_CHECK_ARG(workspace && workspace_bytes >= plan.bytes && ((uintptr_t)workspace & 7) == 0,
-                 "exl3_verify_drafts: workspace %zu bytes, need %zu (8-byte aligned)", workspace_bytes, plan.bytes);
+  const size_t need = verify_bytes(batch, vocab);
+  EXL3_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 7) == 0,
+                 "exl3_verify_drafts: workspace %zu bytes, need %zu (8-byte aligned)", workspace_bytes, need);
   double* mass = static_cast<double*>(workspace);
-  const VerifyArgs a{target_probs, draft_probs, tokens, parents, uniform, num_nodes, nodes, vocab, plan.chunks,
-                     plan.chunk_len, accepted_nodes, counts, out_tokens, mass,
-                     reinterpret_cast<VerifyEnd*>(mass + (size_t)batch * plan.chunks * 2)};
-  verify_mass_kernel<<<dim3(plan.chunks, batch), kMassThreads, 0, as_stream(stream)>>>(a);
+  const int parts = verify_parts(vocab);
+  const VerifyArgs a{target_probs, draft_probs, tokens, parents, uniform, num_nodes, nodes, vocab, parts,
+                     accepted_nodes, counts, out_tokens, mass,
+                     reinterpret_cast<VerifyEnd*>(mass + (size_t)batch * parts * 2)};
+  // parts per wave: at 64 rows of 131072 the sums take 9.7 / 8.8 / 9.6 us at 1 / 2 / 4, at one row of 32003
+  // 4.2 / 5.0 / 6.9 us
+  const int each = (long long)batch * parts > 4096 ? 2 : 1;
+  verify_mass_kernel<<<dim3((parts + kMassWaves * each - 1) / (kMassWaves * each), batch), kMassThreads, 0,
+                       as_stream(stream)>>>(a, each);
   EXL3_CHECK_LAUNCH();
-  verify_pick_kernel<<<batch, kPickThreads, 0, as_stream(stream)>>>(a);
+  verify_pick_kernel<<<batch, 64, 0, as_stream(stream)>>>(a);
   EXL3_CHECK_LAUNCH();
   return EXL3_OK;
 }
