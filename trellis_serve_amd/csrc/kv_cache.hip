@@ -6,16 +6,14 @@
 //   s = c when the page's first slot is among them, else max(the page's scale, c)
 //   older codes, when s grew:  code' = rint(code * s_old / s)          (at most half a step of s per growth)
 //   new codes:  min(max(rint(x / s), -qmax), qmax), NaN as 0            (at most half a step off: s * qmax >= a)
-// Quotients are IEEE divisions: x and s have 11 bits each, so a correctly rounded fp32 quotient falls on a half-way point
-// only when the exact one does, and codes are those of exact arithmetic.
+// x and s have 11 bits each, so a correctly rounded fp32 quotient falls on a half-way point only when the exact one does,
+// and codes are those of exact arithmetic.
 // One wave per (page, kv head, keys or values): 16 slots x 128 values are four 16-byte loads per lane, the maximum one
 // wave reduction, and nobody else writes the page, so the launch needs no synchronisation.  Bound by memory at many
 // tokens; a decode step is a few dependent loads (length, page id, scale) long.
 //
 // kv_gather_kernel.  out = code * scale, rounded once, for rows of consecutive tokens.  A workgroup first finds its rows'
 // pages (one thread a row), then copies 8 codes per lane and step: 128-byte (64) code rows in, 256-byte rows out.
-#include <float.h>
-
 #include <algorithm>
 
 #include "exl3_api.hpp"
@@ -42,18 +40,30 @@ struct KvAppendArgs {
 };
 
 template <bool BF16>
-__device__ __forceinline__ void kv_unpack8(kv_u32x4_t r, float v[8]) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if constexpr (BF16) {
-      v[2 * i] = __builtin_bit_cast(float, r[i] << 16);
-      v[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xFFFF0000u);
-    } else {
-      const uint32_t u = r[i];  // a value of its own: the bit cast of a vector's element takes element 0
-      const half2_t h = __builtin_bit_cast(half2_t, u);
-      v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
-    }
+__device__ __forceinline__ float kv_half(uint32_t pair, int e) {  // half e (0, 1) of a pair
+  if constexpr (BF16) {
+    return __builtin_bit_cast(float, e ? pair & 0xFFFF0000u : pair << 16);
+  } else {
+    const half2_t h = __builtin_bit_cast(half2_t, pair);
+    return (float)h[e];
   }
+}
+
+typedef uint16_t kv_u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(kv_u16x2_t, a),
+                                                                __builtin_bit_cast(kv_u16x2_t, b)));
+}
+template <int ROR>
+__device__ __forceinline__ uint32_t max_ror(uint32_t v) {  // with the lane ROR places off in its row of 16
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + ROR, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = max_ror<1>(max_ror<2>(max_ror<4>(max_ror<8>(v))));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(max(b[0], b[1]));
 }
 
 // the smallest fp16 >= a / qmax (a finite, >= 0), the largest finite fp16 past its range
@@ -69,6 +79,15 @@ __device__ __forceinline__ int kv_code(float x, float s) {
   constexpr float Q = BITS == 8 ? 127.f : 7.f;
   const float r = __builtin_rintf(x / s);
   return r == r ? (int)fminf(fmaxf(r, -Q), Q) : 0;  // NaN: a NaN value, or 0 / 0 in an all-zero page
+}
+
+// x / s for finite |x| <= 127 s, r = 1 / s correctly rounded, as the low bits of a float: rint in two's complement.
+// The residual of x r is exact, so a half-way quotient comes out as itself; any other is a part of 2^-19 away from
+// half-way, more than the quotient's error.
+__device__ __forceinline__ uint32_t kv_code_bits(float x, float s, float r) {
+  const float y = x * r;
+  const float q = __builtin_fmaf(__builtin_fmaf(-y, s, x), r, y);
+  return __builtin_bit_cast(uint32_t, q + 12582912.f);  // 1.5 * 2^23: the unit is the last place
 }
 
 template <int BITS, bool XB>
@@ -98,13 +117,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a) {
   const int lp = len / kPage + pg, first = lp * kPage;  // logical page, its first token
   if (first >= len + count) return;
   const int page = a.page_table[(size_t)b * a.max_pages + lp];
-  if (page < 0 || page >= a.num_pages) return;
 
   const uint16_t* x = is_v ? a.v : a.k;
   const long long ld = is_v ? a.ld_v : a.ld_k;
-  float val[4][8];
+  constexpr uint32_t INF = XB ? 0x7F80 : 0x7C00;
+  kv_u32x4_t raw[4];
   bool live[4];
-  float most = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const int token = first + 4 * i + g - len;  // of the new ones
@@ -115,19 +133,30 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a) {
       src = r0 + node;
       live[i] = node >= 0 && node < avail && src >= 0 && src < a.rows;
     }
-#pragma unroll
-    for (int e = 0; e < 8; e++) val[i][e] = 0.f;
-    if (live[i])
-      kv_unpack8<XB>(*reinterpret_cast<const kv_u32x4_t*>(x + src * ld + hk * kHeadDim + 8 * n), val[i]);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float v = fabsf(val[i][e]);
-      most = v <= FLT_MAX ? fmaxf(most, v) : most;
-    }
+    raw[i] = kv_u32x4_t{0, 0, 0, 0};
+    if (live[i]) raw[i] = *reinterpret_cast<const kv_u32x4_t*>(x + src * ld + hk * kHeadDim + 8 * n);
   }
+  if (page < 0 || page >= a.num_pages) return;
   if (!__builtin_amdgcn_ballot_w64(live[0] || live[1] || live[2] || live[3])) return;
+  // magnitudes of halves order as integers
+  uint32_t pairs = 0;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) pairs = max_u16x2(pairs, raw[i][e] & 0x7FFF7FFFu);
+  const uint32_t largest = wave_max_u32(max(pairs & 0xFFFFu, pairs >> 16));
+  float most = kv_half<XB>(largest, 0);
+  if (largest >= INF) {  // infinities and NaN take no part
+    uint32_t finite = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t lo = raw[i][e] & 0x7FFFu, hi = raw[i][e] >> 16 & 0x7FFFu;
+        finite = max(finite, max(lo < INF ? lo : 0, hi < INF ? hi : 0));
+      }
+    most = kv_half<XB>(wave_max_u32(finite), 0);
+  }
 
   const size_t block = (size_t)page * a.Hkv + hk;
   uint16_t* scale = (is_v ? a.v_scale : a.k_scale) + block;
@@ -168,23 +197,35 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a) {
   }
   const float s = (float)__builtin_bit_cast(_Float16, bits);
   if (lane == 0) *scale = bits;
+  // infinities, NaN, a scale that stopped at fp16's largest, 0 / 0: with their limits, else without
+  const bool plain = __builtin_amdgcn_readfirstlane(largest < INF && most <= s * Q && s > 0.f);
+  const float r = 1.f / s;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     if (!live[i]) continue;
+    uint32_t code[8];
+    if (plain) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) code[e] = kv_code_bits(kv_half<XB>(raw[i][e / 2], e & 1), s, r);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) code[e] = (uint32_t)kv_code<BITS>(kv_half<XB>(raw[i][e / 2], e & 1), s);
+    }
     uint32_t* p = reinterpret_cast<uint32_t*>(codes + (4 * i + g) * ROW);
     if constexpr (BITS == 8) {
-      uint32_t lo = 0, hi = 0;
+      kv_u32x2_t o;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        lo |= (uint32_t)(kv_code<8>(val[i][e], s) & 0xFF) << (8 * e);
-        hi |= (uint32_t)(kv_code<8>(val[i][4 + e], s) & 0xFF) << (8 * e);
+      for (int d = 0; d < 2; d++) {  // the low bytes of four
+        const uint32_t lo = __builtin_amdgcn_perm(code[4 * d + 1], code[4 * d], 0x0C0C0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(code[4 * d + 3], code[4 * d + 2], 0x04000C0Cu);
+        o[d] = lo | hi;
       }
-      *reinterpret_cast<kv_u32x2_t*>(p) = kv_u32x2_t{lo, hi};
+      *reinterpret_cast<kv_u32x2_t*>(p) = o;
     } else {
-      uint32_t r = 0;
+      uint32_t o = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) r |= (uint32_t)(kv_code<4>(val[i][e], s) & 0xF) << (4 * e);
-      *p = r;
+      for (int e = 0; e < 8; e++) o |= (code[e] & 0xF) << (4 * e);
+      *p = o;
     }
   }
 }
