@@ -310,6 +310,25 @@ def test_kv_tree_attention(bits, lens, N, Hq, Hkv, how):
     _check_tree(got, q, k, v, seen, cache, table, lens, bits)
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("lens,copies,N,Hq", [
+    ([9001, 1, 8300], 300, 3, 2), ([9001, 130, 8192], 160, 6, 6), ([8999, 0, 9000], 110, 16, 6),
+    ([1601, 17, 1024], 200, 25, 4), ([2100, 1025, 0], 120, 32, 8), ([1500, 33, 1111], 150, 64, 5),
+    ([1300, 64, 5], 120, 64, 8)])
+def test_kv_tree_attention_long_runs(bits, lens, copies, N, Hq):
+    """Many sequences over the same pages: each workgroup goes through thousands of tokens of several of them."""
+    q, k, v, seen, cache, table = _tree_case(copies + bits, lens, N, Hq, 1, bits, "tree")
+    many = torch.arange(len(lens) * copies) % len(lens)
+    got = _ops().kv_tree_attention(*(t[many.to(t.device)].contiguous() for t in (q, k, v, _t(_masks(seen)))),
+                                   *[_t(c) for c in cache], _t(table)[many.to(q.device)].contiguous(),
+                                   _t(np.int32(lens))[many.to(q.device)].contiguous(), bits)
+    assert not torch.isnan(got).any()
+    got = got.unflatten(0, (copies, len(lens)))
+    lo, hi = got.float().amin(0), got.float().amax(0)
+    for end in (lo, hi):   # the smallest and largest of a value's copies are within its tolerance, so all are
+        _check_tree(end, q, k, v, seen, cache, table, lens, bits)
+
+
 @pytest.mark.parametrize("lens,N,Hq,Hkv", [([64, 0, 500, 7, 90], 16, 10, 2), ([30, 200, 0], 64, 5, 1), ([100, 100], 1, 4, 4)])
 def test_kv_tree_attention_ragged_nodes(lens, N, Hq, Hkv):
     """num_nodes 0, 1, .. N: the rest of a sequence is neither written nor read (its K and V hold NaN)."""

@@ -67,6 +67,7 @@ struct KvTreeArgs {
 // 123 us with 2, 108.5 with 6; 16 nodes 52.6 and 51.1, this kernel 56 without any and 45).
 struct TreeRuns {
   int extra, total, count, per, longer;  // the first `longer` runs are one step longer
+  int len0, nodes0, units0;              // of sequence `lane` (KEPT: for tree_find, for 3 registers)
 
   __device__ __forceinline__ explicit TreeRuns(const KvTreeArgs& a) {
     const int lane = threadIdx.x & 63;
@@ -74,6 +75,7 @@ struct TreeRuns {
     for (int base = 0; base < a.batch; base += 64) {
       int len, nodes;
       const int u = units_of(a, base + lane, len, nodes);
+      if (base == 0) len0 = len, nodes0 = nodes, units0 = u;
       units += wave_total(u);
       steps += wave_total(u * steps_of(a, len));
     }
@@ -114,13 +116,14 @@ __device__ __forceinline__ TreeUnit tree_unit(const KvTreeArgs& a, const TreeRun
 }
 
 // The sequence that `found(first, end)` picks by its first step and the one after its last, among the lanes' sequences
-template <typename Found>
+template <bool KEPT, typename Found>
 __device__ __forceinline__ TreeUnit tree_find(const KvTreeArgs& a, const TreeRuns& runs, Found found) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int base = 0;; base += 64) {
-    int len, nodes;
-    const int mine = runs.units_of(a, base + lane, len, nodes) * (runs.steps_of(a, len) + runs.extra);
+    int len = runs.len0, nodes = runs.nodes0;
+    const int units = !KEPT || base > 0 ? runs.units_of(a, base + lane, len, nodes) : runs.units0;
+    const int mine = units * (runs.steps_of(a, len) + runs.extra);
     const int upto = before + wave_scan(mine);
     const unsigned long long hit = __builtin_amdgcn_ballot_w64(found(base + lane, upto));
     if (hit || base + 64 >= a.batch) {
@@ -132,8 +135,9 @@ __device__ __forceinline__ TreeUnit tree_find(const KvTreeArgs& a, const TreeRun
   }
 }
 // ... the one that step s (below the total) belongs to
+template <bool KEPT>
 __device__ __forceinline__ TreeUnit tree_at_step(const KvTreeArgs& a, const TreeRuns& runs, int s) {
-  return tree_find(a, runs, [&](int, int end) { return end > s; });
+  return tree_find<KEPT>(a, runs, [&](int, int end) { return end > s; });
 }
 
 // The state of RG groups of 16 rows in a wave: lane (n, g) = (l % 16, l / 16) holds row n of each group
@@ -164,6 +168,27 @@ struct TreeRows {
 #pragma unroll
       for (int c = 0; c < 4; c++) q[gi][c] = *reinterpret_cast<const half8_t*>(p + 8 * c);
     }
+  }
+  // The same by a workgroup of 4 waves: wave w brings rows 4 w .. 4 w + 3 of each group into LDS, one 256-byte row per 16
+  // lanes, piece p (8 dims) of row r at place p ^ r.  Each wave loading its own fragments takes four times as many loads,
+  // of 16 bytes from 64 places each.
+  using Staging = half8_t[RG][16][16];
+  static __device__ __forceinline__ void stage_queries(const KvTreeArgs& a, const TreeUnit& u, int hk, int row0, int w,
+                                                       int lane, Staging& to) {
+    const int rr = 4 * w + (lane >> 4), piece = (lane & 15) ^ rr;
+#pragma unroll
+    for (int gi = 0; gi < RG; gi++) {
+      const int r = min(row0 + 16 * gi + rr, u.nodes * a.G - 1), node = r / a.G;
+      const _Float16* p = a.q + ((size_t)u.b * a.nodes + node) * a.ld_q + (hk * a.G + r - node * a.G) * kHeadDim + 8 * piece;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                       (__attribute__((address_space(3))) void*)to[gi][4 * w], 16, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void read_queries(const Staging& from, int n, int g) {
+#pragma unroll
+    for (int gi = 0; gi < RG; gi++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) q[gi][c] = from[gi][n][(4 * g + c) ^ n];
   }
   __device__ __forceinline__ void start() {
 #pragma unroll
@@ -551,13 +576,14 @@ __global__ __launch_bounds__(64 * kSplitWaves, RG <= 2 ? 2 : 1) void kv_tree_spl
       float ml[ROUND][W][16][2];
     } red;
   } sh;
+  __shared__ typename Rows::Staging sh_q;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wg = blockIdx.x;
   const TreeRuns runs(a);
   if (wg >= runs.count) return;
   const int s_end = runs.start(wg + 1);
   for (int s = runs.start(wg); s < s_end;) {
-    const TreeUnit u = tree_at_step(a, runs, s);
+    const TreeUnit u = tree_at_step<true>(a, runs, s);
     const TreePart p(a, u, runs.extra, s, s_end);
     // Lane i holds, for cache step cb + i, the wave's two pages
     const int* ptab = a.page_table + (size_t)u.b * a.max_pages;
@@ -581,21 +607,24 @@ __global__ __launch_bounds__(64 * kSplitWaves, RG <= 2 ? 2 : 1) void kv_tree_spl
       St::load_block(a.vc + ba * St::BLOCK, st + 2 * St::BLOCK, source);
       St::load_block(a.vc + bb * St::BLOCK, st + 3 * St::BLOCK, source);
     };
-    // Loads in the order of their use, each behind the ones it depends on: page ids, queries and nodes, then the first
-    // pages and their scales; the queries' and nodes' work runs while those come in.
+    // Page ids, queries and nodes first, then the scales and the first pages; the queries' and nodes' work runs while
+    // those come in.
     Rows x;
     const bool nodes_here = p.t0 == 0 && 16 * w < u.nodes;
     typename Rows::Nodes nodes;
     if (p.c0 < p.c1) load_ids();
-    x.load_queries(a, u, p.hk, p.row0, n, g);
+    Rows::stage_queries(a, u, p.hk, p.row0, w, lane, sh_q);
     if (nodes_here) nodes.load(a, u, p.hk, w, p.row0, n, g);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     issue_fence();
     if (p.c0 < p.c1) {
+      A.load(a, ida, p.hk), B.load(a, idb, p.hk);
+      issue_fence();
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) issue(p.c0 + i);
-      A.load(a, ida, p.hk), B.load(a, idb, p.hk);
     }
-    issue_fence();
+    lds_barrier();  // all rows of the queries are in
+    x.read_queries(sh_q, n, g);
     x.start();
     if (nodes_here) x.process_nodes(a, u, p.hk, w, nodes, lane);
     if (p.c0 < p.c1) A.use(a.qk_scale), B.use(a.qk_scale);
@@ -899,7 +928,7 @@ __global__ __launch_bounds__(64 * kSharedSlots, 2) void kv_tree_shared_kernel(co
   if (wg >= runs.count) return;
   const int s_end = runs.start(wg + 1);
   for (int s = runs.start(wg); s < s_end;) {
-    const TreeUnit u = tree_at_step(a, runs, s);
+    const TreeUnit u = tree_at_step<false>(a, runs, s);
     const TreePart p(a, u, runs.extra, s, s_end);
     // the unit's groups of rows, dealt evenly: wave w and wave w + 4 share a SIMD
     const int groups = (min(p.rows - p.row0, a.tile) + 15) / 16;
@@ -927,7 +956,7 @@ __global__ __launch_bounds__(64 * kTreeMergeWaves) void kv_tree_merge_kernel(con
   const TreeRuns runs(a);
   const int b = blockIdx.z, unit = blockIdx.y;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const TreeUnit u = tree_find(a, runs, [&](int at, int) { return at == b; });
+  const TreeUnit u = tree_find<true>(a, runs, [&](int at, int) { return at == b; });
   const int rows = u.nodes * a.G, tiles = (rows + a.tile - 1) / a.tile;
   if (unit >= a.Hkv * tiles) return;
   const int first = w % SPLIT, group = w / SPLIT;  // of the parts, and the wave's 4 rows
