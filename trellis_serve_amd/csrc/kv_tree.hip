@@ -38,6 +38,7 @@ constexpr int kSharedSlots = 8;       // shared: waves; each takes rows, and all
 constexpr int kSharedPages = 4;       // pages per step
 constexpr int kSharedGroups = 3;      // most groups of 16 rows per wave
 constexpr int kSplitGroups = 6;
+constexpr int kPairedGroups = 2;      // split: up to as many, two workgroups share a CU
 constexpr int kTreeExtra = 6;         // most steps that the beginning of a unit counts for
 constexpr float kTreeBar = 4.f;       // exponents above it move a row's reference
 constexpr float kTreeLow = -1e30f;    // below any logit, finite: differences of empty states are 0, not NaN
@@ -166,7 +167,7 @@ struct TreeRows {
       const int r = min(row0 + 16 * gi + n, u.nodes * a.G - 1), node = r / a.G;
       const _Float16* p = a.q + ((size_t)u.b * a.nodes + node) * a.ld_q + (hk * a.G + r - node * a.G) * kHeadDim + 32 * g;
 #pragma unroll
-      for (int c = 0; c < 4; c++) q[gi][c] = *reinterpret_cast<const half8_t*>(p + 8 * c);
+      for (int c = 0; c < 4; c++) q[gi][c] = in_key_order(*reinterpret_cast<const half8_t*>(p + 8 * c));
     }
   }
   // The same by a workgroup of 4 waves: wave w brings rows 4 w .. 4 w + 3 of each group into LDS, one 256-byte row per 16
@@ -182,6 +183,16 @@ struct TreeRows {
       const _Float16* p = a.q + ((size_t)u.b * a.nodes + node) * a.ld_q + (hk * a.G + r - node * a.G) * kHeadDim + 8 * piece;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
                                        (__attribute__((address_space(3))) void*)to[gi][4 * w], 16, 0, 0);
+    }
+  }
+  // ... in the order of the key fragments, each wave its own pieces
+  static __device__ __forceinline__ void order_queries(int w, int lane, Staging& q) {
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int gi = 0; gi < RG; gi++) {
+        half8_t& h = q[gi][4 * w + (lane >> 4)][lane & 15];
+        h = in_key_order(h);
+      }
     }
   }
   __device__ __forceinline__ void read_queries(const Staging& from, int n, int g) {
@@ -202,7 +213,6 @@ struct TreeRows {
           const uint32_t two = w[e];
           part = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, two), half2_t{(_Float16)1.f, (_Float16)1.f}, part, false);
         }
-        q[gi][c] = in_key_order(q[gi][c]);
       }
       qsum[gi] = -kBias * sum_over_groups(part);
       m[gi] = 0.f, l[gi] = 0.f, bar[gi] = -INFINITY;
@@ -563,12 +573,15 @@ struct Staged {
 };
 
 template <int BITS, int RG>
-__global__ __launch_bounds__(64 * kSplitWaves, RG <= 2 ? 2 : 1) void kv_tree_split_kernel(const KvTreeArgs a) {
+__global__ __launch_bounds__(64 * kSplitWaves, RG <= kPairedGroups ? 2 : 1) void kv_tree_split_kernel(const KvTreeArgs a) {
   using Rows = TreeRows<BITS, RG>;
   using St = Staged<BITS>;
   // A stage holds a step of a wave: the keys of two pages, then their values.  Two workgroups share a CU's LDS up to 32 rows.
-  constexpr int W = kSplitWaves, STAGES = (RG <= 2 ? 2 : 4) * (BITS == 8 ? 1 : 2), AHEAD = STAGES - 1;
-  constexpr int ROUND = RG <= 2 ? 1 : 3;  // groups of rows merged at a time
+  constexpr int W = kSplitWaves, STAGES = (RG <= kPairedGroups ? 2 : 4) * (BITS == 8 ? 1 : 2), AHEAD = STAGES - 1;
+  // Queries stay in registers, but for 6 groups: with the accumulators they take more than a SIMD has, and are read from LDS
+  // a fragment ahead (19 nodes, 7 sequences up to 20000 tokens: 86 and 74 us; 16 nodes, 5 groups: 65 us either way)
+  constexpr bool QREG = RG <= 5;
+  constexpr int ROUND = RG <= kPairedGroups ? 1 : 3;  // groups of rows merged at a time
   __shared__ union {
     uint8_t stage[W][STAGES][4 * St::BLOCK];
     struct {
@@ -623,6 +636,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, RG <= 2 ? 2 : 1) void kv_tree_spl
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) issue(p.c0 + i);
     }
+    Rows::order_queries(w, lane, sh_q);
     lds_barrier();  // all rows of the queries are in
     x.read_queries(sh_q, n, g);
     x.start();
@@ -648,15 +662,27 @@ __global__ __launch_bounds__(64 * kSplitWaves, RG <= 2 ? 2 : 1) void kv_tree_spl
       half8_t pf[1][RG];
 #pragma unroll
       for (int gi = 0; gi < RG; gi++) sc[0][gi] = sc[1][gi] = float4_t{0.f, 0.f, 0.f, 0.f};
+      half8_t q[2][RG];  // QREG: not used
+      auto read_q = [&](int f) {
+#pragma unroll
+        for (int gi = 0; gi < RG; gi++) q[f & 1][gi] = sh_q[gi][n][(4 * g + f) ^ n];
+      };
+      if constexpr (!QREG) read_q(0);
 #pragma unroll
       for (int f = 0; f < 4; f++) {
+        if constexpr (!QREG) {  // a fragment ahead, and not where it is used
+          if (f < 3) read_q(f + 1);
+          issue_fence();
+        }
         const half8_t ka = ra.kfrag(f), kb = rb.kfrag(f);
 #pragma unroll
         for (int gi = 0; gi < RG; gi++) {
-          sc[0][gi] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, x.q[gi][f], sc[0][gi], 0, 0, 0);
-          sc[1][gi] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, x.q[gi][f], sc[1][gi], 0, 0, 0);
+          const half8_t qf = QREG ? x.q[gi][f] : q[f & 1][gi];
+          sc[0][gi] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf, sc[0][gi], 0, 0, 0);
+          sc[1][gi] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qf, sc[1][gi], 0, 0, 0);
         }
       }
+      if constexpr (!QREG) issue_fence();
       St::read_values(st + 2 * St::BLOCK, n, g, ra);
       St::read_values(st + 3 * St::BLOCK, n, g, rb);
       tree_softmax<BITS, RG, 2>(x, sc, A, &B, c - cb, (c * W + w) * 2 * kPage, u.len, g, pf);
@@ -1022,7 +1048,7 @@ static TreePlan tree_plan(int batch, int nodes, int num_q_heads, int num_kv_head
   p.tile = 16 * per_tile;
   p.step = p.shared ? kSharedPages : 2 * kSplitWaves;
   p.steps = (long long)batch * num_kv_heads * p.tiles * ((max_pages + p.step - 1) / p.step + 1 + kTreeExtra);
-  p.wgs = (int)std::min<long long>(!p.shared && p.rg <= 2 ? 512 : 256, p.steps);
+  p.wgs = (int)std::min<long long>(!p.shared && p.rg <= kPairedGroups ? 512 : 256, p.steps);
   return p;
 }
 
