@@ -219,3 +219,31 @@ def test_token_strides_of_views():
         assert ops._token_stride(t, "x", dims) == want
     with pytest.raises(ValueError, match="one stride"):
         ops._token_stride(wide[:, :3, :256].unflatten(2, (2, 128)), "x", 4)
+
+
+def test_outputs_that_overlap_are_refused():
+    x = torch.zeros(4 * 24 * 128, dtype=torch.float16)
+    q, k = x[: 4 * 16 * 128].view(4, 16, 128), x[4 * 16 * 128:].view(4, 8, 128)
+    cs, pos = torch.zeros(9, 128), torch.zeros(4, dtype=torch.int32)
+    shifted = torch.zeros(4 * 16 * 128 + 8, dtype=torch.float16)
+    q2 = shifted[: 4 * 16 * 128].view(4, 16, 128)
+    for a, b, out in ((q, k, (x[4 * 8 * 128:].view(4, 16, 128), torch.zeros_like(k))),      # q_out over k
+                      (q, k, (torch.zeros_like(q), x[: 4 * 8 * 128].view(4, 8, 128))),      # k_out over q
+                      (q2, k, (shifted[8:].view(4, 16, 128), torch.zeros_like(k)))):        # q_out 8 values into q
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.qk_norm_rope(a, b, None, None, cs, pos, out=out)
+    y = torch.zeros(2 * 5 * 16 * 128, dtype=torch.float16)
+    qt = y.view(2, 5, 16, 128)
+    kt = torch.zeros(2, 5, 2, 128, dtype=torch.float16)
+    cache = [torch.zeros(8, 2, 16, 128, dtype=torch.int8)] * 2 + [torch.zeros(8, 2, dtype=torch.float16)] * 2
+    table, lens = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.kv_tree_attention(qt, kt, kt, None, *cache, table, lens, 8, out=qt)
+    both = torch.zeros(3, 2, 128, dtype=torch.float16)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.kv_gather(*cache, table, lens, 8, torch.zeros(3, dtype=torch.int32), 3, out=(both, both))
+
+
+def test_wide_token_ids_do_not_wrap():
+    t = torch.tensor([[5, 2 ** 32 + 5, -2 ** 40, 99, 100, -1]])
+    assert ops._narrow(t, 100).tolist() == [[5, 100, -1, 99, 100, -1]] and ops._narrow(t, 100).dtype == torch.int32

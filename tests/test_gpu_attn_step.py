@@ -135,6 +135,43 @@ def test_kv_append_ragged(bits, dtype, lens, new, Hkv):
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("B,most,Hkv", [(1, 90, 2), (64, 20, 1), (65, 40, 2), (200, 33, 1), (4500, 3, 1)])
+def test_kv_append_many_sequences_without_a_bound(bits, B, most, Hkv):
+    """Ragged rows, empty sequences among them, and no bound on a sequence's new tokens."""
+    rng = np.random.default_rng(B + bits)
+    lens, new = rng.integers(0, 40, B), rng.integers(0, most + 1, B) * rng.integers(0, 2, B)
+    new[B // 2] = most
+    width = int(max(-(-(a + n) // PAGE) for a, n in zip(lens, new))) + 4   # room: places go by rows
+    cache, table = _random_cache(rng, B * width + 1, Hkv, bits), _table(rng, B, width, B * width + 1)
+    rows = int(new.sum())
+    x, x64 = _half(rng.standard_normal((rows, 2 * Hkv * D)), "fp16")
+    k, v = x[:, :Hkv * D].unflatten(1, (Hkv, D)), x[:, Hkv * D:].unflatten(1, (Hkv, D))
+    start = np.concatenate([[0], np.cumsum(new)])
+    got = [_t(c) for c in cache]
+    _ops().kv_append(k, v, *got, _t(table), _t(np.int32(lens)), bits, row_start=_t(start.astype(np.int32)))
+    rows_of = [list(range(start[b], start[b + 1])) for b in range(B)]
+    wk = ref.append(x64[:, :Hkv * D].reshape(rows, Hkv, D), cache[0], cache[2], table, list(lens), bits, rows_of)
+    wv = ref.append(x64[:, Hkv * D:].reshape(rows, Hkv, D), cache[1], cache[3], table, list(lens), bits, rows_of)
+    _check_append(cache, got, wk, wv)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_kv_append_to_a_page_of_infinite_scale(bits):
+    """The page keeps its scale, and every finite value over it is 0."""
+    rng = np.random.default_rng(bits)
+    cache, table = _random_cache(rng, 3, 2, bits), np.int32([[1]])
+    cache[2][1], cache[3][1] = np.inf, np.inf
+    x, x64 = _half(rng.standard_normal((5, 2, D)), "fp16")
+    got = [_t(c) for c in cache]
+    _ops().kv_append(x, x, *got, _t(table), _t(np.int32([7])), bits, row_start=_t(np.int32([0, 5])))
+    assert np.array_equal(got[2].cpu().numpy(), cache[2]) and np.array_equal(got[3].cpu().numpy(), cache[3])
+    for g, c in zip(got[:2], cache[:2]):
+        want = c.copy()
+        want[1, :, 7:12] = 0
+        assert np.array_equal(g.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
 def test_kv_append_selected_rows(bits):
     """Accepted nodes of a draft tree: counts, -1 padding, a node named twice, nodes outside the sequence's rows."""
     rng = np.random.default_rng(bits)
@@ -469,6 +506,19 @@ def test_verify_candidates(B, N, V, how):
     _check_verify(p, None, tokens, None if how == "chain" else parents, u, wide=N % 2 == 0)
     if B > 1:
         _check_verify(p, None, tokens, None if how == "chain" else parents, u, rng.integers(0, N + 1, B).astype(np.int32))
+
+
+@pytest.mark.parametrize("B,N,V", [(64, 3, 70001), (1, 2, 5000011), (2, 2, 67 * 65536 + 1)])
+def test_verify_large_vocabularies(B, N, V):
+    """Two parts a wave; more parts than a wave scans at once."""
+    rng = np.random.default_rng(V)
+    p = rng.random((B, N, V), dtype=np.float32)
+    p /= p.sum(-1, keepdims=True, dtype=np.float64).astype(np.float32)
+    tokens = rng.integers(0, V, (B, N))
+    u = rng.random((B, N), dtype=np.float32)
+    _check_verify(p, None, tokens, None, u)
+    p[:, :, : V - 3] = 0   # all weight at the end of the last part
+    _check_verify(p, None, tokens, None, u)
 
 
 def test_verify_odd_inputs():

@@ -189,7 +189,7 @@ extern "C" int exl3_qk_norm_rope(const void* q, const void* k, int x_bf16, long 
   const int groups = (num_q_heads + num_kv_heads + 3) / 4;
   const int per = (int)std::min<long long>(groups, std::max<long long>(1, (long long)tokens * groups / 8192));
   const int slices = (groups + per - 1) / per;
-  EXL3_CHECK_ARG((long long)tokens * slices < (1LL << 31), "exl3_qk_norm_rope: %d tokens of %d heads", tokens,
+  EXL3_CHECK_ARG((long long)tokens * slices < (1LL << 26), "exl3_qk_norm_rope: %d tokens of %d heads", tokens,
                  num_q_heads + num_kv_heads);
   const NormRopeArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), ld_q, ld_k, q_weight, k_weight,
                        w_type, eps, cos_sin, max_pos, cos_sin ? rotary_dim : 0, interleaved, positions, positions_i64,

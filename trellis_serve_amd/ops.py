@@ -802,6 +802,17 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Te
     return P, Hkv, B, max_pages
 
 
+def _check_apart(out: torch.Tensor, *inputs) -> None:
+    """An output that other workgroups' inputs lie in would be read and written in any order."""
+    start = out.data_ptr()
+    for t in inputs:
+        if t.numel() and out.numel():
+            at = t.data_ptr()
+            span = t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+            if at < start + out.nbytes and start < at + span:
+                raise ValueError("an output overlaps another tensor of the call")
+
+
 def _cuda_index(first: torch.Tensor, *others) -> int:
     """The index of the device that all tensors are on (None: no tensor)."""
     index = first.get_device()
@@ -876,8 +887,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
             raise ValueError(f"outputs of one type, got {q_out.dtype}, {k_out.dtype}")
         out_dtype = q_out.dtype
         for x, o in ((q, q_out), (k, k_out)):
-            if x.data_ptr() == o.data_ptr() and (x.dtype != o.dtype or not x.is_contiguous()):
+            if x.data_ptr() != o.data_ptr():
+                _check_apart(o, x)
+            elif x.dtype != o.dtype or not x.is_contiguous():
                 raise ValueError("an output may be its input only where both are contiguous and of one type")
+        _check_apart(q_out, k, k_out)
+        _check_apart(k_out, q)
     index = _cuda_index(q, k, q_weight, k_weight, cos_sin, positions if cos_sin is not None else None)
     if not _current(index):
         with torch.cuda.device(index):
@@ -972,6 +987,7 @@ def kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tenso
         dtype = k_out.dtype
         _check_out(k_out, shape, k_cache)
         _check_out(v_out, shape, k_cache, (dtype,))
+        _check_apart(k_out, v_out)
     index = _cuda_index(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, starts)
     if not _current(index):
         with torch.cuda.device(index):
@@ -1022,6 +1038,7 @@ def kv_tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
         live = num_nodes.data_ptr()
     if out is not None:
         _check_out(out, (B, N, Hq, _HEAD_DIM), q, _FP16)
+        _check_apart(out, q, k_new, v_new)
     index = _cuda_index(q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, num_nodes)
     if sm_scale is None:
         sm_scale = _HEAD_DIM ** -0.5
@@ -1044,6 +1061,13 @@ def kv_tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
 def verify_workspace_bytes(batch: int, vocab: int) -> int:
     """Bytes of a `workspace` for verify_drafts at this shape."""
     return _lib.load().exl3_verify_workspace_bytes(batch, vocab)
+
+
+def _narrow(t: torch.Tensor, end: int) -> torch.Tensor:
+    """int32 values; what lies outside [0, end) stays outside."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, end).to(torch.int32)
+    return t.contiguous()
 
 
 def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniform: torch.Tensor,
@@ -1087,11 +1111,9 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniform: tor
     if not _current(index):
         with torch.cuda.device(index):
             return verify_drafts(target_probs, tokens, uniform, parents, draft_probs, num_nodes, workspace)
-    if tokens.dtype != torch.int32 or not tokens.is_contiguous():
-        tokens = tokens.to(torch.int32).contiguous()
+    tokens = _narrow(tokens, V)
     if parents is not None:
-        if parents.dtype != torch.int32 or not parents.is_contiguous():
-            parents = parents.to(torch.int32).contiguous()
+        parents = _narrow(parents, N)
         up = parents.data_ptr()
     accepted = tokens.new_empty((B, N))
     out_tokens = tokens.new_empty((B, N))
