@@ -9,11 +9,15 @@
 // x and s have 11 bits each, so a correctly rounded fp32 quotient falls on a half-way point only when the exact one does,
 // and codes are those of exact arithmetic.
 // One wave per (page, kv head, keys or values): 16 slots x 128 values are four 16-byte loads per lane, the maximum one
-// wave reduction, and nobody else writes the page, so the launch needs no synchronisation.  Bound by memory at many
-// tokens; a decode step is a few dependent loads (length, page id, scale) long.
+// wave reduction, and nobody else writes the page, so the launch needs no synchronisation.  2900 + 1933 + 967 tokens of 8
+// heads (bf16 to 4 bits, 30 MB) take 10.4 us against 5.8 at a copy's rate: a chain of dependent loads (length, row range,
+// rows) over barely more waves than the card holds at once (with IEEE divisions for the codes: 14.8).  A decode step of 16
+// tokens is that chain: 3.7 us.
 //
 // kv_gather_kernel.  out = code * scale, rounded once, for rows of consecutive tokens.  A workgroup first finds its rows'
-// pages (one thread a row), then copies 8 codes per lane and step: 128-byte (64) code rows in, 256-byte rows out.
+// pages (one thread a row), then copies 8 codes per lane and step: 128-byte (64) code rows in, 256-byte rows out.  Bound by
+// memory: 7 prefixes up to 32k tokens (8 bits, 805 MB) take 163-177 us, 4.5-4.9 TB/s; a copy reaches 5.1.
+
 #include <algorithm>
 
 #include "exl3_api.hpp"
@@ -265,7 +269,7 @@ struct KvGatherArgs {
   uint16_t *k_out, *v_out;
 };
 
-constexpr int kGatherRows = 16;  // most rows per workgroup
+constexpr int kGatherRows = 16;  // most rows per workgroup (from 8192 rows on; 4 below, for more workgroups)
 
 template <int BITS, bool OB>
 __global__ __launch_bounds__(256) void kv_gather_kernel(const KvGatherArgs a, int rows_each) {

@@ -15,11 +15,14 @@
 //
 // Two forms.  Up to 96 rows (split): every wave of a workgroup of 4 works on pages of its own, codes straight into LDS stages
 // of the wave, no barrier until the waves' states are merged in LDS; up to 32 rows two workgroups share a CU, with more rows a
-// wave has a SIMD's registers to itself.  Long contexts run at the memory's rate (8 bits, 40 / 8 heads: 5.2 TB/s with 3 to 9
-// nodes, 4.1 with 16).  More rows (shared): decoding codes for 64 rows costs as much as their softmax, so the 8 waves of a
-// workgroup decode a tile of 4 pages together, as MFMA fragments in LDS, and each runs it against rows of its own (64 nodes:
-// 950-970 TFLOP/s on long contexts; the split form with 4 row groups per wave: 720-880).  Bound by VALU issue and LDS
-// latency there: a tile's 5700 cycles hold 2560 of MFMA and about 2900 of VALU per SIMD.
+// wave has a SIMD's registers to itself.  Long contexts run at the memory's rate (8 bits, 40 / 8 heads: 5.1 to 5.4 TB/s with
+// 3 to 9 nodes), with more rows at that of issue (16 nodes 3.8 TB/s, 610 TFLOP/s; 4 bits 690): a step of 80 rows holds 1280
+// cycles of MFMA in some 4800, one wave's chain of products, softmax and products.  More rows (shared): decoding codes for 64
+// rows costs as much as their softmax, so the 8 waves of a workgroup decode a tile of 4 pages together, as MFMA fragments in
+// LDS, and each runs it against rows of its own (64 nodes: 910 TFLOP/s at 8 bits, 1010 at 4; a large fp16 matrix product
+// reaches 1140 here).  Bound by issue there: MFMA takes 39 % and VALU 53 % of a SIMD's cycles, and the two waves of a SIMD
+// hardly overlap them; staggering their shares of decoding or wave priorities gave nothing beyond 1-3 % of either sign.
+// 24 nodes (one group of rows a wave: each fragment read from LDS feeds one product): 600 TFLOP/s.
 //
 // Work split: a unit is (sequence, kv head, tile of rows), its step 0 the nodes, each further one a workgroup's pages at a
 // time.  The steps of all units in a row are dealt to the workgroups in equal runs, whatever the lengths: a unit inside
@@ -510,7 +513,7 @@ __device__ __forceinline__ void tree_store(const KvTreeArgs& a, const TreeUnit& 
   }
 }
 
-// ---- split: up to 32 rows, pages per wave ---------------------------------------------------------------------------------
+// ---- split: up to 96 rows, pages per wave ---------------------------------------------------------------------------------
 
 // Codes of (page, kv head) blocks in LDS, brought there without passing through registers
 template <int BITS>
