@@ -143,7 +143,7 @@ def verify(p, q, tokens, parents, u, num_nodes):
                 continue
             t = int(tokens[b, i])
             known = 0 <= t < V
-            pt = float(p[b, path[-1], t]) if known and t not in refused else 0.0
+            pt = float(p[b, path[-1], t]) if known and t not in refused and np.isfinite(p[b, path[-1], t]) else 0.0
             bar = float(u[b, i]) * (left if q is None else float(q[b, path[-1], t]) if known else 0.0)
             if pt > 0 and bar < pt:
                 path.append(i)

@@ -547,6 +547,27 @@ def test_verify_odd_inputs():
     assert int(got[1].min()) >= 1
 
 
+def test_verify_drafts_of_infinite_probability_are_refused():
+    rng = np.random.default_rng(5)
+    p = _probs(rng, 3, 4, 70)
+    tokens, u = rng.integers(0, 70, (3, 4)), rng.random((3, 4), dtype=np.float32)
+    for b in range(3):
+        p[b, 0, tokens[b, 1]] = (np.inf, np.nan, -np.inf)[b]
+    for q in (None, _probs(rng, 3, 4, 70)):
+        got = _check_verify(p, q, tokens, None, u)
+        assert (got[1] == 1).all()
+
+
+def test_verify_in_a_given_workspace():
+    rng = np.random.default_rng(6)
+    B, N, V = 5, 3, 3001
+    args = _t(_probs(rng, B, N, V)), _t(rng.integers(0, V, (B, N))), _t(rng.random((B, N), dtype=np.float32))
+    ws = torch.full((_ops().verify_workspace_bytes(B, V),), 255, dtype=torch.uint8, device="cuda")
+    want = _ops().verify_drafts(*args)
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(_ops().verify_drafts(*args, workspace=ws), want))
+
+
 def test_verify_emits_the_targets_distribution():
     """The tokens after the root, over many uniform numbers, are distributed as the target's row 0: a chain with sampled drafts
     and a tree of fixed candidates.  8192 sequences over 8 tokens: the expected squared distance of the counts is below 1

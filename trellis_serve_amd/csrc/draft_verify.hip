@@ -68,6 +68,7 @@ __device__ __forceinline__ VerifyWalk verify_walk(const VerifyArgs& a, int b) {
   if (node && token >= 0 && token < a.vocab) {
     const size_t i = ((size_t)b * a.nodes + parent) * a.vocab + token;
     pt = a.p[i];
+    pt = pt < __builtin_inff() ? pt : 0.f;
     if (a.q) qt = a.q[i];
   }
   VerifyWalk w;
