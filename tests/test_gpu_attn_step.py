@@ -455,6 +455,30 @@ def test_kv_tree_attention_is_deterministic(bits):
         assert torch.equal(_ops().kv_tree_attention(*args, workspace=ws), want)
 
 
+@pytest.mark.parametrize("N", [3, 9, 40])
+def test_pages_past_four_gigabytes(N):
+    """The same pages at the end of a cache of more than 2^32 bytes give the same codes, values and attention."""
+    rng = np.random.default_rng(N)
+    lens, Hq, Hkv, far = [300, 5, 77], 24, 8, 270000
+    q, k, v, seen, cache, table = _tree_case(N, lens, N, Hq, Hkv, 8, "tree", spare=4)
+    table[:] = rng.permutation(len(cache[0]))[: table.size].reshape(table.shape)
+    for c in cache[2:]:
+        c[:] = np.abs(rng.normal(0, 0.02, c.shape)).astype(np.float16)
+    near = [_t(c) for c in cache]
+    P, first = len(cache[0]), far - len(cache[0])
+    wide = [torch.empty((far, *c.shape[1:]), dtype=c.dtype, device="cuda") for c in near]
+    for w, c in zip(wide, near):
+        w[first:] = c
+    start, lt, results = _t(np.cumsum([0] + [n + N for n in lens]).astype(np.int32)), _t(np.int32(lens)), []
+    for caches, t in ((near, _t(table)), (wide, _t(table + np.int32(first)))):
+        out = _ops().kv_tree_attention(q, k, v, _t(_masks(seen)), *caches, t, lt, 8)
+        _ops().kv_append(k, v, *caches, t, lt, 8)
+        back = _ops().kv_gather(*caches, t, lt + N, 8, start, int(sum(lens)) + 3 * N)
+        results.append([out, *back, *(c[-P:] for c in caches)])
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
 # ---- verification --------------------------------------------------------------------------------------------------------
 
 def _probs(rng, *shape, sharp=2.0):
