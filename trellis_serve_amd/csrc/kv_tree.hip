@@ -21,7 +21,7 @@
 // rows costs as much as their softmax, so the 8 waves of a workgroup decode a tile of 4 pages together, as MFMA fragments in
 // LDS, and each runs it against rows of its own (64 nodes: 910 TFLOP/s at 8 bits, 1010 at 4; a large fp16 matrix product
 // reaches 1140 here).  Bound by issue there: MFMA takes 39 % and VALU 53 % of a SIMD's cycles, and the two waves of a SIMD
-// hardly overlap them; staggering their shares of decoding or wave priorities gave nothing beyond 1-3 % of either sign.
+// hardly overlap them (the products at a higher wave priority: 3 %; staggering the waves' shares of decoding: nothing).
 // 24 nodes (one group of rows a wave: each fragment read from LDS feeds one product): 600 TFLOP/s.
 //
 // Work split: a unit is (sequence, kv head, tile of rows), its step 0 the nodes, each further one a workgroup's pages at a
@@ -898,6 +898,10 @@ __device__ __forceinline__ void shared_part(const KvTreeArgs& a, SharedMem<BITS>
               for (int gi = 0; gi < RG; gi++) sc[i][gi] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < PER; f++) {
+              // The wave of a SIMD that is at its products goes first, the other's softmax fills in (40 sequences up to 2000
+              // tokens, 64 nodes: 136 -> 132 us; 24 nodes 75 -> 74; with two groups it costs 1 %)
+              if (RG != 2 && (f == 0 || f == 4 * NP)) __builtin_amdgcn_s_setprio(1);
+              if (RG != 2 && (f == 4 * NP - 1 || f == PER - 1)) __builtin_amdgcn_s_setprio(0);
               const int k = PER * pass + f;
               if (k + AHEAD < 8 * PAGES) fr[(k + AHEAD) % FR] = read(k + AHEAD);
               issue_fence();
