@@ -19,9 +19,10 @@
 // 3 to 9 nodes), with more rows at that of issue (16 nodes 3.8 TB/s, 610 TFLOP/s; 4 bits 690): a step of 80 rows holds 1280
 // cycles of MFMA in some 4800, one wave's chain of products, softmax and products.  More rows (shared): decoding codes for 64
 // rows costs as much as their softmax, so the 8 waves of a workgroup decode a tile of 4 pages together, as MFMA fragments in
-// LDS, and each runs it against rows of its own (64 nodes: 910 TFLOP/s at 8 bits, 1010 at 4; a large fp16 matrix product
-// reaches 1140 here).  Bound by issue there: MFMA takes 39 % and VALU 53 % of a SIMD's cycles, and the two waves of a SIMD
-// hardly overlap them (the products at a higher wave priority: 3 %; staggering the waves' shares of decoding: nothing).
+// LDS, and each runs it against rows of its own (64 nodes: 910 to 1010 TFLOP/s; a large fp16 matrix product
+// reaches 1140 here).  Bound by issue there: MFMA takes 41 % and VALU 56 % of a SIMD's cycles, at a clock of 2.0 GHz under
+// that load, and the two waves of a SIMD hardly overlap them (the products at a higher wave priority: 3 %; staggering the
+// waves' shares of decoding: nothing).
 // 24 nodes (one group of rows a wave: each fragment read from LDS feeds one product): 600 TFLOP/s.
 //
 // Work split: a unit is (sequence, kv head, tile of rows), its step 0 the nodes, each further one a workgroup's pages at a
