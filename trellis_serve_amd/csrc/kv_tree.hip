@@ -252,7 +252,8 @@ struct TreeRows {
       const float d = fmaxf(t, bar[gi] == kTreeBar ? 0.f : kTreeLow);  // the first keys of a row lower it too
       if (t > -INFINITY || bar[gi] == kTreeBar) {
         bar[gi] = kTreeBar;
-        const float alpha = __builtin_amdgcn_exp2f(-d);
+        // (an empty row's l and o are zeros: with logits of -128 and below exp2(-d) would make them 0 * inf)
+        const float alpha = __builtin_amdgcn_exp2f(-fmaxf(d, 0.f));
         m[gi] += d;
         l[gi] *= alpha;
 #pragma unroll
