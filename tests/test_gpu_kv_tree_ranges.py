@@ -88,3 +88,31 @@ def test_forms_repeat_bit_for_bit(bits, N, Hq, Hkv):
         ws = torch.full((_ops().kv_tree_workspace_bytes(len(lens), N, Hq, Hkv, case[5].shape[1]),), 255, dtype=torch.uint8,
                         device="cuda")
         assert torch.equal(_run(case, lens, bits, workspace=ws), want)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("N,Hq,Hkv,nodes", [
+    (64, 5, 1, [4, 20, 33, 44, 64, 26]), (64, 16, 1, [2, 7, 14, 30, 58, 0]), (40, 16, 2, [3, 28, 15, 40, 9, 1]),
+    (20, 16, 1, [2, 14, 8, 20, 11, 5]), (33, 4, 1, [1, 33, 17, 5, 25, 29]), (61, 4, 1, [2, 40, 33, 61, 17, 9])])
+def test_fewer_live_nodes_than_the_launch_has_room_for(bits, N, Hq, Hkv, nodes):
+    """Units whose waves get fewer groups of rows than planned, from none to all but one, split over many workgroups: the
+    reference's values, the same bits on every run, and nothing past the live nodes (K and V hold NaN there)."""
+    lens = [1500, 700, 2100, 40, 0, 333]
+    q, k, v, seen, cache, table = _tree_case(N + Hq + bits, lens, N, Hq, Hkv, bits, "tree", scale=2.0)
+    k, v = k.clone(), v.clone()
+    for b, n in enumerate(nodes):
+        k[b, n:] = v[b, n:] = float("nan")
+        seen[b, :, n:] = False
+    args = [q, k, v, _t(_masks(seen)), *[_t(c) for c in cache], _t(table), _t(np.int32(lens)), bits]
+    first = None
+    for fill in (0, 255, 0x3C, 255):
+        out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+        ws = torch.full((_ops().kv_tree_workspace_bytes(len(lens), N, Hq, Hkv, table.shape[1]),), fill, dtype=torch.uint8,
+                        device="cuda")
+        got = _ops().kv_tree_attention(*args, num_nodes=_t(np.int32(nodes)), out=out, workspace=ws)
+        for b, n in enumerate(nodes):
+            assert (got[b, n:] == 7.0).all()
+        first = got if first is None else first
+        assert torch.equal(got, first)
+    clean = [torch.where(x.isnan(), 0, x) for x in (k, v)]
+    _check_tree(first, q, *clean, seen, cache, table, lens, bits, nodes=nodes)

@@ -965,10 +965,16 @@ __global__ __launch_bounds__(64 * kSharedSlots, 2) void kv_tree_shared_kernel(co
   for (int s = runs.start(wg); s < s_end;) {
     const TreeUnit u = tree_at_step<false>(a, runs, s);
     const TreePart p(a, u, runs.extra, s, s_end);
-    // the unit's groups of rows, dealt evenly: wave w and wave w + 4 share a SIMD
+    // The unit's groups of rows, dealt evenly (wave w and wave w + 4 share a SIMD), but RG - 1 to a wave at least while they
+    // last: a wave has code for RG and RG - 1 groups, and where a sequence has fewer live nodes than the launch has room for,
+    // the group that a share of one would be rounded up by is the next wave's.  (Code for RG - 2 too: 35 spilled registers
+    // instead of 22.)  The last share may be short of one, past the unit's rows.
+    constexpr int LEAST = RG > 1 ? RG - 1 : 1;
     const int groups = (min(p.rows - p.row0, a.tile) + 15) / 16;
     const int each = groups / kSharedSlots, more = groups - each * kSharedSlots;
-    const int mine = each + (w < more), row0 = p.row0 + 16 * (w * each + min(w, more));
+    const bool even = each >= LEAST;
+    const int first = even ? w * each + min(w, more) : min(w * LEAST, groups);
+    const int mine = even ? each + (w < more) : min(groups - first, LEAST), row0 = p.row0 + 16 * first;
     if (mine == RG)
       shared_part<BITS, RG>(a, sh, u, p, row0, w, lane, wg);
     else if (RG > 1 && mine > 0)
