@@ -116,3 +116,27 @@ def test_fewer_live_nodes_than_the_launch_has_room_for(bits, N, Hq, Hkv, nodes):
         assert torch.equal(got, first)
     clean = [torch.where(x.isnan(), 0, x) for x in (k, v)]
     _check_tree(first, q, *clean, seen, cache, table, lens, bits, nodes=nodes)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("N,Hq,Hkv", [(1, 4, 1), (11, 4, 1), (24, 4, 1), (31, 4, 1), (64, 5, 1)])
+@pytest.mark.parametrize("scale", [2.0 ** -8, 2.0 ** -14, 2.0 ** -19])
+def test_many_keys_far_below_a_node(bits, N, Hq, Hkv, scale):
+    """8192 cached keys 12 below each node's own logit hold 5 % of its weight between them, each 2^-17 of the node's, and
+    2^-17 times the pages' value scale where that is folded into the probability.  The values of both are of one size.  Many
+    copies of the sequence: most of them are one workgroup's whole."""
+    lens, copies = [8192], 512
+    rng = np.random.default_rng(N + bits)
+    q, k, v, seen, cache, table = _tree_case(N, lens, N, Hq, Hkv, bits, "tree", spare=0)
+    top, w = (127, 7)[bits == 4], np.where(rng.permutation(D) < D // 2, 1, -1)
+    q, k = torch.empty_like(q).copy_(torch.from_numpy(w)), torch.empty_like(k).copy_(torch.from_numpy(w * 12 * D ** -0.5))
+    v = (v.clamp(-3, 3) * (scale * top / 3)).contiguous()
+    seen[:] = np.eye(N, dtype=bool)
+    cache[0][:] = 0
+    cache[1][:] = ref.pack(rng.integers(top // 2, top + 1, (len(cache[1]), Hkv, PAGE, D)), bits)
+    cache[3][:] = np.float16(scale)
+    many = [t.expand(copies, *t.shape[1:]).contiguous() for t in (q, k, v, _t(_masks(seen)))]
+    got = _ops().kv_tree_attention(*many, *[_t(c) for c in cache], _t(table).expand(copies, -1).contiguous(),
+                                   _t(np.int32(lens * copies)), bits)
+    for end in (got.float().amin(0, keepdim=True), got.float().amax(0, keepdim=True)):   # so all copies
+        _check_tree(end, q, k, v, seen, cache, table, lens, bits)

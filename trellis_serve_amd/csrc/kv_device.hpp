@@ -49,6 +49,24 @@ __device__ __forceinline__ float sum_over_groups(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// magnitudes of halves order as integers: maxima of pairs, and over a wave
+typedef uint16_t kv_u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(kv_u16x2_t, a),
+                                                                __builtin_bit_cast(kv_u16x2_t, b)));
+}
+template <int ROR>
+__device__ __forceinline__ uint32_t max_ror(uint32_t v) {  // with the lane ROR places off in its row of 16
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + ROR, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = max_ror<1>(max_ror<2>(max_ror<4>(max_ror<8>(v))));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(max(b[0], b[1]));
+}
+
 // Keeps the loads above it issued here: otherwise they are free to sink to their first use, which turns the
 // next-page prefetch into a load-and-wait.  Registers are not touched, so no wait is implied.  (The cache pointers
 // carry no __restrict__: loads of restrict read-only memory count as invariant and would cross the fence.)

@@ -9,9 +9,14 @@
 //   S^T = K Q^T     4 x MFMA 16x16x32 per page and group
 //   O^T += V^T P^T  8 x MFMA 16x16x32 per group: slots 0..3 of a lane's 8 keys are its keys of the first page, 4..7 of the
 //                   second, so the C layout of the two S^T is the B operand as it stands
-// Softmax in base 2 with a lazy reference: O, l are rescaled only when a logit passes the reference by more than 4.  The
-// page's value scale is folded into the exponent (p' = 2^(s + log2 vs - m)), so P' stays within 16 of fp16 whatever the
-// scales are, and a step has no multiplication per probability; the sum takes p' / vs, once per page and row.
+// Softmax in base 2 with a lazy reference: O, l are rescaled only when a logit passes the reference by more than 15.  The
+// page's value scale is folded into the exponent (p' = 2^(s + log2 vs - m)), so a step has no multiplication per
+// probability; the sum takes p' / vs, once per page and row, in fp32.  P' is rounded to fp16 for the second product, which
+// takes both operands in one 16-bit type: fp16 holds every code and 3 bits more of P' than bf16 would (half a step: 2^-12 to
+// 2^-11 of a key's share).  Its range is the other limit, steps of 2^-24 at the bottom.  The reference therefore lies 11 below
+// a row's largest exponent when it is set, so the largest P' stays between 2^11 and 2^15, and a tile of nodes is brought to
+// the size of codes by a power of two, like a page of that scale.  With P' of at least 2^11 against codes of 127 each key
+// below fp16's range costs an output at most 2^-25 * 2^-11 of the largest value (2^-35 where that is a node's).
 //
 // Two forms.  Up to 96 rows (split): every wave of a workgroup of 4 works on pages of its own, codes straight into LDS stages
 // of the wave, no barrier until the waves' states are merged in LDS; up to 32 rows two workgroups share a CU, with more rows a
@@ -44,7 +49,8 @@ constexpr int kSharedGroups = 3;      // most groups of 16 rows per wave
 constexpr int kSplitGroups = 6;
 constexpr int kPairedGroups = 2;      // split: up to as many, two workgroups share a CU
 constexpr int kTreeExtra = 6;         // most steps that the beginning of a unit counts for
-constexpr float kTreeBar = 4.f;       // exponents above it move a row's reference
+constexpr float kTreeHead = 11.f;     // what a row's largest exponent is brought to (P' in fp16: to 2^15, no overflow)
+constexpr float kTreeBar = 15.f;      // exponents above it move a row's reference
 constexpr float kTreeLow = -1e30f;    // below any logit, finite: differences of empty states are 0, not NaN
 
 struct KvTreeArgs {
@@ -232,8 +238,8 @@ struct TreeRows {
     return r;
   }
 
-  // x: NS exponents per group, relative to the references.  Where a lane has one past its bar the references move to the
-  // largest: once a row has seen a key the bar is 4 (p' stays within 16), before that any key passes it.
+  // x: NS exponents per group, relative to the references.  Where a lane has one past its bar the references move to
+  // kTreeHead below the largest: once a row has seen a key the bar is kTreeBar, before that any key passes it.
   template <int NS>
   __device__ __forceinline__ void raise(float (&x)[RG][NS]) {
     float top[RG];
@@ -248,7 +254,7 @@ struct TreeRows {
     if (!__builtin_amdgcn_ballot_w64(any)) return;
 #pragma unroll
     for (int gi = 0; gi < RG; gi++) {
-      const float t = max_over_groups(top[gi]);
+      const float t = max_over_groups(top[gi]) - kTreeHead;
       const float d = fmaxf(t, bar[gi] == kTreeBar ? 0.f : kTreeLow);  // the first keys of a row lower it too
       if (t > -INFINITY || bar[gi] == kTreeBar) {
         bar[gi] = kTreeBar;
@@ -358,6 +364,18 @@ struct TreeRows {
       // such a key would reach the rows that do not see it as 0 * inf: it leaves the product and is added below
       if ((odd[i] >> (16 * g) & 0xFFFF) || key > last) vr[i] = half8_t{};
     }
+    // values times 2^up: the largest in [64, 128), where the least step of P' costs what it costs a page of codes
+    uint32_t pairs = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const kv_u32x4_t w = __builtin_bit_cast(kv_u32x4_t, vr[i]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) pairs = max_u16x2(pairs, w[e] & 0x7FFF7FFFu);
+    }
+    const int up = min(max(21 - (int)(wave_max_u32(max(pairs & 0xFFFFu, pairs >> 16)) >> 10), 0), 15);
+    const _Float16 vup = __builtin_bit_cast(_Float16, (uint16_t)((15 + up) << 10));
+#pragma unroll
+    for (int i = 0; i < 4; i++) vr[i] *= vup;
     float x[RG][4];
     unsigned seen[RG];  // bit j: this row sees node 16 t + j
 #pragma unroll
@@ -368,7 +386,8 @@ struct TreeRows {
       for (int c = 0; c < 4; c++)
         s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], q[gi][c], s, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[gi][i] = (seen[gi] >> (4 * g + i) & 1) ? __builtin_fmaf(s[i], a.qk_scale, -m[gi]) : -INFINITY;
+      for (int i = 0; i < 4; i++)
+        x[gi][i] = (seen[gi] >> (4 * g + i) & 1) ? __builtin_fmaf(s[i], a.qk_scale, -m[gi] - (float)up) : -INFINITY;
     }
     raise<4>(x);
 #pragma unroll
@@ -380,7 +399,7 @@ struct TreeRows {
         p[i] = __builtin_amdgcn_exp2f(x[gi][i]);
         pf[i] = (_Float16)p[i];
       }
-      l[gi] += (p[0] + p[1]) + (p[2] + p[3]);
+      l[gi] = __builtin_fmaf((p[0] + p[1]) + (p[2] + p[3]), (float)vup, l[gi]);
 #pragma unroll
       for (int db = 0; db < 8; db++)
         o[gi][db] = __builtin_amdgcn_mfma_f32_16x16x16f16(half4_t{vr[0][db], vr[1][db], vr[2][db], vr[3][db]}, pf,
@@ -391,7 +410,7 @@ struct TreeRows {
           const unsigned long long lanes = (j & 3) == 0 ? odd[0] : (j & 3) == 1 ? odd[1] : (j & 3) == 2 ? odd[2] : odd[3];
           if (!(lanes >> (16 * (j >> 2)) & 0xFFFF)) continue;
           const float pj = (j & 3) == 0 ? p[0] : (j & 3) == 1 ? p[1] : (j & 3) == 2 ? p[2] : p[3];
-          const float pk = __shfl(pj, n + 16 * (j >> 2));
+          const float pk = __shfl(pj, n + 16 * (j >> 2)) * (float)vup;
           if (seen[gi] >> j & 1) {
             const _Float16* vp = a.v_new + (seq + 16 * t + j) * a.ld_v + hk * kHeadDim + 32 * g;
 #pragma unroll
