@@ -311,7 +311,8 @@ int exl3_kv_decode_attention(const void* q, const void* k_cache, const void* v_c
  * No counterpart in the reference: its engines bring these steps themselves.  Token strides (ld_*) count elements from
  * one token's heads to the next's, multiples of 8, so q, k and v may be columns of the fused linear's output; a token's
  * heads are contiguous, and every tensor is 16-byte aligned.  Caches, page tables and seq_lens as
- * exl3_kv_decode_attention has them. */
+ * exl3_kv_decode_attention has them.  What a call writes (outputs, workspace, for exl3_kv_append the caches and scales)
+ * overlaps nothing else of the call, but for exl3_qk_norm_rope in place. */
 
 /* q_out, k_out [tokens][heads][128] = the heads of q and k, each normalised over its 128 values with its weight,
  *   y = x * rsqrt(mean(x^2) + eps) * w      (weights fp16 | bf16 | fp32 [128], w_type EXL3_F16 / _BF16 / _F32; both or

@@ -331,6 +331,15 @@ static int check_cache(const char* what, const void* k_cache, const void* v_cach
   return EXL3_OK;
 }
 
+struct Span {
+  const void* at;
+  size_t bytes;
+  bool meets(const Span& o) const {
+    const uintptr_t a = (uintptr_t)at, b = (uintptr_t)o.at;
+    return at && o.at && a < b + o.bytes && b < a + bytes;
+  }
+};
+
 }  // namespace exl3
 
 using namespace exl3;
@@ -361,6 +370,17 @@ extern "C" int exl3_kv_append(const void* k, const void* v, int x_bf16, long lon
   if (row_start && !select && 2 * by_rows < places) pages_each = 0, places = by_rows;
   const long long items = 2 * places * num_kv_heads;
   EXL3_CHECK_ARG(items < kMaxWaves, "exl3_kv_append: %d sequences of up to %d new tokens", batch, max_new);
+  // what one wave writes, no other may read or write: caches and scales apart from each other and from every input
+  const size_t blocks = (size_t)num_pages * num_kv_heads, heads = (size_t)num_kv_heads * head_dim, ints = sizeof(int);
+  const size_t code_bytes = blocks * page_size * head_dim * bits / 8;
+  const Span all[] = {{k_cache, code_bytes}, {v_cache, code_bytes}, {k_scale, blocks * 2}, {v_scale, blocks * 2},
+                      {k, 2 * ((size_t)(rows - 1) * ld_k + heads)}, {v, 2 * ((size_t)(rows - 1) * ld_v + heads)},
+                      {page_table, (size_t)batch * max_pages * ints}, {seq_lens, batch * ints},
+                      {row_start, (batch + (size_t)1) * ints}, {select, (size_t)batch * max_new * ints},
+                      {counts, batch * ints}};
+  for (int i = 0; i < 4; i++)
+    for (int j = i + 1; j < (int)(sizeof(all) / sizeof(all[0])); j++)
+      EXL3_CHECK_ARG(!all[i].meets(all[j]), "exl3_kv_append: a cache or its scales overlap another tensor of the call");
   const KvAppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), ld_k, ld_v, rows, row_start,
                        rows_per_seq, select, counts, max_new, static_cast<uint8_t*>(k_cache),
                        static_cast<uint8_t*>(v_cache), static_cast<uint16_t*>(k_scale),

@@ -803,10 +803,10 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Te
 
 
 def _check_apart(out: torch.Tensor, *inputs) -> None:
-    """An output that other workgroups' inputs lie in would be read and written in any order."""
+    """An output (or a workspace) that other workgroups' inputs lie in would be read and written in any order."""
     start = out.data_ptr()
     for t in inputs:
-        if t.numel() and out.numel():
+        if t is not None and t.numel() and out.numel():
             at = t.data_ptr()
             span = t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
             if at < start + out.nbytes and start < at + span:
@@ -891,8 +891,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
                 _check_apart(o, x)
             elif x.dtype != o.dtype or not x.is_contiguous():
                 raise ValueError("an output may be its input only where both are contiguous and of one type")
-        _check_apart(q_out, k, k_out)
-        _check_apart(k_out, q)
+        rest = (q_weight, k_weight, cos_sin, positions if cos_sin is not None else None)
+        _check_apart(q_out, k, k_out, *rest)
+        _check_apart(k_out, q, *rest)
     index = _cuda_index(q, k, q_weight, k_weight, cos_sin, positions if cos_sin is not None else None)
     if not _current(index):
         with torch.cuda.device(index):
@@ -987,7 +988,9 @@ def kv_gather(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tenso
         dtype = k_out.dtype
         _check_out(k_out, shape, k_cache)
         _check_out(v_out, shape, k_cache, (dtype,))
-        _check_apart(k_out, v_out)
+        read = (k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, starts)
+        _check_apart(k_out, v_out, *read)
+        _check_apart(v_out, *read)
     index = _cuda_index(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, starts)
     if not _current(index):
         with torch.cuda.device(index):
@@ -1038,7 +1041,10 @@ def kv_tree_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
         live = num_nodes.data_ptr()
     if out is not None:
         _check_out(out, (B, N, Hq, _HEAD_DIM), q, _FP16)
-        _check_apart(out, q, k_new, v_new)
+        _check_apart(out, q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, num_nodes)
+    if workspace is not None:
+        _check_apart(workspace, out, q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens,
+                     num_nodes)
     index = _cuda_index(q, k_new, v_new, tree_mask, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, num_nodes)
     if sm_scale is None:
         sm_scale = _HEAD_DIM ** -0.5
@@ -1107,6 +1113,8 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniform: tor
     if num_nodes is not None:
         _check_int32(num_nodes, "num_nodes", (B,))
         live = num_nodes.data_ptr()
+    if workspace is not None:
+        _check_apart(workspace, target_probs, tokens, uniform, parents, draft_probs, num_nodes)
     index = _cuda_index(target_probs, tokens, uniform, parents, draft_probs, num_nodes)
     if not _current(index):
         with torch.cuda.device(index):
