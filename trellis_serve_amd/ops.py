@@ -919,6 +919,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
       [B, Hkv, 128]        one a sequence;
       [rows, Hkv, 128]     with row_start int32 [B + 1]: rows row_start[b] .. row_start[b + 1] - 1 are sequence b's
                            (`max_new`: the most a sequence has, if known on the host; it sizes the launch).
+    No sequence gets more than `max_new` tokens, where it is given.
     select int32 [B, S]: token j of sequence b is its row select[b, j] (the accepted nodes of verify_drafts, with its
     `counts`).  A page's scale covers its new tokens and what it held; older codes are rounded anew where it grows.  Tokens
     past the table and pages outside the cache are not written; no two sequences may append to one page."""
@@ -947,11 +948,15 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if select is not None:
         if select.dim() != 2:
             raise ValueError(f"select must be int32 [{B}, S]")
+        if max_new is not None and max_new < select.shape[1]:
+            raise ValueError(f"max_new = {max_new}, but select names up to {select.shape[1]} tokens (limit them by counts)")
         max_new = select.shape[1]
         _check_int32(select, "select", (B, max_new))
         picks = select.data_ptr()
-    elif max_new is None or row_start is None:
+    elif max_new is None:
         max_new = rows if row_start is not None else per_seq
+    elif row_start is None:
+        max_new = min(max_new, per_seq)
     if max_new < 0:
         raise ValueError(f"max_new = {max_new}")
     index = _cuda_index(k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, select, counts)
