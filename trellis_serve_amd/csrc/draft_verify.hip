@@ -8,9 +8,11 @@
 //     p(t_j) > 0 and u_j m < p(t_j); a refused one takes m -= p(t_j) and its token is struck from p (p = 0 for a brother
 //     with the same token).  The next token comes from p without the struck tokens.
 //   Next token: the smallest v with w(0) + .. + w(v) > u_0 * (the sum of w).
-// Given its drafts, either rule leaves every emitted token distributed as the target's.  Products and sums are in 64 bits:
-// the products of two floats are exact there, and the running sums of 10^5 terms are off by 10^-12 of a term at most, so
-// decisions do not depend on the order of the sums.
+// Given its drafts, either rule leaves every emitted token distributed as the target's.  Products and sums are in 64 bits.
+// The product of two floats is exact there, so a chain's decisions are; m is rounded once per refused child.  A running sum
+// over 10^5 terms goes through some tens of additions (16 a lane, a scan over the wave, the parts), each off by at most 2^-53 of the row's
+// total.  So another order of summation picks another token only where u * total lies within some 10^-14 of the total from
+// the edge between the two; the floats u themselves are 6 * 10^-8 apart.
 //
 // The walk reads one probability per node (lane i: node i) and is wave-uniform afterwards.  Only the row that the next
 // token comes from is read whole.  verify_mass_kernel: (chunks of the row, sequences) workgroups, each repeats the walk
