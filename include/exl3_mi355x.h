@@ -329,7 +329,7 @@ int exl3_qk_norm_rope(const void* q, const void* k, int x_bf16, long long ld_q, 
 
 /* Quantizes new keys and values into the cache, at positions seq_lens[b], seq_lens[b] + 1, ... of sequence b (seq_lens are
  * the lengths before the call and are not changed).  k, v fp16 | bf16, `rows` token rows of num_kv_heads x 128.  Sequence
- * b's rows are row_start[b] .. row_start[b + 1] - 1 (int32 [batch + 1]), or, with row_start NULL, rows_per_seq rows each
+ * b's rows are row_start[b] .. row_start[b + 1] - 1 (int32 [batch + 1], ascending), or, with row_start NULL, rows_per_seq each
  * (rows = batch * rows_per_seq).  Its new tokens are all of them, or those that row select[b][j] names, counted from the
  * sequence's first (int32 [batch][max_new], e.g. accepted_nodes of exl3_verify_drafts); of them the first counts[b]
  * (int32 [batch], NULL: all) and at most max_new.

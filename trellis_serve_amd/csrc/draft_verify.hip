@@ -10,9 +10,9 @@
 //   Next token: the smallest v with w(0) + .. + w(v) > u_0 * (the sum of w).
 // Given its drafts, either rule leaves every emitted token distributed as the target's.  Products and sums are in 64 bits.
 // The product of two floats is exact there, so a chain's decisions are; m is rounded once per refused child.  A running sum
-// over 10^5 terms goes through some tens of additions (16 a lane, a scan over the wave, the parts), each off by at most 2^-53 of the row's
-// total.  So another order of summation picks another token only where u * total lies within some 10^-14 of the total from
-// the edge between the two; the floats u themselves are 6 * 10^-8 apart.
+// over 10^5 terms goes through some tens of additions (16 a lane, a scan over the wave, the parts), each off by at most
+// 2^-53 of the row's total.  So another order of summation picks another token only where u * total lies within some 10^-14
+// of the total from the edge between the two; the floats u themselves are 6 * 10^-8 apart.
 //
 // The walk reads one probability per node (lane i: node i) and is wave-uniform afterwards.  Only the row that the next
 // token comes from is read whole.  verify_mass_kernel: (chunks of the row, sequences) workgroups, each repeats the walk

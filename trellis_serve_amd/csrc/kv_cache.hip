@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a) {
   int count = a.select ? a.max_new : min(avail, a.max_new);
   if (a.counts) count = min(count, a.counts[b]);
   count = min(count, a.max_pages * kPage - len);  // nothing past the table
-  if (count <= 0 || pg > count / kPage + 1) return;
+  if (count <= 0 || pg < 0 || pg > count / kPage + 1) return;  // (below 0: row starts that do not ascend)
   const int lp = len / kPage + pg, first = lp * kPage;  // logical page, its first token
   if (first >= len + count) return;
   const int page = a.page_table[(size_t)b * a.max_pages + lp];

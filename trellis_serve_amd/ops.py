@@ -917,7 +917,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     a wider row allowed:
       [B, n, Hkv, 128]     n rows a sequence (with `counts` int32 [B]: the first counts[b] of them);
       [B, Hkv, 128]        one a sequence;
-      [rows, Hkv, 128]     with row_start int32 [B + 1]: rows row_start[b] .. row_start[b + 1] - 1 are sequence b's
+      [rows, Hkv, 128]     with row_start int32 [B + 1], ascending: rows row_start[b] .. row_start[b + 1] - 1 are sequence b's
                            (`max_new`: the most a sequence has, if known on the host; it sizes the launch).
     No sequence gets more than `max_new` tokens, where it is given.
     select int32 [B, S]: token j of sequence b is its row select[b, j] (the accepted nodes of verify_drafts, with its
