@@ -40,3 +40,18 @@ def test_a_bound_below_the_rows_of_a_sequence(bits, max_new):
     want = [ref.append(x.reshape(3 * n, Hkv, 128), c, s, table, lens, bits, rows_of)
             for x, c, s in ((k64, cache[0], cache[2]), (v64, cache[1], cache[3]))]
     _check_append(cache, got, *want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_new", [5, 2 ** 31, 2 ** 32, 2 ** 32 + 2, 2 ** 63 - 1])
+def test_a_bound_past_32_bits_is_no_bound(max_new):
+    from test_gpu_attn_step import _check_append, _half, _random_cache, _t, _table
+    rng = np.random.default_rng(5)
+    lens, start = [3, 30], [0, 5, 9]
+    cache, table = _random_cache(rng, 8, 2, 8), _table(rng, 2, 4, 8)
+    x, x64 = _half(rng.standard_normal((9, 2, 128)), "fp16")
+    got = [_t(c) for c in cache]
+    ops.kv_append(x, x, *got, _t(table), _t(np.int32(lens)), 8, row_start=_t(np.int32(start)), max_new=max_new)
+    rows_of = [list(range(start[b], start[b + 1])) for b in range(2)]
+    _check_append(cache, got, *[ref.append(x64, c, s, table, lens, 8, rows_of) for c, s in ((cache[0], cache[2]),
+                                                                                         (cache[1], cache[3]))])

@@ -953,10 +953,9 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         max_new = select.shape[1]
         _check_int32(select, "select", (B, max_new))
         picks = select.data_ptr()
-    elif max_new is None:
-        max_new = rows if row_start is not None else per_seq
-    elif row_start is None:
-        max_new = min(max_new, per_seq)
+    else:
+        most = rows if row_start is not None else per_seq
+        max_new = most if max_new is None else min(max_new, most)
     if max_new < 0:
         raise ValueError(f"max_new = {max_new}")
     index = _cuda_index(k, v, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, row_start, select, counts)
