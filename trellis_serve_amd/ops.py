@@ -736,8 +736,9 @@ def kv_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
 
 # ---- Around the quantized-KV attention: what a decode or speculative step does between its linears and the cache.  The
 # reference has no counterpart of these (its engines bring them).  Their workspaces come from torch's allocator on the
-# current stream, call by call: calls on several streams and captured graphs never share one.  A caller that may not
-# allocate passes `workspace`; calls that share it must then be ordered.
+# current stream, call by call: calls on several streams and captured graphs never share one.  A caller's own `workspace`
+# saves that allocation (and its `out`, where there is one, the results'; verify_drafts makes its own); calls that share it
+# must then be ordered.
 
 # The checks are written for their cost: the library call of 23 arguments and its launch take 3.7 us, each attribute read of
 # a tensor 0.06 to 0.09, an allocation 1.5 (new_empty) to 1.7.
