@@ -10,7 +10,7 @@
 // and codes are those of exact arithmetic.
 // One wave per (page, kv head, keys or values): 16 slots x 128 values are four 16-byte loads per lane, the maximum one
 // wave reduction, and nobody else writes the page, so the launch needs no synchronisation.  2900 + 1933 + 967 tokens of 8
-// heads (bf16 to 4 bits, 30 MB) take 10.4 us against 5.8 at a copy's rate: a chain of dependent loads (length, row range,
+// heads (bf16 to 4 bits, 30 MB) take 10.6 us against 5.8 at a copy's rate: a chain of dependent loads (length, row range,
 // rows) over barely more waves than the card holds at once (with IEEE divisions for the codes: 14.8).  A decode step of 16
 // tokens is that chain: 3.7 us.
 //

@@ -20,15 +20,15 @@
 //
 // Two forms.  Up to 96 rows (split): every wave of a workgroup of 4 works on pages of its own, codes straight into LDS stages
 // of the wave, no barrier until the waves' states are merged in LDS; up to 32 rows two workgroups share a CU, with more rows a
-// wave has a SIMD's registers to itself.  Long contexts run at the memory's rate (8 bits, 40 / 8 heads: 5.1 to 5.4 TB/s with
-// 3 to 9 nodes), with more rows at that of issue (16 nodes 3.8 TB/s, 610 TFLOP/s; 4 bits 690): a step of 80 rows holds 1280
-// cycles of MFMA in some 4800, one wave's chain of products, softmax and products.  More rows (shared): decoding codes for 64
-// rows costs as much as their softmax, so the 8 waves of a workgroup decode a tile of 4 pages together, as MFMA fragments in
-// LDS, and each runs it against rows of its own (64 nodes: 910 to 1010 TFLOP/s; a large fp16 matrix product
-// reaches 1140 here).  Bound by issue there: MFMA takes 41 % and VALU 56 % of a SIMD's cycles, at a clock of 2.0 GHz under
-// that load, and the two waves of a SIMD hardly overlap them (the products at a higher wave priority: 3 %; staggering the
-// waves' shares of decoding: nothing).
-// 24 nodes (one group of rows a wave: each fragment read from LDS feeds one product): 600 TFLOP/s.
+// wave has a SIMD's registers to itself.  Long contexts (16 sequences up to 32768 tokens, 40 / 8 heads, 8 bits) run at 5.2, 4.8
+// and 4.7 TB/s with 3, 5 and 9 nodes, what the memory gives here; with more rows issue takes over (16 nodes 3.2 to 3.5 TB/s,
+// 520 to 560 TFLOP/s; 4 bits 590): a step of 80 rows holds 1280 cycles of MFMA in some 5000, one wave's chain of products,
+// softmax and products.  More rows (shared): decoding codes for 64 rows costs as much as their softmax, so the 8 waves of a
+// workgroup decode a tile of 4 pages together, as MFMA fragments in LDS, and each runs it against rows of its own (64 nodes:
+// 810 to 830 TFLOP/s at 8 bits, 870 to 920 at 4; a large fp16 matrix product reaches 1140 here).  Bound by issue there: MFMA
+// takes 41 % and VALU 56 % of a SIMD's cycles, at a clock of 2.0 GHz under that load, and the two waves of a SIMD hardly
+// overlap them (the products at a higher wave priority: 3 %; staggering the waves' shares of decoding: nothing).
+// 24 nodes (one group of rows a wave: each fragment read from LDS feeds one product): 520 to 590 TFLOP/s.
 //
 // Work split: a unit is (sequence, kv head, tile of rows), its step 0 the nodes, each further one a workgroup's pages at a
 // time.  The steps of all units in a row are dealt to the workgroups in equal runs, whatever the lengths: a unit inside
