@@ -393,6 +393,97 @@ int exl3_verify_drafts(const float* target_probs, const float* draft_probs, cons
                        const float* uniform, const int* num_nodes, int batch, int nodes, int vocab, int* accepted_nodes,
                        int* counts, int* out_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Around the attention and at the ends of a serving step -----------------------------------------------------------
+ * No counterpart in the reference: its engines bring these steps themselves.  What a call writes overlaps nothing else of
+ * the call, but where in-place use is named. */
+
+/* Workspace bytes of exl3_kv_step_plan.  No zero-fill needed. */
+size_t exl3_kv_step_plan_workspace_bytes(int batch);
+/* The pages, rows and slots of a step from the requests' lengths, on the device.  Sequence b holds seq_lens[b] tokens (clamped
+ * into its table row) and asks for new_lens[b] more, or gives its last -new_lens[b] tokens up (all of them, at most).
+ *   free_pages int32 [num_free]: a ring of free page ids; free_state int32 [2]: the place of its first live entry, and how
+ *     many are live.  Pages are taken from its beginning, in order of b, and written behind the others of the sequence into
+ *     page_table int32 [batch][max_pages]; pages that a shrinking sequence gives up go to its end.  free_state_out gets the
+ *     state after the step (it may be free_state itself).  A page is in the ring or in one table row, never in both.
+ *   A sequence gets all of its tokens or none: none when its table row is too short, when its rows pass `rows`, or when the
+ *     pages asked for so far, its own among them, are more than there are (one that needs no page still gets its tokens).
+ *   row_start int32 [batch + 1]: the running sums of the tokens asked for (at most `rows`); counts int32 [batch]: the tokens
+ *     got, what exl3_kv_append takes as counts; lens_after int32 [batch].
+ *   Per row r of the step's `rows` (row_start[b] + i is new token i of b): positions int32, its position; row_lens int32, the
+ *     tokens that it sees (position + 1); row_seq int32, b; slots int64, page * 16 + position % 16.  -1, 0, -1, -1 for rows
+ *     of refused sequences and behind the last one.
+ * Deterministic; one or two launches; batch * max_pages below 2^30, rows below 2^28.  Calls that share a workspace must not
+ * overlap. */
+int exl3_kv_step_plan(int* page_table, int max_pages, const int* seq_lens, const int* new_lens, int batch, int page_size,
+                      int* free_pages, int num_free, const int* free_state, int* free_state_out, int rows, int* row_start,
+                      int* counts, int* lens_after, int* positions, int* row_lens, int* row_seq, long long* slots,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* From one block of a model to the next: for each row x (a block's output) and r (the residual stream) of `dim` values
+ * (1 to 65536; strides ld_* in elements)
+ *   u = x, or with post_weight  x * rsqrt(mean(x^2) + eps) * post_weight
+ *   h = r + scale * act(gate) * u         act: the value itself, or its sigmoid (gate_sigmoid)
+ *   y = h * rsqrt(mean(h^2) + eps) * weight
+ * with 1 + w for both weights where weight_offset is set.  gate_kind 0: no gate; 1: [dim]; 2: a value a row, ld_g apart; 3:
+ * [rows][dim].  residual NULL: r = 0.  weight and y both NULL: h alone; h NULL: y alone.  x and y fp16 | bf16 (x_type),
+ * residual and h fp16 | bf16 | fp32 (r_type), weights w_type, gate g_type; y, h contiguous.  fp32 inside, y from the h before
+ * its rounding.  h may be the residual itself where that is contiguous. */
+int exl3_add_norm(const void* x, int x_type, long long ld_x, const void* residual, int r_type, long long ld_r,
+                  const void* weight, const void* post_weight, int w_type, int weight_offset, const void* gate, int g_type,
+                  int gate_kind, long long ld_g, int gate_sigmoid, float scale, float eps, int rows, int dim, void* y, void* h,
+                  void* stream);
+
+/* bounds [num_pages][num_kv_heads][2][row of codes, as k_cache has them]: the largest and the smallest key code of every
+ * channel over a page's tokens, made anew for the pages that hold tokens first[b] .. seq_lens[b] - 1 of sequence b (first
+ * NULL: 0), of which the last max_new at most.  After exl3_kv_append: first = the lengths before it, seq_lens those after.
+ * Pages outside [0, num_pages) are left out. */
+int exl3_kv_page_bounds(const void* k_cache, int num_pages, const int* page_table, int max_pages, const int* seq_lens,
+                        const int* first, int max_new, int batch, int num_kv_heads, int head_dim, int page_size, int bits,
+                        void* bounds, void* stream);
+
+/* Rows of the two calls below: row r is a query of sequence row_seq[r] (int32 [rows]; NULL: sequence r, rows = batch) that sees
+ * its first seq_lens[r] tokens (int32 [rows]).  A row of another sequence than 0 .. batch - 1 sees none.  q fp16
+ * [rows][num_q_heads][128], row stride ld_q. */
+/* Workspace bytes of exl3_kv_select_pages.  No zero-fill needed. */
+size_t exl3_kv_select_workspace_bytes(int rows, int num_kv_heads, int max_pages);
+/* pages_out int32 [rows][num_kv_heads][top]: the pages (numbers within the sequence, ascending, -1 behind the last) that a row
+ * reads: all where it sees at most `top`, else its first `first` and last `last` ones (last >= 1, first + last <= top), and of
+ * the rest those of the largest worth, ties to the lower page:
+ *   worth = max over the group's heads of fp32(S * (a * k_scale)),  a = max |q|,  S = sum_d q8_d (q8_d > 0 ? hi_d : lo_d),
+ *   q8 = rint(127 q / a) to nearest even (infinities +-127 and NaN 0, neither counts for a),
+ * an upper bound of the page's logits but for the rounding of q8 and the (positive) scale of the softmax.  NaN worths come
+ * last.  Two launches; deterministic; calls that share a workspace must not overlap. */
+int exl3_kv_select_pages(const void* q, long long ld_q, const void* k_scale, const void* bounds, int num_pages,
+                         const int* page_table, int batch, int max_pages, const int* row_seq, const int* seq_lens, int rows,
+                         int num_q_heads, int num_kv_heads, int head_dim, int page_size, int bits, int top, int first,
+                         int last, int* pages_out, void* workspace, size_t workspace_bytes, void* stream);
+/* Workspace bytes of exl3_kv_sparse_attention (0 where it needs none).  No zero-fill needed. */
+size_t exl3_kv_sparse_workspace_bytes(int rows, int num_q_heads, int num_kv_heads, int top);
+/* out fp16 [rows][num_q_heads][128] = softmax(sm_scale q . K^T) V over those tokens of the pages pages[r][kv head][0 .. top)
+ * that the row sees; entries that are no page of what it sees are left out, the others are distinct.  A row that sees nothing
+ * gives zeros.  One or two launches; deterministic; calls that share a workspace must not overlap. */
+int exl3_kv_sparse_attention(const void* q, long long ld_q, const void* k_cache, const void* v_cache, const void* k_scale,
+                             const void* v_scale, int num_pages, const int* page_table, int batch, int max_pages,
+                             const int* row_seq, const int* seq_lens, int rows, int num_q_heads, int num_kv_heads,
+                             int head_dim, int page_size, int bits, const int* pages, int top, float sm_scale, void* out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of exl3_sample.  No zero-fill needed. */
+size_t exl3_sample_workspace_bytes(int rows, int vocab);
+/* Tokens from logits [rows][vocab] (fp16 | bf16 | fp32, row stride ld; NaN as -inf; vocab up to 2^24): with w = exp((l - max l) /
+ * temperature) and the elements in order of falling logits (ties by rising index), kept is the shortest of
+ *   the first top_k (<= 0: all);  those whose predecessors have less than top_p of the sum of w over the first top_k (>= 1 or
+ *   NaN: all);  those with w >= min_p (<= 0 or NaN: all; above 1 as 1);
+ * and the first element always.  tokens int32 [rows]: the smallest v whose running sum of w over the kept passes uniform[r]
+ * times their sum (uniform fp32 in [0, 1)); probs fp32 [rows][vocab]: w over that sum, 0 for the others.  Either may be NULL.
+ * temperature, top_p, min_p fp32 [rows] and top_k int32 [rows] per row, or NULL: all_* for every row.  A temperature that is
+ * not above 0 keeps the first element alone.  A row without a logit above -inf gives -1, and zeros.  Weights and sums are in 64
+ * bits; deterministic; calls that share a workspace must not overlap. */
+int exl3_sample(const void* logits, int type, long long ld, int rows, int vocab, const float* uniform,
+                const float* temperature, double all_temperature, const int* top_k, int all_top_k, const float* top_p,
+                double all_top_p, const float* min_p, double all_min_p, int* tokens, float* probs, void* workspace,
+                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -49,7 +49,8 @@ class Exl3MoeClass(ctypes.Structure):
                 ("K_gate_up", ctypes.c_int), ("K_down", ctypes.c_int)]
 
 
-_P, _I, _SZ, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong, ctypes.c_float
+_P, _I, _SZ, _LL, _F, _D = (ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong, ctypes.c_float,
+                            ctypes.c_double)
 _SIGNATURES: dict[str, tuple] = {
     "exl3_abi_version": (_I, []),
     "exl3_last_error": (ctypes.c_char_p, []),
@@ -97,6 +98,18 @@ _SIGNATURES: dict[str, tuple] = {
                                     _I, _I, _I, _F, _P, _P, _SZ, _P]),
     "exl3_verify_workspace_bytes": (_SZ, [_I, _I]),
     "exl3_verify_drafts": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "exl3_kv_step_plan_workspace_bytes": (_SZ, [_I]),
+    "exl3_kv_step_plan": (_I, [_P, _I, _P, _P, _I, _I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "exl3_add_norm": (_I, [_P, _I, _LL, _P, _I, _LL, _P, _P, _I, _I, _P, _I, _I, _LL, _I, _F, _F, _I, _I, _P, _P, _P]),
+    "exl3_kv_page_bounds": (_I, [_P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "exl3_kv_select_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "exl3_kv_select_pages": (_I, [_P, _LL, _P, _P, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _SZ,
+                                  _P]),
+    "exl3_kv_sparse_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "exl3_kv_sparse_attention": (_I, [_P, _LL, _P, _P, _P, _P, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _F, _P,
+                                      _P, _SZ, _P]),
+    "exl3_sample_workspace_bytes": (_SZ, [_I, _I]),
+    "exl3_sample": (_I, [_P, _I, _LL, _I, _I, _P, _P, _D, _P, _I, _P, _D, _P, _D, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

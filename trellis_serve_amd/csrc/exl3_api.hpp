@@ -51,6 +51,24 @@ int xcd_probe(int device);
 // whether a probe has passed (and EXL3_GEMV_XCD_LOCAL is not 0): workgroups whose ids agree mod 8 share an XCD
 bool xcd_groups_ok();
 
+// A tensor's bytes, to tell whether what a call writes meets anything else of it
+struct Span {
+  const void* at;
+  size_t bytes;
+  bool meets(const Span& o) const {
+    const uintptr_t a = (uintptr_t)at, b = (uintptr_t)o.at;
+    return at && o.at && a < b + o.bytes && b < a + bytes;
+  }
+};
+// The first `written` of the spans meet no other of them
+template <int N>
+inline bool apart(const Span (&all)[N], int written) {
+  for (int i = 0; i < written; i++)
+    for (int j = i + 1; j < N; j++)
+      if (all[i].meets(all[j])) return false;
+  return true;
+}
+
 inline bool valid_bits(int K) { return K == 2 || K == 3 || K == 4 || K == 5 || K == 6 || K == 8; }
 inline bool valid_cb(int cb) { return cb >= 0 && cb <= 2; }
 

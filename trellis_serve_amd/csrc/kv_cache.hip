@@ -331,15 +331,6 @@ static int check_cache(const char* what, const void* k_cache, const void* v_cach
   return EXL3_OK;
 }
 
-struct Span {
-  const void* at;
-  size_t bytes;
-  bool meets(const Span& o) const {
-    const uintptr_t a = (uintptr_t)at, b = (uintptr_t)o.at;
-    return at && o.at && a < b + o.bytes && b < a + bytes;
-  }
-};
-
 }  // namespace exl3
 
 using namespace exl3;
@@ -378,9 +369,7 @@ extern "C" int exl3_kv_append(const void* k, const void* v, int x_bf16, long lon
                       {page_table, (size_t)batch * max_pages * ints}, {seq_lens, batch * ints},
                       {row_start, (batch + (size_t)1) * ints}, {select, (size_t)batch * max_new * ints},
                       {counts, batch * ints}};
-  for (int i = 0; i < 4; i++)
-    for (int j = i + 1; j < (int)(sizeof(all) / sizeof(all[0])); j++)
-      EXL3_CHECK_ARG(!all[i].meets(all[j]), "exl3_kv_append: a cache or its scales overlap another tensor of the call");
+  EXL3_CHECK_ARG(apart(all, 4), "exl3_kv_append: a cache or its scales overlap another tensor of the call");
   const KvAppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), ld_k, ld_v, rows, row_start,
                        rows_per_seq, select, counts, max_new, static_cast<uint8_t*>(k_cache),
                        static_cast<uint8_t*>(v_cache), static_cast<uint16_t*>(k_scale),

@@ -1,0 +1,195 @@
+// A serving step's pages, rows and slots from the requests' lengths (gfx950).
+//
+// Sequence b holds len_b tokens and asks for new_b more, or gives its last -new_b up.  Pages hold 16 tokens:
+//   have = ceil(len / 16);  need = ceil((len + new) / 16) - have  of a sequence that grows, taken from a ring of free pages
+//   in order of b: b's first is entry (need_0 + .. + need_b-1) of the ring's live part;  give = have - ceil((len + new) /
+//   16) of one that shrinks, put behind the live part in order of b.
+// A sequence is refused (it gets no token, its rows are -1) when its table row or the step's rows end before its tokens, or
+// when the running sum of need passes the live part: what one sequence gets depends on those before it only through sums, so
+// the whole is two prefix sums and a copy.  Saturating sums of numbers >= 0 are associative, which keeps them in 32 bits.
+//
+// step_plan_kernel: one workgroup scans the sequences, 1024 at a time, and, where the step is small, fills the rows too.
+// Otherwise step_fill_kernel does: waves of one sequence write its rows, its new table entries and its returned pages.  The
+// ring's state may be updated in place, since only the first kernel reads it.
+#include <algorithm>
+
+#include "exl3_api.hpp"
+#include "kv_device.hpp"
+
+namespace exl3 {
+
+constexpr int kPlanThreads = 1024;
+
+struct StepPlanArgs {
+  int* table;
+  int max_pages;
+  const int *lens, *new_lens;
+  int batch;
+  int* ring;
+  int ring_pages;
+  const int* state;
+  int* state_out;
+  int rows;
+  int *row_start, *counts, *lens_after, *positions, *row_lens, *row_seq;
+  long long* slots;
+  int* base;  // [batch + 2]: a sequence's first taken (or returned) page; then the ring's head and count before the step
+  int slices; // waves per sequence of the fill
+};
+
+// inclusive scan over the workgroup of `v`, sums stopping at `most` (< 2^30); `carry` is what came before and becomes the
+// total; part: LDS, one int a wave
+__device__ __forceinline__ int plan_scan(int v, int most, int& carry, int* part) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int s = min(v, most);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(s, d);
+    s = lane >= d ? min(s + o, most) : s;
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  int before = carry, total = carry;
+  for (int w = 0; w < kPlanThreads / 64; w++) {
+    if (w == wave) before = total;
+    total = min(total + part[w], most);
+  }
+  carry = total;
+  return min(before + s, most);
+}
+
+__device__ __forceinline__ int plan_pages(int tokens) { return (int)(((unsigned)tokens + kPage - 1) / kPage); }
+
+// Slice `slice` of sequence b's rows, table entries and returned pages, or (b == batch) of the rows behind the last sequence
+__device__ __forceinline__ void plan_fill(const StepPlanArgs& a, int b, int slice) {
+  const int lane = threadIdx.x & 63, first = slice * 64 + lane, step = a.slices * 64;
+  if (b == a.batch) {
+    for (int r = a.row_start[b] + first; r < a.rows; r += step)
+      a.positions[r] = -1, a.row_lens[r] = 0, a.row_seq[r] = -1, a.slots[r] = -1;
+    return;
+  }
+  const int len = min(max(a.lens[b], 0), a.max_pages * kPage), asked = a.new_lens[b], have = plan_pages(len);
+  const int base = a.base[b];
+  const unsigned head = a.base[a.batch], P = a.ring_pages;
+  int* row = a.table + (size_t)b * a.max_pages;
+  if (asked < 0) {
+    const unsigned to = head + (unsigned)a.base[a.batch + 1] + (unsigned)base;
+    const int keep = plan_pages(a.lens_after[b]);
+    for (int j = first; j < have - keep; j += step) a.ring[(to + j) % P] = row[keep + j];
+    return;
+  }
+  const int r0 = a.row_start[b], n = a.row_start[b + 1] - r0, count = a.counts[b];
+  const int need = plan_pages(len + count) - have;
+  auto taken = [&](int j) {  // base + j is below the live pages
+    const unsigned at = head + base + j;
+    return a.ring[at < P ? at : at - P];
+  };
+  for (int j = first; j < need; j += step) row[have + j] = taken(j);
+  for (int i = first; i < n; i += step) {
+    const int r = r0 + i, pos = len + i, lp = pos / kPage;
+    const bool live = i < count;
+    int page = 0;
+    if (live) page = lp < have ? row[lp] : taken(lp - have);
+    a.positions[r] = live ? pos : -1;
+    a.row_lens[r] = live ? pos + 1 : 0;
+    a.row_seq[r] = live ? b : -1;
+    a.slots[r] = live ? (long long)page * kPage + pos % kPage : -1;
+  }
+}
+
+template <bool FILL>
+__global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(const StepPlanArgs a) {
+  __shared__ int part[kPlanThreads / 64];
+  const int head = (int)((unsigned)a.state[0] % (unsigned)a.ring_pages);
+  const int live = min(max(a.state[1], 0), a.ring_pages);
+  constexpr int kMost = (1 << 30) - 1;
+  const int room = a.max_pages * kPage;
+  int rows = 0, pages = 0, given = 0, popped = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
+    const bool in = b < a.batch;
+    const int len = in ? min(max(a.lens[b], 0), room) : 0, asked = in ? a.new_lens[b] : 0;
+    const int grow = max(asked, 0), have = plan_pages(len);
+    const int end = plan_scan(grow, a.rows + 1, rows, part);
+    const bool fits = grow <= room - len && end <= a.rows;
+    const int need = fits ? plan_pages(len + grow) - have : 0;
+    const int sum = plan_scan(need, kMost, pages, part);
+    const bool ok = fits && (need == 0 || sum <= live);
+    const int left = asked < 0 ? (asked < -len ? 0 : len + asked) : len;
+    const int give = have - plan_pages(left);
+    const int back = plan_scan(give, kMost, given, part);
+    plan_scan(ok ? need : 0, kMost, popped, part);
+    if (in) {
+      a.row_start[b + 1] = min(end, a.rows);
+      a.counts[b] = ok ? grow : 0;
+      a.lens_after[b] = asked < 0 ? left : ok ? len + grow : len;
+      a.base[b] = asked < 0 ? back - give : sum - need;
+    }
+  }
+  if (threadIdx.x == 0) {
+    a.row_start[0] = 0;
+    a.base[a.batch] = head, a.base[a.batch + 1] = live;
+    const unsigned at = (unsigned)head + (unsigned)popped;
+    a.state_out[0] = (int)(at % (unsigned)a.ring_pages);
+    a.state_out[1] = min(live - popped + given, a.ring_pages);
+  }
+  if constexpr (FILL) {
+    __syncthreads();
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int i = wave; i < (a.batch + 1) * a.slices; i += kPlanThreads / 64) plan_fill(a, i / a.slices, i % a.slices);
+  }
+}
+
+__global__ __launch_bounds__(256) void step_fill_kernel(const StepPlanArgs a) {
+  const long long i = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= (long long)(a.batch + 1) * a.slices) return;
+  plan_fill(a, (int)(i / a.slices), (int)(i % a.slices));
+}
+
+}  // namespace exl3
+
+using namespace exl3;
+
+extern "C" size_t exl3_kv_step_plan_workspace_bytes(int batch) {
+  return batch <= 0 ? 0 : ((size_t)batch + 2) * sizeof(int);
+}
+
+extern "C" int exl3_kv_step_plan(int* page_table, int max_pages, const int* seq_lens, const int* new_lens, int batch,
+                                 int page_size, int* free_pages, int num_free, const int* free_state, int* free_state_out,
+                                 int rows, int* row_start, int* counts, int* lens_after, int* positions, int* row_lens,
+                                 int* row_seq, long long* slots, void* workspace, size_t workspace_bytes, void* stream) {
+  EXL3_CHECK_ARG(page_size == kPage, "exl3_kv_step_plan: page_size = %d (supported: 16)", page_size);
+  EXL3_CHECK_ARG(batch >= 0 && max_pages >= 1 && max_pages <= (1 << 26) && (long long)batch * max_pages < (1LL << 30) &&
+                     num_free >= 1 && num_free <= (1 << 28) && rows >= 0 && rows < (1 << 28),
+                 "exl3_kv_step_plan: batch = %d, max_pages = %d, free pages = %d, rows = %d", batch, max_pages, num_free,
+                 rows);
+  if (batch == 0 && rows == 0) return EXL3_OK;
+  EXL3_CHECK_ARG(batch >= 1, "exl3_kv_step_plan: %d rows of no sequence", rows);
+  EXL3_CHECK_ARG(page_table && seq_lens && new_lens && free_pages && free_state && free_state_out && row_start && counts &&
+                     lens_after && (rows == 0 || (positions && row_lens && row_seq && slots)),
+                 "exl3_kv_step_plan: null pointer");
+  const size_t need = exl3_kv_step_plan_workspace_bytes(batch);
+  EXL3_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0,
+                 "exl3_kv_step_plan: workspace %zu bytes, need %zu (4-byte aligned)", workspace_bytes, need);
+  const size_t n = (size_t)batch * sizeof(int), r = (size_t)rows * sizeof(int);
+  const Span all[] = {{page_table, n * max_pages}, {free_pages, num_free * sizeof(int)}, {free_state_out, 2 * sizeof(int)},
+                      {row_start, n + sizeof(int)}, {counts, n}, {lens_after, n}, {positions, r}, {row_lens, r},
+                      {row_seq, r}, {slots, 2 * r}, {workspace, need}, {seq_lens, n}, {new_lens, n},
+                      {free_state == free_state_out ? nullptr : free_state, 2 * sizeof(int)}};
+  EXL3_CHECK_ARG(apart(all, 11), "exl3_kv_step_plan: what the call writes overlaps another tensor of it");
+  StepPlanArgs a{page_table, max_pages, seq_lens, new_lens, batch, free_pages, num_free, free_state, free_state_out, rows,
+                 row_start, counts, lens_after, positions, row_lens, row_seq, slots, static_cast<int*>(workspace), 1};
+  if (batch <= 256 && rows <= 2048) {
+    step_plan_kernel<true><<<1, kPlanThreads, 0, as_stream(stream)>>>(a);
+    EXL3_CHECK_LAUNCH();
+    return EXL3_OK;
+  }
+  // waves per sequence: one while the sequences fill the card, then enough for about 256 rows a wave on average
+  a.slices = (int)std::max<long long>(1, std::min<long long>(64, rows / (256LL * batch)));
+  step_plan_kernel<false><<<1, kPlanThreads, 0, as_stream(stream)>>>(a);
+  EXL3_CHECK_LAUNCH();
+  const long long waves = (long long)(batch + 1) * a.slices;
+  step_fill_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, as_stream(stream)>>>(a);
+  EXL3_CHECK_LAUNCH();
+  return EXL3_OK;
+}

@@ -7,6 +7,7 @@ Nothing here computes on the CPU: a missing library raises ExtensionMissing.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -1138,3 +1139,377 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, uniform: tor
         counts.data_ptr(), out_tokens.data_ptr(), ws.data_ptr(), ws.nbytes,
         torch._C._cuda_getCurrentRawStream(index)), "verify_drafts")
     return accepted, counts, out_tokens
+
+
+# ---- Around the attention and at the ends of a serving step: pages and rows from the requests' lengths, the step between two
+# blocks, attention over chosen pages, sampling.  Workspaces as above.
+
+class StepPlan(NamedTuple):
+    """What kv_step_plan returns, int32 (slots int64): of the sequences row_start [B + 1], counts [B], lens_after [B]; of the
+    step's rows positions, row_lens, row_seq and slots [rows]."""
+    row_start: torch.Tensor
+    counts: torch.Tensor
+    lens_after: torch.Tensor
+    positions: torch.Tensor
+    row_lens: torch.Tensor
+    row_seq: torch.Tensor
+    slots: torch.Tensor
+
+
+def kv_step_plan(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+                 free_state: torch.Tensor, rows: int, state_out: torch.Tensor | None = None) -> StepPlan:
+    """The pages, rows and slots of a step from the requests' lengths, without the host knowing them.  Sequence b holds
+    seq_lens[b] tokens and asks for new_lens[b] more (int32 [B]), or, below 0, gives its last -new_lens[b] ones up.  free_pages
+    int32 is a ring of free page ids, free_state int32 [2] the place of its first live entry and how many are live: pages are
+    taken from its beginning in order of b and written into page_table int32 [B, max_pages]; pages given up go to its end;
+    state_out (None: free_state itself) gets its state after the step.  A sequence gets all of its tokens or none: none when its
+    table row is too short, its rows pass `rows`, or the pages asked for so far are more than there are.
+    Returns, for the step's `rows` rows (new token i of b is row row_start[b] + i): row_start (kv_append's), counts (the tokens
+    got; kv_append's), lens_after, positions (qk_norm_rope's), row_lens and row_seq (kv_select_pages' and
+    kv_sparse_attention's seq_lens and row_seq), slots (page * 16 + place).  Rows of refused sequences and behind the last one
+    have -1, 0, -1 and -1."""
+    shape = page_table.shape
+    if page_table.dtype != torch.int32 or len(shape) != 2 or not page_table.is_contiguous():
+        raise ValueError(f"page_table must be a contiguous int32 [B, max_pages] tensor, got {page_table.dtype} {tuple(shape)}")
+    B, max_pages = shape
+    _check_int32(seq_lens, "seq_lens", (B,))
+    _check_int32(new_lens, "new_lens", (B,))
+    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        raise ValueError(f"free_pages must be a contiguous int32 [P] tensor, got {free_pages.dtype} {tuple(free_pages.shape)}")
+    _check_int32(free_state, "free_state", (2,))
+    if state_out is None:
+        state_out = free_state
+    else:
+        _check_int32(state_out, "state_out", (2,))
+    if rows < 0:
+        raise ValueError(f"rows = {rows}")
+    index = _cuda_index(page_table, seq_lens, new_lens, free_pages, free_state, state_out)
+    if not _current(index):
+        with torch.cuda.device(index):
+            return kv_step_plan(page_table, seq_lens, new_lens, free_pages, free_state, rows, state_out)
+    # one allocation, the workspace at its end
+    buf = page_table.new_empty(5 * rows + 4 * B + 3)
+    slots, row_start, counts, after, positions, row_lens, row_seq, ws = buf.split(
+        (2 * rows, B + 1, B, B, rows, rows, rows, B + 2))
+    slots = slots.view(torch.int64)
+    if B == 0:
+        row_start.zero_()
+    _lib.check(_lib.load().exl3_kv_step_plan(
+        page_table.data_ptr(), max_pages, seq_lens.data_ptr(), new_lens.data_ptr(), B, 16, free_pages.data_ptr(),
+        free_pages.numel(), free_state.data_ptr(), state_out.data_ptr(), rows, row_start.data_ptr(), counts.data_ptr(),
+        after.data_ptr(), positions.data_ptr(), row_lens.data_ptr(), row_seq.data_ptr(), slots.data_ptr(), ws.data_ptr(),
+        4 * (B + 2), torch._C._cuda_getCurrentRawStream(index)), "kv_step_plan")
+    return StepPlan(row_start, counts, after, positions, row_lens, row_seq, slots)
+
+
+def _row_stride(t: torch.Tensor, name: str, shape: tuple, dtypes) -> int:
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: a row's values must be contiguous, got strides {stride}")
+    return stride[0] if shape[0] > 1 else shape[1]
+
+
+def add_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, eps: float = 1e-6,
+             post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_sigmoid: bool = False,
+             scale: float = 1.0, unit_offset: bool = False,
+             out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None
+             ) -> tuple[torch.Tensor | None, torch.Tensor]:
+    """From one block to the next in one launch: u = x, a block's output fp16|bf16 [T, dim] (with post_weight its RMS norm);
+    h = residual + scale * gate * u; y = RMS norm of h by `weight`.  Returns (y, h): y in x's type, h in the residual's (fp16,
+    bf16 or fp32; x's where there is none).  weight None: y is None (after the last block of a part).  gate [dim], [T, 1] or
+    [T, dim] (taken through a sigmoid with gate_sigmoid); weights and gate fp16|bf16|fp32, weights of one type, as 1 + w with
+    unit_offset.  fp32 inside, y from the h before its rounding.  out: (y, h) to write to; h may be the residual itself where
+    that is contiguous."""
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, dim], got {tuple(x.shape)}")
+    shape, dtype = x.shape, x.dtype
+    T, dim = shape
+    ld_x = _row_stride(x, "x", shape, _HALVES)
+    r_dtype, ld_r = dtype, dim
+    if residual is not None:
+        ld_r = _row_stride(residual, "residual", shape, _WEIGHT_TYPE)
+        r_dtype = residual.dtype
+    w_type = g_type = kind = ld_g = 0
+    w_dtype = None
+    for name, w in (("weight", weight), ("post_weight", post_weight)):
+        if w is not None:
+            w_dtype = w_dtype or w.dtype
+            if w.dtype != w_dtype or w_dtype not in _WEIGHT_TYPE or w.shape != (dim,) or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [{dim}] tensor, both weights of one type (fp16, bf16, fp32)")
+            w_type = _WEIGHT_TYPE[w_dtype]
+    if gate is not None:
+        if gate.dtype not in _WEIGHT_TYPE:
+            raise ValueError(f"gate must be fp16, bf16 or fp32, got {gate.dtype}")
+        g_type, g_shape = _WEIGHT_TYPE[gate.dtype], gate.shape
+        if g_shape == (dim,) and (gate.is_contiguous()):
+            kind = 1
+        elif g_shape == shape and (dim > 1):
+            kind, ld_g = 3, _row_stride(gate, "gate", shape, _WEIGHT_TYPE)
+        elif g_shape == (T, 1):
+            kind, ld_g = 2, gate.stride(0) if T > 1 else 1
+        else:
+            raise ValueError(f"gate must be a contiguous [{dim}] tensor, [{T}, 1] or [{T}, {dim}], got {tuple(g_shape)}")
+        if kind == 2 and ld_g < 1:
+            raise ValueError(f"gate: strides {gate.stride()}")
+    y = h = None
+    if out is not None:
+        y, h = out
+        if (y is None) != (weight is None):
+            raise ValueError("out[0] comes with a weight")
+        if y is not None:
+            _check_out(y, shape, x, (dtype,))
+        if h is not None:
+            _check_out(h, shape, x, (r_dtype,))
+    index = _cuda_index(x, residual, weight, post_weight, gate)
+    if not _current(index):
+        with torch.cuda.device(index):
+            return add_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, unit_offset, out)
+    if y is None and weight is not None:
+        y = x.new_empty(shape)
+    if h is None:
+        h = x.new_empty(shape, dtype=r_dtype)
+    _lib.check(_lib.load().exl3_add_norm(
+        x.data_ptr(), dtype == torch.bfloat16, ld_x, _ptr(residual), _WEIGHT_TYPE[r_dtype], ld_r, _ptr(weight),
+        _ptr(post_weight), w_type, unit_offset, _ptr(gate), g_type, kind, ld_g, gate_sigmoid, scale, eps, T, dim, _ptr(y),
+        h.data_ptr(), torch._C._cuda_getCurrentRawStream(index)), "add_norm")
+    return y, h
+
+
+def kv_page_bounds(k_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int, bounds: torch.Tensor,
+                   first: torch.Tensor | None = None, max_new: int | None = None) -> None:
+    """Makes anew, in `bounds` ([P, Hkv, 2, 16 * bits], 1-byte like k_cache and packed like its rows), the largest and the
+    smallest key code of every channel of the pages that hold tokens first[b] .. seq_lens[b] - 1 of sequence b (int32 [B]; first
+    None: 0), of which the last `max_new` at most, if given (it sizes the launch).  After kv_append: first = the lengths before
+    it, seq_lens = those after (kv_step_plan's lens_after).  Bounds are codes: they go with the page's k_scale."""
+    if bits != 8 and bits != 4:
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[2] != 16 or shape[3] != 16 * bits or k_cache.element_size() != 1:
+        raise ValueError(f"k_cache must be 1-byte [P, Hkv, 16, {16 * bits}] at {bits} bits, got {tuple(shape)}")
+    P, Hkv = shape[0], shape[1]
+    if bounds.shape != (P, Hkv, 2, 16 * bits) or bounds.element_size() != 1:
+        raise ValueError(f"bounds must be 1-byte [{P}, {Hkv}, 2, {16 * bits}], got {bounds.dtype} {tuple(bounds.shape)}")
+    table = page_table.shape
+    if page_table.dtype != torch.int32 or len(table) != 2:
+        raise ValueError("page_table must be int32 [B, max_pages]")
+    B, max_pages = table
+    if not (k_cache.is_contiguous() and bounds.is_contiguous() and page_table.is_contiguous()):
+        raise ValueError("the cache, the bounds and the page table must be contiguous")
+    _check_int32(seq_lens, "seq_lens", (B,))
+    _check_int32(first, "first", (B,))
+    max_new = 16 * max_pages if max_new is None else min(max_new, 16 * max_pages)
+    if max_new < 0:
+        raise ValueError(f"max_new = {max_new}")
+    index = _cuda_index(k_cache, page_table, seq_lens, bounds, first)
+    if not _current(index):
+        with torch.cuda.device(index):
+            return kv_page_bounds(k_cache, page_table, seq_lens, bits, bounds, first, max_new)
+    _lib.check(_lib.load().exl3_kv_page_bounds(
+        k_cache.data_ptr(), P, page_table.data_ptr(), max_pages, seq_lens.data_ptr(), _ptr(first), max_new, B, Hkv, _HEAD_DIM,
+        16, bits, bounds.data_ptr(), torch._C._cuda_getCurrentRawStream(index)), "kv_page_bounds")
+
+
+def _check_rows(q: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, row_seq: torch.Tensor | None,
+                Hkv: int) -> tuple[int, int, int, int, int]:
+    """Query rows of a paged cache; returns (row stride, rows, query heads, sequences, table width)."""
+    ld_q = _token_stride(q, "q", 3, _FP16)
+    R, Hq, _ = q.shape
+    if Hkv < 1 or Hq % Hkv or not 1 <= Hq // Hkv <= 16:
+        raise ValueError(f"1 to 16 query heads per kv head, got heads {Hq} / {Hkv}")
+    table = page_table.shape
+    if page_table.dtype != torch.int32 or len(table) != 2 or not page_table.is_contiguous():
+        raise ValueError("page_table must be a contiguous int32 [B, max_pages] tensor")
+    _check_int32(seq_lens, "seq_lens", (R,))
+    _check_int32(row_seq, "row_seq", (R,))
+    if row_seq is None and R != table[0]:
+        raise ValueError(f"{R} rows of {table[0]} sequences need row_seq")
+    return ld_q, R, Hq, table[0], table[1]
+
+
+def kv_select_workspace_bytes(rows: int, num_kv_heads: int, max_pages: int) -> int:
+    """Bytes of a `workspace` for kv_select_pages at this shape."""
+    return _lib.load().exl3_kv_select_workspace_bytes(rows, num_kv_heads, max_pages)
+
+
+def kv_select_pages(q: torch.Tensor, bounds: torch.Tensor, k_scale: torch.Tensor, page_table: torch.Tensor,
+                    seq_lens: torch.Tensor, bits: int, top: int, first: int = 1, last: int = 2,
+                    row_seq: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The pages that each query row is to read: int32 [R, Hkv, top], numbers within the sequence, ascending, -1 behind the
+    last.  q fp16 [R, Hq, 128]; row r is a query of sequence row_seq[r] (int32 [R]; None: r) that sees its first seq_lens[r]
+    tokens (int32 [R]; a decode step's lengths with the new token, kv_step_plan's row_lens).  Where it sees more than `top`
+    pages: the first `first` and the last `last` (1 at least) of them, and of the rest those whose bounds (kv_page_bounds) and
+    k_scale allow the largest logit of any of the kv head's queries, in integers of 8 bits a value, ties to the lower page.
+    Serves softmax scales above 0."""
+    if bits != 8 and bits != 4:
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
+    shape = bounds.shape
+    if len(shape) != 4 or shape[2] != 2 or shape[3] != 16 * bits or bounds.element_size() != 1 or not bounds.is_contiguous():
+        raise ValueError(f"bounds must be a contiguous 1-byte [P, Hkv, 2, {16 * bits}] tensor at {bits} bits, got "
+                         f"{bounds.dtype} {tuple(shape)}")
+    P, Hkv = shape[0], shape[1]
+    if k_scale.dtype != torch.float16 or k_scale.shape != (P, Hkv) or not k_scale.is_contiguous():
+        raise ValueError(f"k_scale must be a contiguous fp16 [{P}, {Hkv}] tensor")
+    ld_q, R, Hq, B, max_pages = _check_rows(q, page_table, seq_lens, row_seq, Hkv)
+    if last < 1 or first < 0 or first + last > top:
+        raise ValueError(f"first = {first} and last = {last} (1 at least) of top = {top} pages")
+    if out is not None:
+        _check_out(out, (R, Hkv, top), q, (torch.int32,))
+    index = _cuda_index(q, bounds, k_scale, page_table, seq_lens, row_seq)
+    if not _current(index):
+        with torch.cuda.device(index):
+            return kv_select_pages(q, bounds, k_scale, page_table, seq_lens, bits, top, first, last, row_seq, out, workspace)
+    if out is None:
+        out = seq_lens.new_empty((R, Hkv, top))
+    lib = _lib.load()
+    ws = _call_workspace(workspace, lib.exl3_kv_select_workspace_bytes(R, Hkv, max_pages), q)
+    _lib.check(lib.exl3_kv_select_pages(
+        q.data_ptr(), ld_q, k_scale.data_ptr(), bounds.data_ptr(), P, page_table.data_ptr(), B, max_pages, _ptr(row_seq),
+        seq_lens.data_ptr(), R, Hq, Hkv, _HEAD_DIM, 16, bits, top, first, last, out.data_ptr(), ws.data_ptr(), ws.nbytes,
+        torch._C._cuda_getCurrentRawStream(index)), "kv_select_pages")
+    return out
+
+
+def kv_sparse_workspace_bytes(rows: int, num_q_heads: int, num_kv_heads: int, top: int) -> int:
+    """Bytes of a `workspace` for kv_sparse_attention at this shape (0: it needs none)."""
+    return _lib.load().exl3_kv_sparse_workspace_bytes(rows, num_q_heads, num_kv_heads, top)
+
+
+def kv_sparse_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, bits: int,
+                        pages: torch.Tensor, sm_scale: float | None = None, row_seq: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each query row over the pages chosen for it.  q, page_table, seq_lens and row_seq as kv_select_pages has
+    them, pages int32 [R, Hkv, top] as it returns them (or of another choice: distinct page numbers within the sequence; others
+    are left out), the cache as kv_decode_attention has it.  A row that sees nothing gives zeros.  Returns fp16
+    [R, Hq, 128]."""
+    shape = k_cache.shape
+    if bits != 8 and bits != 4:
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
+    if len(shape) != 4 or shape != v_cache.shape or shape[2] != 16 or shape[3] != 16 * bits:
+        raise ValueError(f"k_cache / v_cache must both be [P, Hkv, 16, {16 * bits}] at {bits} bits, got "
+                         f"{tuple(shape)} / {tuple(v_cache.shape)}")
+    if k_cache.element_size() != 1 or v_cache.element_size() != 1:
+        raise ValueError("caches must hold 1-byte codes (int8 / uint8)")
+    P, Hkv = shape[0], shape[1]
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float16 or t.shape != (P, Hkv) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous fp16 [{P}, {Hkv}] tensor")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    ld_q, R, Hq, B, max_pages = _check_rows(q, page_table, seq_lens, row_seq, Hkv)
+    p_shape = pages.shape
+    if pages.dtype != torch.int32 or len(p_shape) != 3 or p_shape[:2] != (R, Hkv) or not pages.is_contiguous():
+        raise ValueError(f"pages must be a contiguous int32 [{R}, {Hkv}, top] tensor, got {pages.dtype} {tuple(p_shape)}")
+    top = p_shape[2]
+    if out is not None:
+        _check_out(out, (R, Hq, _HEAD_DIM), q, _FP16)
+    index = _cuda_index(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, pages, row_seq)
+    if sm_scale is None:
+        sm_scale = _HEAD_DIM ** -0.5
+    if not _current(index):
+        with torch.cuda.device(index):
+            return kv_sparse_attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, bits, pages, sm_scale,
+                                       row_seq, out, workspace)
+    if out is None:
+        out = q.new_empty((R, Hq, _HEAD_DIM))
+    lib = _lib.load()
+    need = lib.exl3_kv_sparse_workspace_bytes(R, Hq, Hkv, top)
+    at = size = 0
+    if need:
+        ws = _call_workspace(workspace, need, q)
+        at, size = ws.data_ptr(), ws.nbytes
+    _lib.check(lib.exl3_kv_sparse_attention(
+        q.data_ptr(), ld_q, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), P,
+        page_table.data_ptr(), B, max_pages, _ptr(row_seq), seq_lens.data_ptr(), R, Hq, Hkv, _HEAD_DIM, 16, bits,
+        pages.data_ptr(), top, sm_scale, out.data_ptr(), at, size, torch._C._cuda_getCurrentRawStream(index)),
+        "kv_sparse_attention")
+    return out
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    """Bytes of a `workspace` for sample_tokens and sampling_probs at this shape."""
+    return _lib.load().exl3_sample_workspace_bytes(rows, vocab)
+
+
+def _setting(value, name: str, dtype: torch.dtype, lead: tuple, tensors: list) -> tuple[int | None, float]:
+    """A setting of every row (a number), or one a row (a tensor): (pointer, number)."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.shape != lead or not value.is_contiguous():
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of shape {tuple(lead)}, got {value.dtype} "
+                         f"{tuple(value.shape)}")
+    tensors.append(value)
+    return value.data_ptr(), 0
+
+
+def _sample(what: str, logits: torch.Tensor, uniform: torch.Tensor | None, temperature, top_k, top_p, min_p, want_probs: bool,
+            probs: torch.Tensor | None, workspace: torch.Tensor | None):
+    shape = logits.shape
+    if logits.dtype not in _WEIGHT_TYPE or len(shape) < 1:
+        raise ValueError(f"logits must be fp16, bf16 or fp32 [..., V], got {logits.dtype} {tuple(shape)}")
+    lead, V = shape[:-1], shape[-1]
+    if len(shape) == 2:
+        rows, ld = shape[0], logits.stride(0)
+        if logits.stride(1) != 1 and V > 1:
+            raise ValueError(f"logits: a row must be contiguous, got strides {logits.stride()}")
+        ld = ld if rows > 1 else V
+    else:
+        if not logits.is_contiguous():
+            raise ValueError("logits of other than two dimensions must be contiguous")
+        rows, ld = logits.numel() // max(V, 1), V
+    tensors = [logits]
+    at_u = None
+    if uniform is not None:
+        if uniform.dtype != torch.float32 or uniform.shape != lead or not uniform.is_contiguous():
+            raise ValueError(f"uniform must be a contiguous fp32 tensor of shape {tuple(lead)}")
+        tensors.append(uniform)
+        at_u = uniform.data_ptr()
+    at_t, all_t = _setting(temperature, "temperature", torch.float32, lead, tensors)
+    at_k, all_k = _setting(top_k, "top_k", torch.int32, lead, tensors)
+    at_p, all_p = _setting(top_p, "top_p", torch.float32, lead, tensors)
+    at_m, all_m = _setting(min_p, "min_p", torch.float32, lead, tensors)
+    if not all_t >= 0 or not 0 <= all_p or not 0 <= all_m <= 1 or all_k < 0:
+        raise ValueError(f"temperature = {all_t}, top_k = {all_k}, top_p = {all_p}, min_p = {all_m}")
+    if probs is not None:
+        _check_out(probs, shape, logits, (torch.float32,))
+    index = _cuda_index(*tensors)
+    if not _current(index):
+        with torch.cuda.device(index):
+            return _sample(what, logits, uniform, temperature, top_k, top_p, min_p, want_probs, probs, workspace)
+    tokens = None if uniform is None else logits.new_empty(lead, dtype=torch.int32)
+    if probs is None and want_probs:
+        probs = logits.new_empty(shape, dtype=torch.float32)
+    lib = _lib.load()
+    need = lib.exl3_sample_workspace_bytes(rows, V)
+    ws = _call_workspace(workspace, need, logits)
+    _lib.check(lib.exl3_sample(
+        logits.data_ptr(), _WEIGHT_TYPE[logits.dtype], ld, rows, V, at_u, at_t, all_t, at_k, min(all_k, V), at_p, all_p, at_m,
+        all_m, _ptr(tokens), _ptr(probs), ws.data_ptr(), ws.nbytes, torch._C._cuda_getCurrentRawStream(index)), what)
+    return tokens, probs
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  return_probs: bool = False, probs: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """Tokens drawn from logits fp16|bf16|fp32 [..., V] by given random numbers: with w = exp((l - max l) / temperature) and a
+    row's elements in order of falling logits (ties by rising index), kept is the shortest of the first top_k (0: all), those
+    whose predecessors have less than top_p of the first top_k's sum of w, and those with w >= min_p; the first element always.
+    The token is the smallest one whose running sum of w over the kept passes uniform (fp32 [...], in [0, 1)) times their sum.
+    Each setting is a number or a tensor [...] (fp32; top_k int32) with a value a row; temperature 0 takes the largest logit, the
+    lowest of equals; NaN logits count as -inf; a row without a logit above -inf gives -1.
+    Returns int32 [...], and with return_probs (or `probs` to write to) the distribution drawn from, fp32 [..., V]: what
+    verify_drafts takes as draft_probs."""
+    tokens, probs = _sample("sample_tokens", logits, uniform, temperature, top_k, top_p, min_p,
+                            return_probs, probs, workspace)
+    return tokens if probs is None else (tokens, probs)
+
+
+def sampling_probs(logits: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """The distribution that sample_tokens draws from with these settings, fp32 [..., V]: what verify_drafts takes as
+    target_probs (a row without a logit above -inf: zeros)."""
+    return _sample("sampling_probs", logits, None, temperature, top_k, top_p, min_p, True, out, workspace)[1]
