@@ -14,13 +14,15 @@
 // 2^-50 of a chunk's largest weight or 2^-42 to 2^-52 of the row's: another summation decides differently only where a
 // threshold lies within some 10^-12 of the total of an edge.
 //
-// sample_chunk_kernel: (chunks of 8192 elements, rows) workgroups.  A chunk's largest logit m, its sum of exp((l - m) / t), and
-//   counts and sums in 256 bins an eighth of an octave of w wide.  An element's bin is a monotone function of its logit alone,
-//   so the chunks' bins match, and an element of a lower bin comes before every one of a higher.
-// sample_row_kernel: a workgroup per row adds the bins up and so knows the bins that each rule's last element is in.  Only
-//   their elements (some hundreds) are looked at one by one, in LDS: the cut comes from histograms of ever smaller ranges.
-//   Then the chunk, and in it the element, where the running sum passes the threshold.  Rows so flat that those bins hold more
-//   than the list takes go through the same search over the whole row instead.
+// sample_chunk_kernel: (chunks, rows) workgroups.  A chunk's largest logit m, its sum of exp((l - m) / t), and counts and sums
+//   in 256 bins an eighth of an octave of w wide.  An element's bin is a monotone function of its logit alone, so the chunks'
+//   bins match, and an element of a lower bin comes before every one of a higher.  Elements that the chunk alone shows to be cut
+//   (less than (1 - p) / vocab of its sum, behind its k-th, below m of its largest) stay out of the bins.
+// sample_border_kernel: a workgroup per row adds the bins up and so knows the bins that each rule's last element is in.
+// sample_list_kernel: (chunks, rows) workgroups list those bins' elements (some hundreds a row) and sum what lies before them.
+// sample_row_kernel: a workgroup per row finds the cut in the list, by histograms of ever smaller ranges; then the chunk, and in
+//   it the element, where the running sum passes the threshold.  Rows so flat that their border bins hold more than the list
+//   takes go through the same search over the whole row.
 // sample_probs_kernel: (chunks, rows) workgroups write the probabilities.
 #include <math.h>
 
@@ -37,28 +39,39 @@ typedef unsigned long long u64_t;
 typedef uint32_t sample_u32x4_t __attribute__((ext_vector_type(4), aligned(2)));  // rows start at any element
 
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kChunk = 8192;                     // elements of a chunk
-constexpr int kMaxChunks = kMaxVocab / kChunk;
-constexpr int kChunkThreads = 1024;
-constexpr int kEach = kChunk / kChunkThreads;    // 8 elements a thread
+constexpr int kEach = 8;                          // elements of a chunk's thread
+constexpr int kLargeChunk = 8192;                 // 1024 threads
+constexpr int kSmallChunk = 4096;                 // 512
+constexpr int kMaxChunks = kMaxVocab / kSmallChunk;
 constexpr int kBins = 256;
-constexpr int kRowThreads = 1024;
+constexpr int kBorderThreads = 256;               // a bin each, and a chunk each
+constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kCrossBins = 1024;
 constexpr int kList = 4096;
-constexpr double kBinUnit = 0x1p-50;             // a bin's sum is in 2^-50 of the chunk's largest weight
+constexpr int kSliceRows = 1024;                  // rows of a workspace
+constexpr double kBinUnit = 0x1p-50;              // a bin's sum is in 2^-50 of the chunk's largest weight
 constexpr double kBinBase = 0x1p52 * kBinUnit;
+static_assert(kMaxChunks <= kBorderThreads && kBins == kBorderThreads);
 
 struct SampleChunk {
   double sum;    // of exp((l - m) / t)
   float m, top;  // the largest logit, its place on the bins' scale
 };
-struct SampleCut {
-  uint32_t key;  // of the last kept element
-  int at;        // its index
-  double min_w;  // what a kept weight is not below
-  double inv;    // 1 / the sum of the kept weights; 0: no logit above -inf
-  float m;       // the row's largest logit
+
+// What a row's kernels know of it
+struct SampleBorder {
+  double sum;                 // of all weights
+  double before_k, before_p;  // of those in the bins before k_bin, p_first
+  double inv;                 // 1 / the sum of the kept weights (sample_row_kernel); 0: no logit above -inf
+  float m, top;               // the largest logit, its place
+  int first, last;            // the bins with elements that may be kept or not; before them all are, behind them none; first
+                              // kBins: no rule
+  int k_bin, k_left;          // the bin of the k-th element (-1: it does not matter), its rank there
+  int p_first, p_last;        // the bins that top-p's last element may be in
+  int listed;
+  int cut_at;                 // the last kept element's index
+  uint32_t cut;               // its key
 };
 
 struct SampleArgs {
@@ -72,10 +85,12 @@ struct SampleArgs {
   int* tokens;
   float* probs;
   int chunks;
-  SampleChunk* chunk;  // [rows][chunks]
-  u64_t* bin_mass;     // [rows][chunks][kBins]
-  int* bin_count;      // [rows][chunks][kBins]
-  SampleCut* cuts;     // [rows]
+  SampleBorder* border;  // [rows]
+  SampleChunk* chunk;    // [rows][chunks]
+  u64_t* chunk_mass;     // [rows][chunks]: what lies before the border bins, in the row's units
+  u64_t* bin_mass;       // [rows][chunks][kBins]
+  int* bin_count;        // [rows][chunks][kBins], where there is a top-k
+  u64_t* list;           // [rows][kList]: key << 32 | ~index
 };
 
 // A row's rules, and the scales of its weights (2^(scale (l - M))) and bins
@@ -83,6 +98,7 @@ struct SampleRules {
   double scale, p, m;
   float bin_scale;
   int k;
+  bool by_k, by_p, by_m;
 };
 
 __device__ __forceinline__ SampleRules sample_rules(const SampleArgs& a, int row) {
@@ -98,6 +114,7 @@ __device__ __forceinline__ SampleRules sample_rules(const SampleArgs& a, int row
   r.scale = 1.4426950408889634074 / t;
   // any positive number makes the bins a monotone function of the logit
   r.bin_scale = (float)fmin(fmax(8.0 * r.scale, 0x1p-126), 0x1p60);
+  r.by_k = r.k < a.vocab, r.by_p = r.p < 1.0, r.by_m = r.m > 0.0;
   return r;
 }
 
@@ -142,45 +159,55 @@ __device__ __forceinline__ u64_t sample_units(double w, double base) {
   return __builtin_bit_cast(u64_t, w + base) - __builtin_bit_cast(u64_t, base);
 }
 
-__device__ __forceinline__ uint32_t sample_key(float f) {  // orders like the logits, both zeros the same
-  const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float sample_logit(uint32_t key) {
-  return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-}
-
-template <int TYPE>
-__device__ __forceinline__ float sample_value(uint32_t bits) {
-  float f;
-  if constexpr (TYPE == EXL3_F32)
-    f = __builtin_bit_cast(float, bits);
-  else if constexpr (TYPE == EXL3_BF16)
-    f = __builtin_bit_cast(float, bits << 16);
-  else
-    f = (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
-  return f == f ? f : -INFINITY;
-}
-
 template <int TYPE>
 struct SampleRow {
   using Raw = std::conditional_t<TYPE == EXL3_F32, uint32_t, uint16_t>;
   static constexpr int VEC = 16 / sizeof(Raw);  // elements of a 16-byte load
+  static constexpr int LOW = TYPE == EXL3_F32 ? 0 : TYPE == EXL3_BF16 ? 16 : 13;  // bits that the type leaves 0 in a float
   const Raw* row;
   int vocab;
 
-  __device__ __forceinline__ float at(int i) const { return sample_value<TYPE>(row[i]); }
+  __device__ __forceinline__ static float value(uint32_t bits) {
+    float f;
+    if constexpr (TYPE == EXL3_F32)
+      f = __builtin_bit_cast(float, bits);
+    else if constexpr (TYPE == EXL3_BF16)
+      f = __builtin_bit_cast(float, bits << 16);
+    else
+      f = (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+    return f == f ? f : -INFINITY;
+  }
+  __device__ __forceinline__ float at(int i) const { return value(row[i]); }
   // elements i .. i + VEC - 1, -inf past the row; `whole` (uniform): none is
   __device__ __forceinline__ void get(int i, bool whole, float v[VEC]) const {
     if (whole || i + VEC <= vocab) {
       const sample_u32x4_t r = *reinterpret_cast<const sample_u32x4_t*>(row + i);
 #pragma unroll
       for (int e = 0; e < VEC; e++)
-        v[e] = sample_value<TYPE>(TYPE == EXL3_F32 ? r[e % 4] : (r[e / 2 % 4] >> (16 * (e & 1))) & 0xFFFFu);
+        v[e] = value(TYPE == EXL3_F32 ? r[e % 4] : (r[e / 2 % 4] >> (16 * (e & 1))) & 0xFFFFu);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; e++) v[e] = i + e < vocab ? at(i + e) : -INFINITY;
     }
+  }
+  // a thread's kEach elements of a chunk: VEC j 's at first + j * step
+  __device__ __forceinline__ void get_each(int first, int step, bool whole, float v[kEach]) const {
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < kEach / VEC; j++) get(first + j * step, true, v + j * VEC);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach / VEC; j++) get(first + j * step, false, v + j * VEC);
+    }
+  }
+  // whole numbers that order like the logits, both zeros the same
+  __device__ __forceinline__ static uint32_t key(float f) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.f);
+    return (u & 0x80000000u ? ~u : u | 0x80000000u) >> LOW;
+  }
+  __device__ __forceinline__ static float logit(uint32_t key) {
+    const uint32_t u = key << LOW;
+    return __builtin_bit_cast(float, u & 0x80000000u ? u & 0x7FFFFFFFu : ~u & (0xFFFFFFFFu << LOW));
   }
 };
 
@@ -190,502 +217,632 @@ __device__ __forceinline__ SampleRow<TYPE> sample_row(const SampleArgs& a, int r
   return Row{static_cast<const typename Row::Raw*>(a.logits) + (size_t)row * a.ld, a.vocab};
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const SampleArgs a) {
-  constexpr int VEC = SampleRow<TYPE>::VEC, WAVES = kChunkThreads / 64;
+// ---- sums and maxima over a wave ---------------------------------------------------------------------------------------
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64_t dpp_u64(u64_t v) {  // 0 where no lane feeds
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, ROWS == 0xF);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, ROWS == 0xF);
+  return (u64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ u64_t wave_scan_u64(u64_t v) {  // inclusive
+  v += dpp_u64<0x111, 0xF>(v);
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
+  v += dpp_u64<0x142, 0xA>(v);
+  v += dpp_u64<0x143, 0xC>(v);
+  return v;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  return v + __builtin_bit_cast(double, dpp_u64<CTRL, ROWS>(__builtin_bit_cast(u64_t, v)));
+}
+__device__ __forceinline__ double wave_scan_double(double v) {  // inclusive, in a fixed order
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);
+  return dpp_add<0x143, 0xC>(v);
+}
+__device__ __forceinline__ float wave_max_f32(float v) {  // of values that are no NaN
+  v = fmaxf(v, lane_xor<1>(v));
+  v = fmaxf(v, lane_xor<2>(v));
+  v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xF, 0xF, false)));
+  v = fmaxf(v, lane_xor<8>(v));
+  return max_over_groups(v);
+}
+
+// ---- the chunks --------------------------------------------------------------------------------------------------------
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_chunk_kernel(const SampleArgs a) {
+  constexpr int VEC = SampleRow<TYPE>::VEC, WAVES = THREADS / 64, CHUNK = THREADS * kEach;
   __shared__ u64_t mass[kBins];
-  __shared__ int count[kBins];
+  __shared__ int count[kBins], firsts[kBins];
   __shared__ float part[WAVES];
   __shared__ double sums[WAVES];
+  __shared__ int deepest;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
   const SampleRow<TYPE> x = sample_row<TYPE>(a, row);
-  const SampleRules rules = sample_rules(a, row);
-  const bool bins = rules.k < a.vocab || rules.p < 1.0 || rules.m > 0.0;
-  const int first = c * kChunk;
+  const int first = c * CHUNK;
+  const bool whole = first + CHUNK <= a.vocab;
   float l[kEach];
-  const bool whole = first + kChunk <= a.vocab;
-  if (whole) {
+  x.get_each(first + tid * VEC, THREADS * VEC, whole, l);
+  const SampleRules rules = sample_rules(a, row);
+  const bool bins = rules.by_k || rules.by_p || rules.by_m;
+  // behind a chunk's k-th largest element, for k up to 512: bins of its threads' largest elements tell (others are more)
+  const bool by_firsts = rules.by_k && rules.k <= 512;
+  if (bins && tid < kBins) mass[tid] = 0, count[tid] = 0, firsts[tid] = 0;
+  float mine = l[0];
 #pragma unroll
-    for (int j = 0; j < kEach / VEC; j++) x.get(first + (j * kChunkThreads + tid) * VEC, true, l + j * VEC);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kEach / VEC; j++) x.get(first + (j * kChunkThreads + tid) * VEC, false, l + j * VEC);
-  }
-  if (bins && tid < kBins) mass[tid] = 0, count[tid] = 0;
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kEach; i++) m = fmaxf(m, l[i]);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+  for (int i = 1; i < kEach; i++) mine = fmaxf(mine, l[i]);
+  float m = wave_max_f32(mine);
   if (lane == 0) part[wave] = m;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; w++) m = fmaxf(m, part[w]);
   const size_t at = (size_t)row * a.chunks + c;
   const float top = sample_place(m, rules.bin_scale);
-  double sum = 0.0;
-  if (m > -INFINITY) {
+  const bool any = m > -INFINITY;
+  double w[kEach], sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+    const bool in = any && (whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab);
+    w[i] = in ? sample_weight(l[i], m, rules.scale) : 0.0;
+    sum += w[i];
+  }
+  sum = wave_scan_double(sum);
+  if (lane == 63) sums[wave] = sum;
+  if (any && by_firsts) {
+    const int bin = sample_bin(mine, rules.bin_scale, top);
+    if (bin < kBins - 1) atomicAdd(&firsts[bin], 1);
+  }
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; i++) sum += sums[i];
+  if (tid == 0) a.chunk[at] = SampleChunk{sum, m, top};
+  if (!bins) return;
+  // Elements of bins past `deep` take no part in any rule.  By weight that holds with bins to spare while places are exact to a
+  // small part of one; exponents stand for logarithms (bins of 8 times floor(log2), up to 7 more than needed).
+  int deep = kBins - 2;
+  if (any && fabsf(top) < 0x1p16f) {
+    auto bins_to = [](double w) { return 11 - 8 * __builtin_amdgcn_frexp_exp(w); };
+    if (rules.by_m && !(rules.by_k && rules.by_p)) deep = min(deep, bins_to(rules.m));
+    if (rules.by_p && !rules.by_k) deep = min(deep, bins_to((1.0 - rules.p) * sum / (double)a.vocab));
+  }
+  if (any && by_firsts) {
+    if (wave == 0) {
+      int n[4], all = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) n[i] = firsts[4 * lane + i], all += n[i];
+      int run = wave_scan(all) - all, d = kBins;
+#pragma unroll
+      for (int i = 3; i >= 0; i--) {
+        int upto = run;
+#pragma unroll
+        for (int j = 0; j <= i; j++) upto += n[j];
+        if (upto >= rules.k) d = 4 * lane + i;
+      }
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(d < kBins);
+      const int found = hit ? __builtin_amdgcn_readlane(d, __builtin_ctzll(hit)) : kBins;
+      if (lane == 0) deepest = found;
+    }
+    __syncthreads();
+    deep = min(deep, deepest);
+  }
+  if (any) {
 #pragma unroll
     for (int i = 0; i < kEach; i++) {
-      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // four chains at a time: all sixteen do not fit the registers
-      const double w = sample_weight(l[i], m, rules.scale);
-      const bool in = whole || first + (i / VEC * kChunkThreads + tid) * VEC + i % VEC < a.vocab;
-      sum += in ? w : 0.0;
-      if (bins && in) {
-        const int bin = sample_bin(l[i], rules.bin_scale, top);
-        atomicAdd(&count[bin], 1);
-        atomicAdd(&mass[bin], sample_units(w, kBinBase));
+      const int bin = sample_bin(l[i], rules.bin_scale, top);
+      const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
+      if (in && bin <= deep) {
+        atomicAdd(&mass[bin], sample_units(w[i], kBinBase));
+        if (rules.by_k) atomicAdd(&count[bin], 1);
       }
     }
   }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  if (lane == 0) sums[wave] = sum;
   __syncthreads();
-  if (tid == 0) {
-    sum = 0.0;
-    for (int w = 0; w < WAVES; w++) sum += sums[w];
-    a.chunk[at] = SampleChunk{sum, m, top};
-  }
-  if (bins && tid < kBins) {
+  if (tid < kBins) {
     a.bin_mass[at * kBins + tid] = mass[tid];
-    a.bin_count[at * kBins + tid] = count[tid];
+    if (rules.by_k) a.bin_count[at * kBins + tid] = count[tid];
   }
 }
 
+// ---- the border bins ---------------------------------------------------------------------------------------------------
+
+__global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(const SampleArgs a) {
+  constexpr int WAVES = kBorderThreads / 64;
+  __shared__ double factor[kMaxChunks], sums[WAVES], masses[WAVES], at_k[2], at_p;
+  __shared__ float part[2][WAVES];
+  __shared__ int shift[kMaxChunks], counts[WAVES], k_at[2], below[2][WAVES];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, C = a.chunks;
+  const SampleRules rules = sample_rules(a, row);
+  SampleChunk chunk{0.0, -INFINITY, -INFINITY};
+  if (tid < C) chunk = a.chunk[(size_t)row * C + tid];
+  const float m = wave_max_f32(chunk.m), t = wave_max_f32(chunk.top);
+  if (lane == 0) part[0][wave] = m, part[1][wave] = t;
+  if (tid == 0) k_at[0] = kBins - 1;
+  __syncthreads();
+  float M = part[0][0], top = part[1][0];
+#pragma unroll
+  for (int w = 1; w < WAVES; w++) M = fmaxf(M, part[0][w]), top = fmaxf(top, part[1][w]);
+  SampleBorder b{};
+  b.m = M, b.top = top, b.first = kBins, b.last = kBins - 1, b.k_bin = -1, b.p_last = -1, b.cut_at = a.vocab - 1;
+  if (!(M > -INFINITY)) {  // nothing to draw from
+    if (tid == 0) a.border[row] = b;
+    return;
+  }
+  const double f = chunk.m > -INFINITY ? sample_weight(chunk.m, M, rules.scale) : 0.0;
+  if (tid < C) factor[tid] = f * kBinUnit, shift[tid] = (int)fminf(top - chunk.top, (float)kBins);
+  const double s = wave_scan_double(f * chunk.sum);
+  if (lane == 63) sums[wave] = s;
+  __syncthreads();
+  b.sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) b.sum += sums[w];
+  if (rules.by_k || rules.by_p || rules.by_m) {
+    // the bins of all chunks; the last one is what is not in the others
+    double mass = 0.0;
+    int count = 0;
+    if (tid < kBins - 1) {
+#pragma unroll 4
+      for (int c = 0; c < C; c++) {
+        const int bin = tid - shift[c];
+        if (bin < 0) continue;
+        const size_t at = ((size_t)row * C + c) * kBins + bin;
+        mass += factor[c] * (double)a.bin_mass[at];
+        if (rules.by_k) count += a.bin_count[at];
+      }
+    }
+    double mass_to = wave_scan_double(mass);
+    int count_to = wave_scan(count);
+    if (lane == 63) masses[wave] = mass_to, counts[wave] = count_to;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) mass_to += masses[w], count_to += counts[w];
+    const double mass_from = mass_to - mass;  // (a rounding apart from the bin before's mass_to)
+    const int count_from = count_to - count;
+    double bar_lo = b.sum, bar_hi = b.sum;
+    if (rules.by_k) {
+      if (tid < kBins - 1 && count_from < rules.k && count_to >= rules.k) k_at[0] = tid;
+      __syncthreads();
+      b.k_bin = k_at[0];
+      if (tid == b.k_bin) k_at[1] = rules.k - count_from, at_k[0] = mass_from, at_k[1] = tid < kBins - 1 ? mass_to : b.sum;
+      __syncthreads();
+      b.k_left = k_at[1], b.before_k = bar_lo = at_k[0], bar_hi = fmax(at_k[1], bar_lo);
+    }
+    if (rules.by_p) {
+      // a bin's sum is off by half a unit an element, the threshold by the part of the first k in their last bin
+      const double slack = (double)a.vocab * kBinUnit + 1e-13 * b.sum;
+      const double lo = rules.p * bar_lo - slack, hi = rules.p * bar_hi + slack;
+      const int short_of = __builtin_popcountll(__builtin_amdgcn_ballot_w64(tid < kBins - 1 && mass_to < lo));
+      const int from = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mass_from < hi));
+      if (lane == 0) below[0][wave] = short_of, below[1][wave] = from;
+      __syncthreads();
+      int p_last = -1;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) b.p_first += below[0][w], p_last += below[1][w];
+      b.p_last = max(b.p_first, p_last);
+      if (tid == b.p_first) at_p = mass_from;
+      __syncthreads();
+      b.before_p = at_p;
+      b.first = min(b.first, b.p_first), b.last = min(b.last, b.p_last);
+    }
+    if (rules.by_m) {
+      // w >= m from the logit M + log2(m) / scale on; places are off by a few 2^-24 of themselves
+      const double y0 = (double)M * rules.bin_scale, y = y0 + log2(rules.m) * (rules.bin_scale / rules.scale);
+      const double e = 0.01 + (fabs(y) + fabs(y0)) * 1e-6;
+      const bool far = !(e < 64.0);  // (infinite M too)
+      const double lo = (double)top - floor(y + e), hi = (double)top - floor(y - e);
+      b.first = min(b.first, far ? 0 : (int)fmin(fmax(lo, 0.0), kBins - 1.0));
+      b.last = min(b.last, far ? kBins - 1 : (int)fmin(fmax(hi, 0.0), kBins - 1.0));
+    }
+    if (rules.by_k) {
+      if (!rules.by_p && b.k_bin > b.last)
+        b.k_bin = -1;  // min-p stops before
+      else
+        b.first = min(b.first, b.k_bin), b.last = min(b.last, b.k_bin);
+    }
+    b.first = min(b.first, b.last);
+  }
+  if (tid == 0) a.border[row] = b;
+}
+
+// ---- their elements ----------------------------------------------------------------------------------------------------
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_list_kernel(const SampleArgs a) {
+  using Row = SampleRow<TYPE>;
+  constexpr int VEC = Row::VEC, WAVES = THREADS / 64, CHUNK = THREADS * kEach;
+  __shared__ int part[WAVES], base;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
+  SampleBorder* border = a.border + row;
+  const int g_first = border->first, g_last = border->last, k_bin = border->k_bin;
+  const float M = border->m, top = border->top;
+  if (!(M > -INFINITY)) return;
+  const SampleRules rules = sample_rules(a, row);
+  const size_t at = (size_t)row * a.chunks + c;
+  const SampleChunk chunk = a.chunk[at];
+  const float ahead = top - chunk.top;  // bins
+  if (wave == 0) {
+    // its weights in the bins before the border
+    const double one = (double)(1ull << a.shift), f = chunk.m > -INFINITY ? sample_weight(chunk.m, M, rules.scale) : 0.0;
+    double s = 0.0;
+    if (g_first == kBins) {
+      s = lane == 63 ? chunk.sum : 0.0;
+    } else {
+      const int end = g_first - (int)fminf(ahead, (float)kBins);
+#pragma unroll
+      for (int i = 0; i < kBins / 64; i++)
+        if (64 * i + lane < end) s += (double)a.bin_mass[at * kBins + 64 * i + lane];
+      s = wave_scan_double(s) * kBinUnit;
+    }
+    if (lane == 63) a.chunk_mass[at] = (u64_t)__builtin_rint(s * f * one);
+  }
+  if (g_first == kBins || ahead > (float)max(g_last, k_bin)) return;  // none listed
+  const int first = c * CHUNK;
+  const bool whole = first + CHUNK <= a.vocab;
+  float l[kEach];
+  sample_row<TYPE>(a, row).get_each(first + tid * VEC, THREADS * VEC, whole, l);
+  unsigned take = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    const int b = sample_bin(l[i], rules.bin_scale, top);
+    const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
+    take |= (unsigned)(in && ((b >= g_first && b <= g_last) || b == k_bin)) << i;
+  }
+  const int mine = __builtin_popcount(take), upto = wave_scan(mine);
+  if (lane == 63) part[wave] = upto;
+  __syncthreads();
+  int before = upto - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) before += w < wave ? part[w] : 0, all += part[w];
+  if (all == 0) return;
+  if (tid == 0) base = atomicAdd(&border->listed, all);
+  __syncthreads();
+  int to = base + before;
+  u64_t* list = a.list + (size_t)row * kList;
+#pragma unroll
+  for (int i = 0; i < kEach; i++)
+    if (take >> i & 1) {
+      if (to < kList) list[to] = (u64_t)Row::key(l[i]) << 32 | (uint32_t)~(first + (i / VEC * THREADS + tid) * VEC + i % VEC);
+      to++;
+    }
+}
+
+// ---- the cut and the token ---------------------------------------------------------------------------------------------
+
+struct SampleFound {
+  u64_t before, here;
+  int bin;
+};
 struct SampleShared {
-  u64_t list[kList];  // key << 32 | ~index
-  u64_t hist[kCrossBins], part[kRowWaves], chunk_mass[kMaxChunks];
-  double cum_mass[kBins + 1], factor[kMaxChunks], red[4][kBins], sum;
-  int cum_count[kBins + 1], red_count[4][kBins];
-  float shift[kMaxChunks];
-  uint32_t key[kRowWaves];
-  u64_t before;
-  int bin, listed, k_bin, p_first, p_last, token, last;
+  u64_t list[kList], hist[kCrossBins], part[2][kRowWaves], chunk_mass[kMaxChunks];
+  SampleFound found[2];
+  uint32_t ends[2][kRowWaves];
+  int token, last;
 };
 
-__device__ __forceinline__ u64_t shfl_up_u64(u64_t v, int d) {
-  const uint32_t lo = __shfl_up((int)(uint32_t)v, d), hi = __shfl_up((int)(uint32_t)(v >> 32), d);
-  return (u64_t)hi << 32 | lo;
-}
+// A workgroup's steps in LDS; `turn` alternates between two places, so that one barrier a step is enough
+struct SampleGroup {
+  SampleShared& sh;
+  int turn = 0;
 
-// sum before this thread, and of all
-__device__ __forceinline__ u64_t row_scan(u64_t v, u64_t& total, SampleShared& sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64_t s = v;
+  // sum before this thread, and of all
+  __device__ __forceinline__ u64_t scan(u64_t v, u64_t& total) {
+    const int wave = threadIdx.x >> 6;
+    const u64_t s = wave_scan_u64(v);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 63) sh.part[turn][wave] = s;
+    __syncthreads();
+    u64_t before = 0;
+    total = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const u64_t o = shfl_up_u64(s, d);
-    s += lane >= d ? o : 0;
+    for (int w = 0; w < kRowWaves; w++) {
+      const u64_t one = sh.part[turn][w];
+      before += w < wave ? one : 0;
+      total += one;
+    }
+    return before + s - v;
   }
-  __syncthreads();
-  if (lane == 63) sh.part[wave] = s;
-  __syncthreads();
-  u64_t before = 0;
-  total = 0;
-  for (int w = 0; w < kRowWaves; w++) {
-    before += w < wave ? sh.part[w] : 0;
-    total += sh.part[w];
-  }
-  return before + s - v;
-}
 
-// Of the elements i < n with a value get(i, value, mass) in [lo, hi]: the value at which their masses, summed from hi down, reach
-// `target` (at least 1, at most their sum); target becomes what is left of it for that value.  Every pass leaves a range of
-// 1/1024 of the one before.
-template <class Get>
-__device__ uint32_t row_cross(int n, uint32_t lo, uint32_t hi, u64_t& target, SampleShared& sh, Get get) {
-  while (lo < hi) {
-    const uint32_t span = hi - lo;
-    const int shift = max(0, 32 - __builtin_clz(span) - 10);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kCrossBins; i += kRowThreads) sh.hist[i] = 0;
-    if (threadIdx.x == 0) sh.bin = 0, sh.before = 0;
-    __syncthreads();
+  // Of the elements i < n with a value get(i, value, mass): the value at which their masses, summed from the largest value down,
+  // reach `target` (at least 1, at most their sum); target becomes what is left of it for that value, `here` that value's sum.
+  // Every pass leaves a range of 1/1024 of the one before.
+  template <class Get>
+  __device__ uint32_t cross(int n, u64_t& target, u64_t& here, Get get) {
+    uint32_t lo = ~0u, hi = 0;
     for (int i = threadIdx.x; i < n; i += kRowThreads) {
       uint32_t v;
       u64_t m;
-      if (get(i, lo, hi, v, m)) atomicAdd(&sh.hist[(hi - v) >> shift], m);
+      if (get(i, v, m)) lo = min(lo, v), hi = max(hi, v);
     }
+    hi = wave_max_u32(hi), lo = wave_max_u32(~lo);
     __syncthreads();
-    u64_t total;
-    const u64_t here = sh.hist[threadIdx.x], before = row_scan(here, total, sh);
-    if (before < target && before + here >= target) sh.bin = threadIdx.x, sh.before = before;
+    if ((threadIdx.x & 63) == 0) sh.ends[0][threadIdx.x >> 6] = lo, sh.ends[1][threadIdx.x >> 6] = hi;
     __syncthreads();
-    target -= sh.before;
-    hi -= min((uint32_t)sh.bin, span >> shift) << shift;
-    const uint32_t size = (1u << shift) - 1;
-    lo = hi - lo > size ? hi - size : lo;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; w++) lo = max(lo, sh.ends[0][w]), hi = max(hi, sh.ends[1][w]);
+    lo = ~lo;
+    here = 0;
+    bool more = lo <= hi;
+    while (more) {
+      const uint32_t span = hi - lo;
+      const int shift = span ? max(0, 32 - __builtin_clz(span) - 10) : 0;
+      for (int i = threadIdx.x; i < kCrossBins; i += kRowThreads) sh.hist[i] = 0;
+      turn ^= 1;
+      SampleFound& found = sh.found[turn];
+      if (threadIdx.x == 0) found = SampleFound{0, 0, 0};
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kRowThreads) {
+        uint32_t v;
+        u64_t m;
+        if (get(i, v, m) && v >= lo && v <= hi) atomicAdd(&sh.hist[(hi - v) >> shift], m);
+      }
+      __syncthreads();
+      u64_t bin[kCrossBins / kRowThreads], all = 0, total;
+#pragma unroll
+      for (int i = 0; i < kCrossBins / kRowThreads; i++) {
+        bin[i] = sh.hist[threadIdx.x * (kCrossBins / kRowThreads) + i];
+        all += bin[i];
+      }
+      turn ^= 1;  // (scan turns again: it does not touch what `found` refers to)
+      u64_t before = scan(all, total);
+#pragma unroll
+      for (int i = 0; i < kCrossBins / kRowThreads; i++) {
+        if (before < target && before + bin[i] >= target)
+          found = SampleFound{before, bin[i], (int)threadIdx.x * (kCrossBins / kRowThreads) + i};
+        before += bin[i];
+      }
+      __syncthreads();
+      target -= found.before;
+      here = found.here;
+      hi -= min((uint32_t)found.bin, span >> shift) << shift;
+      const uint32_t size = (1u << shift) - 1;
+      lo = hi - lo > size ? hi - size : lo;
+      more = lo < hi;
+    }
+    return hi;
   }
-  __syncthreads();
-  return hi;
-}
 
-template <int TYPE>
+  template <class Get>
+  __device__ __forceinline__ u64_t sum(int n, Get get) {
+    u64_t s = 0, total;
+    for (int i = threadIdx.x; i < n; i += kRowThreads) s += get(i);
+    scan(s, total);
+    return total;
+  }
+};
+
+template <int TYPE, int CHUNK>
 __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArgs a) {
-  constexpr int VEC = SampleRow<TYPE>::VEC;
+  using Row = SampleRow<TYPE>;
+  constexpr int VEC = Row::VEC, EACH = CHUNK / kRowThreads;
   __shared__ SampleShared sh;
+  SampleGroup group{sh};
   const int row = blockIdx.x, tid = threadIdx.x, V = a.vocab, C = a.chunks;
-  const SampleRow<TYPE> x = sample_row<TYPE>(a, row);
-  const SampleRules rules = sample_rules(a, row);
-  const bool by_k = rules.k < V, by_p = rules.p < 1.0, by_m = rules.m > 0.0;
-  const SampleChunk* chunk = a.chunk + (size_t)row * C;
-
-  float M = -INFINITY, top = -INFINITY;
-  for (int c = tid; c < C; c += kRowThreads) M = fmaxf(M, chunk[c].m), top = fmaxf(top, chunk[c].top);
-  // (C <= 128: the first two waves hold them; a key orders like its float)
-  auto most = [&](float f) {
-    const uint32_t v = wave_max_u32(sample_key(f));
-    __syncthreads();
-    if ((tid & 63) == 0) sh.key[tid >> 6] = v;
-    __syncthreads();
-    return sample_logit(max(sh.key[0], sh.key[1]));
-  };
-  M = most(M);
-  if (!(M > -INFINITY)) {  // nothing to draw from
-    if (tid == 0) {
-      if (a.tokens) a.tokens[row] = -1;
-      if (a.cuts) a.cuts[row] = SampleCut{0, 0, 0.0, 0.0, M};
-    }
+  SampleBorder* border = a.border + row;
+  const SampleBorder b = *border;
+  if (!(b.m > -INFINITY)) {
+    if (tid == 0 && a.tokens) a.tokens[row] = -1;
     return;
   }
-  top = most(top);
-  const double one = (double)(1ull << a.shift);
-  auto weight = [&](float l) { return sample_weight(l, M, rules.scale); };
-  const double base = (double)(1ull << (52 - a.shift));
-  auto mass = [&](float l) { return sample_units(weight(l), base); };
-  auto bin_of = [&](float l) { return sample_bin(l, rules.bin_scale, top); };
+  const Row x = sample_row<TYPE>(a, row);
+  const SampleRules rules = sample_rules(a, row);
+  const bool fast = b.listed <= kList;
+  const int n = fast ? b.listed : V;
+  if (fast)
+    for (int i = tid; i < n; i += kRowThreads) sh.list[i] = a.list[(size_t)row * kList + i];
+  const bool ruled = b.first < kBins;
   for (int c = tid; c < C; c += kRowThreads) {
-    sh.factor[c] = chunk[c].m > -INFINITY ? weight(chunk[c].m) : 0.0;
-    sh.shift[c] = fminf(top - chunk[c].top, (float)kBins);
-  }
-  if (tid == 0) sh.listed = 0;
-  __syncthreads();
-  if (tid < 64) {  // in a fixed order
-    double s = 0.0;
-    for (int c = tid; c < C; c += 64) s += sh.factor[c] * chunk[c].sum;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
-    if (tid == 0) sh.sum = s;
+    const size_t at = (size_t)row * C + c;
+    if (ruled) {
+      sh.chunk_mass[c] = a.chunk_mass[at];
+    } else {
+      const SampleChunk chunk = a.chunk[at];
+      const double f = chunk.m > -INFINITY ? sample_weight(chunk.m, b.m, rules.scale) : 0.0;
+      sh.chunk_mass[c] = (u64_t)__builtin_rint(f * chunk.sum * (double)(1ull << a.shift));
+    }
   }
   __syncthreads();
-  const double sum_all = sh.sum;
-
-  // the cut: the last kept element's key and index, and a bound on kept weights
-  uint32_t cut = 0;
-  int cut_at = V - 1;
-  auto before_cut = [&](uint32_t key, int i) { return key > cut || (key == cut && i <= cut_at); };
-  auto kept = [&](float l, int i) {
-    return before_cut(sample_key(l), i) && (!by_m || weight(l) >= rules.m);
-  };
-  // the first `count` elements of key `at` by index, among the elements get(i, key, index) for i < n
-  auto cut_ties = [&](int n, uint32_t at, u64_t count, auto get) {
-    const uint32_t last = ~0u - (uint32_t)(V - 1);
-    const uint32_t v = row_cross(n, last, ~0u, count, sh, [&](int i, uint32_t lo, uint32_t hi, uint32_t& v, u64_t& m) {
-      uint32_t key;
-      int index;
-      get(i, key, index);
-      v = ~(uint32_t)index, m = 1;
-      return key == at && v >= lo && v <= hi;
-    });
-    cut = at, cut_at = (int)~v;
-  };
-  // of the sum of get's masses
-  auto sum_of = [&](int n, auto get) {
-    u64_t sum = 0, total;
-    for (int i = tid; i < n; i += kRowThreads) sum += get(i);
-    row_scan(sum, total, sh);
-    return total;
-  };
-
-  // ---- from the bins: where each rule's last element is
-  int g_first = kBins, g_last = kBins - 1, k_bin = -1, p_first = 0, p_last = kBins - 1;
-  int listed = 0;
-  if (by_k || by_p || by_m) {
-    const int bin = tid & (kBins - 1), quarter = tid / kBins;
-    double s = 0.0;
-    int n = 0;
-    if (bin < kBins - 1)
-      for (int c = quarter; c < C; c += 4) {
-        const int local = bin - (int)sh.shift[c];
-        if (local < 0) continue;
-        const size_t at = ((size_t)row * C + c) * kBins + local;
-        s += sh.factor[c] * (double)a.bin_mass[at];
-        n += a.bin_count[at];
-      }
-    sh.red[quarter][bin] = s, sh.red_count[quarter][bin] = n;
-    __syncthreads();
-    u64_t all;
-    n = 0, s = 0.0;
-    if (tid < kBins) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) s += sh.red[i][tid], n += sh.red_count[i][tid];
-      s *= kBinUnit;
-    }
-    const int before = (int)row_scan((u64_t)n, all, sh);
-    // sums of the bins before, in a fixed order: inside each wave, then the waves'
-    double run = s;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double o = __shfl_up(run, d);
-      run += (tid & 63) >= d ? o : 0.0;
-    }
-    if ((tid & 63) == 63 && tid < kBins) sh.red[0][tid >> 6] = run;
-    __syncthreads();
-    if (tid < kBins) {
-      double base = 0.0;
-      for (int w = 0; w < tid >> 6; w++) base += sh.red[0][w];
-      sh.cum_mass[tid + 1] = base + run;
-      sh.cum_count[tid + 1] = before + n;
-    }
-    if (tid == 0) sh.cum_mass[0] = 0.0, sh.cum_count[0] = 0, sh.k_bin = kBins - 1, sh.p_first = kBins - 1, sh.p_last = 0;
-    __syncthreads();
-    if (tid == 0) sh.cum_mass[kBins] = fmax(sum_all, sh.cum_mass[kBins]), sh.cum_count[kBins] = V;  // the last bin: the rest
-    __syncthreads();
-    if (by_k && tid < kBins && sh.cum_count[tid] < rules.k && sh.cum_count[tid + 1] >= rules.k) sh.k_bin = tid;
-    __syncthreads();
-    if (by_k) k_bin = sh.k_bin;
-    if (by_p) {
-      // a bin's sum is off by half a unit an element, the threshold by the part of the first k in their last bin
-      const double slack = (double)V * kBinUnit + 1e-13 * sum_all;
-      const double lo = rules.p * (by_k ? sh.cum_mass[k_bin] : sum_all) - slack;
-      const double hi = rules.p * (by_k ? sh.cum_mass[k_bin + 1] : sum_all) + slack;
-      if (tid < kBins) {
-        if (sh.cum_mass[tid + 1] >= lo) atomicMin(&sh.p_first, tid);
-        if (sh.cum_mass[tid] < hi) atomicMax(&sh.p_last, tid);
-      }
-      __syncthreads();
-      p_first = sh.p_first, p_last = max(sh.p_first, sh.p_last);
-      g_first = min(g_first, p_first), g_last = min(g_last, p_last);
-    }
-    if (by_m) {
-      // w >= m from the logit M + log2(m) / scale on; places are off by a few 2^-24 of themselves
-      const double y = (double)M * rules.bin_scale + log2(rules.m) * (rules.bin_scale / rules.scale);
-      const double e = 0.01 + fabs(y) * 1e-6 + fabs((double)M * rules.bin_scale) * 1e-6;
-      const double lo = (double)top - floor(y + e), hi = (double)top - floor(y - e);
-      const bool far = !(e < 64.0);  // (infinite M too)
-      g_first = min(g_first, far ? 0 : (int)fmin(fmax(lo, 0.0), kBins - 1.0));
-      g_last = min(g_last, far ? kBins - 1 : (int)fmin(fmax(hi, 0.0), kBins - 1.0));
-    }
-    if (by_k) {
-      if (!by_p && k_bin > g_last) k_bin = -1;  // min-p stops before
-      else g_first = min(g_first, k_bin), g_last = min(g_last, k_bin);
-    }
-    listed = sh.cum_count[g_last + 1] - sh.cum_count[g_first];
-    const bool apart = k_bin > g_last;  // its elements are listed too
-    if (apart) listed += sh.cum_count[k_bin + 1] - sh.cum_count[k_bin];
-    if (listed <= kList) {
-      for (int i = tid * VEC; i < V; i += kRowThreads * VEC) {
-        float l[VEC];
-        x.get(i, false, l);
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          const int b = bin_of(l[e]);
-          if (((b >= g_first && b <= g_last) || b == k_bin) && i + e < V)
-            sh.list[atomicAdd(&sh.listed, 1)] = (u64_t)sample_key(l[e]) << 32 | (uint32_t)~(i + e);
-        }
-      }
-      __syncthreads();
-    }
-  }
-  const bool fast = listed <= kList;
-
-  // ---- the cut
-  const uint32_t largest = sample_key(M);
+  const double one = (double)(1ull << a.shift), base = (double)(1ull << (52 - a.shift));
+  auto weight = [&](float l) { return sample_weight(l, b.m, rules.scale); };
+  auto mass = [&](float l) { return sample_units(weight(l), base); };
+  auto bin_of = [&](uint32_t key) { return sample_bin(Row::logit(key), rules.bin_scale, b.top); };
   auto element = [&](int i, uint32_t& key, int& index) {
     if (fast) {
       const u64_t v = sh.list[i];
       key = (uint32_t)(v >> 32), index = (int)~(uint32_t)v;
     } else {
-      key = sample_key(x.at(i)), index = i;
+      key = Row::key(x.at(i)), index = i;
     }
   };
-  const int n = fast ? listed : V;
-  if (by_k && (!fast || k_bin >= 0)) {
-    u64_t target = fast ? rules.k - sh.cum_count[k_bin] : rules.k;
-    const uint32_t at = row_cross(n, 0, largest, target, sh, [&](int i, uint32_t lo, uint32_t hi, uint32_t& v, u64_t& m) {
-      int index;
-      element(i, v, index);
-      m = 1;
-      return v >= lo && v <= hi && (!fast || bin_of(sample_logit(v)) == k_bin);
-    });
-    cut_ties(n, at, target, element);
-  }
-  if (by_p) {
-    u64_t target = 0, most = 0;
-    if (fast) {
-      double total = sum_all;
-      if (by_k)
-        total = sh.cum_mass[k_bin] + (double)sum_of(n, [&](int i) -> u64_t {
-                  uint32_t key;
-                  int index;
-                  element(i, key, index);
-                  const float l = sample_logit(key);
-                  return bin_of(l) == k_bin && before_cut(key, index) ? mass(l) : 0;
-                }) / one;
-      most = sum_of(n, [&](int i) -> u64_t {
-        uint32_t key;
-        int index;
-        element(i, key, index);
-        const float l = sample_logit(key);
-        const int b = bin_of(l);
-        return b >= p_first && b <= p_last && before_cut(key, index) ? mass(l) : 0;
-      });
-      const double bar = __builtin_ceil((rules.p * total - sh.cum_mass[p_first]) * one);
-      target = bar >= 1.0 ? min((u64_t)bar, most) : 1;
-    } else {
-      most = sum_of(V, [&](int i) -> u64_t {
-        const float l = x.at(i);
-        return before_cut(sample_key(l), i) ? mass(l) : 0;
-      });
-      const double bar = __builtin_ceil(rules.p * (double)most);
-      target = bar >= 1.0 ? min((u64_t)bar, most) : 1;
-    }
-    if (most > 0) {
-      const uint32_t at = row_cross(n, cut, largest, target, sh, [&](int i, uint32_t lo, uint32_t hi, uint32_t& v, u64_t& m) {
-        int index;
-        element(i, v, index);
-        if (v < lo || v > hi || !before_cut(v, index)) return false;
-        const float l = sample_logit(v);
-        if (fast) {
-          const int b = bin_of(l);
-          if (b < p_first || b > p_last) return false;
-        }
-        m = mass(l);
-        return true;
-      });
-      const u64_t each = mass(sample_logit(at));
-      if (each > 0) cut_ties(n, at, (target + each - 1) / each, element);
-    }
-  }
 
-  // ---- the token
-  u64_t total = 0;
-  const float u = a.uniform ? a.uniform[row] : 0.f;
-  auto threshold = [&]() {  // the smallest whole number above u times the sum
-    const double bar = (u > 0.f ? (double)u : 0.0) * (double)total;
-    return bar < (double)total ? min((u64_t)bar + 1, total) : total;
-  };
-  if (!fast) {
-    total = sum_of(V, [&](int i) -> u64_t {
-      const float l = x.at(i);
-      return kept(l, i) ? mass(l) : 0;
-    });
-    if (a.tokens) {
-      u64_t target = threshold();
-      const uint32_t last = ~0u - (uint32_t)(V - 1);
-      const uint32_t v = row_cross(V, last, ~0u, target, sh, [&](int i, uint32_t lo, uint32_t hi, uint32_t& v, u64_t& m) {
-        v = ~(uint32_t)i;
-        if (v < lo || v > hi) return false;
-        const float l = x.at(i);
-        if (!kept(l, i)) return false;
-        m = mass(l);
-        return true;
-      });
-      if (tid == 0) a.tokens[row] = (int)~v;
-    }
-  } else {
-    // each chunk's kept sum: its bins before g_first, and its listed elements
-    for (int c = tid >> 6; c < C; c += kRowWaves) {
-      double s = 0.0;
-      if (g_first == kBins) {
-        s = chunk[c].sum;
-      } else {
-        const int end = g_first - (int)sh.shift[c];
-        for (int b = tid & 63; b < end; b += 64) s += (double)a.bin_mass[((size_t)row * C + c) * kBins + b];
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
-        s *= kBinUnit;
-      }
-      if ((tid & 63) == 0) sh.chunk_mass[c] = (u64_t)__builtin_rint(s * sh.factor[c] * one);
-    }
-    __syncthreads();
-    for (int i = tid; i < n; i += kRowThreads) {
+  // the last kept element
+  uint32_t cut = 0;
+  int cut_at = V - 1;
+  auto before_cut = [&](uint32_t key, int i) { return key > cut || (key == cut && i <= cut_at); };
+  auto kept = [&](float l, int i) { return before_cut(Row::key(l), i) && (!rules.by_m || weight(l) >= rules.m); };
+  // the first `count` of the `ties` elements of key `at`, by index
+  auto cut_ties = [&](uint32_t at, u64_t count, u64_t ties) {
+    cut = at, cut_at = V - 1;
+    if (count >= ties) return;
+    u64_t here;
+    cut_at = (int)~group.cross(n, count, here, [&](int i, uint32_t& v, u64_t& m) {
       uint32_t key;
       int index;
       element(i, key, index);
-      const float l = sample_logit(key);
-      if (bin_of(l) <= g_last && kept(l, index)) atomicAdd(&sh.chunk_mass[index / kChunk], mass(l));
-    }
-    __syncthreads();
-    const u64_t here = tid < C ? sh.chunk_mass[tid] : 0;
-    const u64_t before = row_scan(here, total, sh);
-    if (a.tokens) {
-      const u64_t target = threshold();
-      if (tid == 0) sh.bin = 0, sh.before = 0, sh.token = V, sh.last = -1;
-      __syncthreads();
-      if (here > 0 && before < target && before + here >= target) sh.bin = tid, sh.before = before;
-      __syncthreads();
-      const u64_t left = target - sh.before;
-      const int i0 = sh.bin * kChunk + tid * (kChunk / kRowThreads);
-      u64_t w[kChunk / kRowThreads], sum = 0, all;
-#pragma unroll
-      for (int j = 0; j < kChunk / kRowThreads / VEC; j++) {
-        float l[VEC];
-        x.get(i0 + j * VEC, false, l);
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          const int i = i0 + j * VEC + e;
-          w[j * VEC + e] = i < V && kept(l[e], i) ? mass(l[e]) : 0;
-          sum += w[j * VEC + e];
-        }
+      v = ~(uint32_t)index, m = 1;
+      return key == at;
+    });
+  };
+  if (rules.by_k && (!fast || b.k_bin >= 0)) {
+    u64_t target = fast ? b.k_left : rules.k, ties;
+    const uint32_t at = group.cross(n, target, ties, [&](int i, uint32_t& v, u64_t& m) {
+      int index;
+      element(i, v, index);
+      m = 1;
+      return !fast || bin_of(v) == b.k_bin;
+    });
+    cut_ties(at, target, ties);
+  }
+  if (rules.by_p) {
+    auto in_p = [&](uint32_t key, int index) {
+      if (!before_cut(key, index)) return false;
+      const int g = fast ? bin_of(key) : b.p_first;
+      return g >= b.p_first && g <= b.p_last;
+    };
+    auto mass_at = [&](int i) -> u64_t {
+      uint32_t key;
+      int index;
+      element(i, key, index);
+      return in_p(key, index) ? mass(Row::logit(key)) : 0;
+    };
+    double total = b.sum;
+    const u64_t most = group.sum(n, mass_at);
+    if (!fast)
+      total = (double)most / one;
+    else if (rules.by_k)
+      total = b.before_k + (double)group.sum(n, [&](int i) -> u64_t {
+                uint32_t key;
+                int index;
+                element(i, key, index);
+                return bin_of(key) == b.k_bin && before_cut(key, index) ? mass(Row::logit(key)) : 0;
+              }) / one;
+    const double bar = __builtin_ceil((rules.p * total - (fast ? b.before_p : 0.0)) * one);
+    u64_t target = bar >= 1.0 ? min((u64_t)bar, most) : 1, here;
+    if (most > 0) {
+      const uint32_t at = group.cross(n, target, here, [&](int i, uint32_t& v, u64_t& m) {
+        int index;
+        element(i, v, index);
+        if (!in_p(v, index)) return false;
+        m = mass(Row::logit(v));
+        return true;
+      });
+      const u64_t each = mass(Row::logit(at));
+      if (each > 0) {
+        const u64_t count = (target + each - 1) / each;
+        // where the key is top-k's too, the ties are those that it keeps
+        if (at != cut || count < here / each) cut_ties(at, count, here / each);
       }
-      u64_t run = row_scan(sum, all, sh);
-      int found = V, last = -1;
-#pragma unroll
-      for (int j = 0; j < kChunk / kRowThreads; j++) {
-        run += w[j];
-        if (w[j] > 0) {
-          last = i0 + j;
-          if (run >= left) found = min(found, i0 + j);
-        }
-      }
-      if (found < V) atomicMin(&sh.token, found);
-      if (last >= 0) atomicMax(&sh.last, last);  // rounding may leave the threshold to nobody
-      __syncthreads();
-      if (tid == 0) a.tokens[row] = sh.token < V ? sh.token : sh.last;
     }
   }
-  if (a.cuts && tid == 0) a.cuts[row] = SampleCut{cut, cut_at, by_m ? rules.m : 0.0, one / (double)total, M};
-}
 
-template <int TYPE>
-__global__ __launch_bounds__(kChunkThreads) void sample_probs_kernel(const SampleArgs a) {
-  constexpr int VEC = SampleRow<TYPE>::VEC;
-  typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
-  const int row = blockIdx.y;
-  const SampleRow<TYPE> x = sample_row<TYPE>(a, row);
-  const SampleCut cut = a.cuts[row];
-  const double scale = sample_rules(a, row).scale;
-  float* out = a.probs + (size_t)row * a.vocab;
+  // the kept sum of every chunk, and the token
+  u64_t total = 0;
+  if (!fast) {
+    for (int c = tid; c < C; c += kRowThreads) sh.chunk_mass[c] = 0;
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += kRowThreads) {
+    uint32_t key;
+    int index;
+    element(i, key, index);
+    const float l = Row::logit(key);
+    if ((!fast || bin_of(key) <= b.last) && kept(l, index)) atomicAdd(&sh.chunk_mass[index / CHUNK], mass(l));
+  }
+  __syncthreads();
+  const u64_t here = tid < C ? sh.chunk_mass[tid] : 0;
+  const u64_t before = group.scan(here, total);
+  if (tid == 0) border->cut = cut, border->cut_at = cut_at, border->inv = one / (double)total;
+  if (!a.tokens) return;
+  const float u = a.uniform[row];
+  const double bar = (u > 0.f ? (double)u : 0.0) * (double)total;  // the smallest whole number above it
+  const u64_t target = bar < (double)total ? min((u64_t)bar + 1, total) : total;
+  if (tid == 0) sh.token = V, sh.last = -1, sh.found[0] = SampleFound{0, 0, 0};
+  __syncthreads();
+  if (here > 0 && before < target && before + here >= target) sh.found[0] = SampleFound{before, here, tid};
+  __syncthreads();
+  const u64_t left = target - sh.found[0].before;
+  const int i0 = sh.found[0].bin * CHUNK + tid * EACH;
+  u64_t w[EACH], sum = 0, all;
 #pragma unroll
-  for (int j = 0; j < kEach / VEC; j++) {
-    const int i = blockIdx.x * kChunk + (j * kChunkThreads + (int)threadIdx.x) * VEC;
-    float l[VEC], p[VEC];
-    x.get(i, false, l);
+  for (int j = 0; j < EACH / VEC; j++) {
+    float l[VEC];
+    x.get(i0 + j * VEC, false, l);
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
-      const uint32_t key = sample_key(l[e]);
-      p[e] = 0.f;
-      if (cut.inv > 0.0 && (key > cut.key || (key == cut.key && i + e <= cut.at))) {
-        const double w = sample_weight(l[e], cut.m, scale);
-        p[e] = w >= cut.min_w ? (float)(w * cut.inv) : 0.f;
-      }
+      const int i = i0 + j * VEC + e;
+      w[j * VEC + e] = i < V && kept(l[e], i) ? mass(l[e]) : 0;
+      sum += w[j * VEC + e];
     }
-    if (i + VEC <= a.vocab) {
+  }
+  u64_t run = group.scan(sum, all);
+  int found = V, last = -1;
 #pragma unroll
-      for (int e = 0; e < VEC; e += 4) *reinterpret_cast<f4_t*>(out + i + e) = f4_t{p[e], p[e + 1], p[e + 2], p[e + 3]};
+  for (int j = 0; j < EACH; j++) {
+    run += w[j];
+    if (w[j] > 0) {
+      last = i0 + j;
+      if (run >= left) found = min(found, i0 + j);
+    }
+  }
+  if (found < V && run - sum < left) atomicMin(&sh.token, found);
+  if (last >= 0) atomicMax(&sh.last, last);  // rounding may leave the threshold to nobody
+  __syncthreads();
+  if (tid == 0) a.tokens[row] = sh.token < V ? sh.token : sh.last;
+}
+
+template <int TYPE, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_probs_kernel(const SampleArgs a) {
+  using Row = SampleRow<TYPE>;
+  constexpr int VEC = Row::VEC;
+  typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
+  const int row = blockIdx.y, first = blockIdx.x * (THREADS * kEach);
+  const bool whole = first + THREADS * kEach <= a.vocab;
+  float l[kEach], p[kEach];
+  sample_row<TYPE>(a, row).get_each(first + (int)threadIdx.x * VEC, THREADS * VEC, whole, l);
+  const SampleBorder* border = a.border + row;
+  const double inv = border->inv;
+  const float m = border->m;
+  const uint32_t cut = border->cut;
+  const int cut_at = border->cut_at;
+  const SampleRules rules = sample_rules(a, row);
+  float* out = a.probs + (size_t)row * a.vocab;
+#pragma unroll
+  for (int i = 0; i < kEach; i++) {
+    const int at = first + (i / VEC * THREADS + (int)threadIdx.x) * VEC + i % VEC;
+    const uint32_t key = Row::key(l[i]);
+    p[i] = 0.f;
+    if (inv > 0.0 && (key > cut || (key == cut && at <= cut_at))) {
+      const double w = sample_weight(l[i], m, rules.scale);
+      p[i] = w >= rules.m ? (float)(w * inv) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kEach / VEC; j++) {
+    const int at = first + (j * THREADS + (int)threadIdx.x) * VEC;
+    const float* q = p + j * VEC;
+    if (at + VEC <= a.vocab) {
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4) *reinterpret_cast<f4_t*>(out + at + e) = f4_t{q[e], q[e + 1], q[e + 2], q[e + 3]};
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; e++)
-        if (i + e < a.vocab) out[i + e] = p[e];
+        if (at + e < a.vocab) out[at + e] = q[e];
     }
   }
 }
 
-static size_t sample_chunk_bytes(int rows, int vocab) {
-  const size_t chunks = (vocab + kChunk - 1) / kChunk;
-  return rows * chunks * (sizeof(SampleChunk) + kBins * (sizeof(u64_t) + sizeof(int)));
+// Chunks of 8192 elements, or 4096 for more workgroups where there are few elements in all (one row of 32003 fp32: TODO us)
+static int sample_chunk(int rows, int vocab) { return (long long)rows * vocab <= (1 << 19) ? kSmallChunk : kLargeChunk; }
+static size_t sample_bytes(int rows, int chunks) {
+  return rows * (sizeof(SampleBorder) + kList * sizeof(u64_t) +
+                 chunks * (sizeof(SampleChunk) + sizeof(u64_t) + kBins * (sizeof(u64_t) + sizeof(int))));
+}
+
+template <int TYPE, int THREADS>
+static hipError_t sample_launch(const SampleArgs& a, bool ruled, hipStream_t st) {
+  const dim3 grid(a.chunks, a.rows);
+  sample_chunk_kernel<TYPE, THREADS><<<grid, THREADS, 0, st>>>(a);
+  sample_border_kernel<<<a.rows, kBorderThreads, 0, st>>>(a);
+  if (ruled) sample_list_kernel<TYPE, THREADS><<<grid, THREADS, 0, st>>>(a);
+  sample_row_kernel<TYPE, THREADS * kEach><<<a.rows, kRowThreads, 0, st>>>(a);
+  if (a.probs) sample_probs_kernel<TYPE, THREADS><<<grid, THREADS, 0, st>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace exl3
@@ -694,15 +851,18 @@ using namespace exl3;
 
 extern "C" size_t exl3_sample_workspace_bytes(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab) return 0;
-  return sample_chunk_bytes(rows, vocab) + rows * sizeof(SampleCut);
+  // the most that up to `rows` rows need: fewer may take smaller chunks
+  const int slice = std::min(rows, kSliceRows), chunk = sample_chunk(rows, vocab);
+  const int few = std::min(rows, (1 << 19) / vocab);
+  return std::max(sample_bytes(slice, (vocab + chunk - 1) / chunk), sample_bytes(few, (vocab + kSmallChunk - 1) / kSmallChunk));
 }
 
 extern "C" int exl3_sample(const void* logits, int type, long long ld, int rows, int vocab, const float* uniform,
                            const float* temperature, double all_temperature, const int* top_k, int all_top_k,
                            const float* top_p, double all_top_p, const float* min_p, double all_min_p, int* tokens, float* probs,
                            void* workspace, size_t workspace_bytes, void* stream) {
-  EXL3_CHECK_ARG(rows >= 0 && rows <= 65535 && vocab >= 1 && vocab <= kMaxVocab,
-                 "exl3_sample: rows = %d (up to 65535), vocab = %d (1 to %d)", rows, vocab, kMaxVocab);
+  EXL3_CHECK_ARG(rows >= 0 && rows < (1 << 26) && vocab >= 1 && vocab <= kMaxVocab,
+                 "exl3_sample: rows = %d, vocab = %d (1 to %d)", rows, vocab, kMaxVocab);
   EXL3_CHECK_ARG(type >= EXL3_F16 && type <= EXL3_F32, "exl3_sample: logits type %d", type);
   if (rows == 0) return EXL3_OK;
   EXL3_CHECK_ARG(tokens || probs, "exl3_sample: neither tokens nor probabilities");
@@ -718,24 +878,26 @@ extern "C" int exl3_sample(const void* logits, int type, long long ld, int rows,
   EXL3_CHECK_ARG(apart(all, 3), "exl3_sample: an output or the workspace overlaps another tensor of the call");
   int shift = 52;
   while ((1ll << (62 - shift)) < vocab) shift--;
-  const int chunks = (vocab + kChunk - 1) / kChunk;
-  SampleChunk* chunk = static_cast<SampleChunk*>(workspace);
-  u64_t* bin_mass = reinterpret_cast<u64_t*>(chunk + n * chunks);
-  int* bin_count = reinterpret_cast<int*>(bin_mass + n * chunks * kBins);
-  SampleCut* cuts = reinterpret_cast<SampleCut*>(static_cast<char*>(workspace) + sample_chunk_bytes(rows, vocab));
-  const SampleArgs a{logits, ld, rows, vocab, shift, uniform, temperature, top_p, min_p, top_k, all_temperature, all_top_p,
-                     all_min_p, all_top_k, tokens, probs, chunks, chunk, bin_mass, bin_count, probs ? cuts : nullptr};
-  hipStream_t st = as_stream(stream);
-  const dim3 grid(chunks, rows);
-#define EXL3_BY_TYPE(kern) (type == EXL3_F32 ? kern<EXL3_F32> : type == EXL3_BF16 ? kern<EXL3_BF16> : kern<EXL3_F16>)
-  EXL3_BY_TYPE(sample_chunk_kernel)<<<grid, kChunkThreads, 0, st>>>(a);
-  EXL3_CHECK_LAUNCH();
-  EXL3_BY_TYPE(sample_row_kernel)<<<rows, kRowThreads, 0, st>>>(a);
-  EXL3_CHECK_LAUNCH();
-  if (probs) {
-    EXL3_BY_TYPE(sample_probs_kernel)<<<grid, kChunkThreads, 0, st>>>(a);
-    EXL3_CHECK_LAUNCH();
+  const int chunk = sample_chunk(rows, vocab), chunks = (vocab + chunk - 1) / chunk;
+  const bool ruled = temperature || top_k || top_p || min_p || !(all_temperature > 0.0) || (all_top_k > 0 && all_top_k < vocab) ||
+                     all_top_p < 1.0 || all_min_p > 0.0;
+  for (int first = 0; first < rows; first += kSliceRows) {
+    const int slice = std::min(rows - first, kSliceRows);
+    auto from = [&](auto* p, long long step) { return p ? p + first * step : p; };
+    SampleArgs a{static_cast<const char*>(logits) + (size_t)first * ld * bytes, ld, slice, vocab, shift, from(uniform, 1),
+                 from(temperature, 1), from(top_p, 1), from(min_p, 1), from(top_k, 1), all_temperature, all_top_p, all_min_p,
+                 all_top_k, from(tokens, 1), from(probs, vocab), chunks};
+    a.border = static_cast<SampleBorder*>(workspace);
+    a.list = reinterpret_cast<u64_t*>(a.border + slice);
+    a.bin_mass = a.list + (size_t)slice * kList;
+    a.chunk_mass = a.bin_mass + (size_t)slice * chunks * kBins;
+    a.chunk = reinterpret_cast<SampleChunk*>(a.chunk_mass + (size_t)slice * chunks);
+    a.bin_count = reinterpret_cast<int*>(a.chunk + (size_t)slice * chunks);
+    const bool large = chunk == kLargeChunk;
+    hipStream_t st = as_stream(stream);
+    EXL3_CHECK_HIP(type == EXL3_F32    ? (large ? sample_launch<EXL3_F32, 1024>(a, ruled, st) : sample_launch<EXL3_F32, 512>(a, ruled, st))
+                   : type == EXL3_BF16 ? (large ? sample_launch<EXL3_BF16, 1024>(a, ruled, st) : sample_launch<EXL3_BF16, 512>(a, ruled, st))
+                                       : (large ? sample_launch<EXL3_F16, 1024>(a, ruled, st) : sample_launch<EXL3_F16, 512>(a, ruled, st)));
   }
-#undef EXL3_BY_TYPE
   return EXL3_OK;
 }
