@@ -420,7 +420,7 @@ int exl3_kv_step_plan(int* page_table, int max_pages, const int* seq_lens, const
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* From one block of a model to the next: for each row x (a block's output) and r (the residual stream) of `dim` values
- * (1 to 65536; strides ld_* in elements)
+ * (1 to 32768; strides ld_* in elements)
  *   u = x, or with post_weight  x * rsqrt(mean(x^2) + eps) * post_weight
  *   h = r + scale * act(gate) * u         act: the value itself, or its sigmoid (gate_sigmoid)
  *   y = h * rsqrt(mean(h^2) + eps) * weight

@@ -12,10 +12,15 @@
 
 #include "exl3_api.hpp"
 #include "exl3_device.hpp"
+#include "kv_device.hpp"
 
 namespace exl3 {
 
-typedef uint32_t an_u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t an_u32x4_t __attribute__((ext_vector_type(4), aligned(2)));  // rows start at any value
+typedef uint32_t an_b128_t __attribute__((ext_vector_type(4)));
+typedef float an_f32x4_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef float an_f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 an_bf16x2_t __attribute__((ext_vector_type(2)));
 
 enum { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
 
@@ -30,141 +35,294 @@ struct AddNormArgs {
   void *y, *h;
 };
 
-template <int VEC>
-__device__ __forceinline__ void an_load(const void* p, int type, long long at, float v[VEC]) {
-  if constexpr (VEC == 1) {
-    if (type == EXL3_F32) {
-      v[0] = static_cast<const float*>(p)[at];
+__device__ __forceinline__ void an_unpack(an_u32x4_t r, int type, float v[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t u = r[i];
+    if (type == EXL3_BF16) {
+      v[2 * i] = __builtin_bit_cast(float, u << 16), v[2 * i + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
     } else {
-      const uint16_t u = static_cast<const uint16_t*>(p)[at];
-      v[0] = type == EXL3_BF16 ? __builtin_bit_cast(float, (uint32_t)u << 16) : (float)__builtin_bit_cast(_Float16, u);
-    }
-  } else {
-    if (type == EXL3_F32) {
-      const float4_t* q = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at);
-      const float4_t a = q[0], b = q[1];
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
-      return;
-    }
-    const an_u32x4_t r = *reinterpret_cast<const an_u32x4_t*>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t u = r[i];
-      if (type == EXL3_BF16) {
-        v[2 * i] = __builtin_bit_cast(float, u << 16), v[2 * i + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
-      } else {
-        const half2_t h = __builtin_bit_cast(half2_t, u);
-        v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
-      }
+      const half2_t h = __builtin_bit_cast(half2_t, u);
+      v[2 * i] = (float)h[0], v[2 * i + 1] = (float)h[1];
     }
   }
 }
 
-template <int VEC>
-__device__ __forceinline__ void an_store(void* p, int type, long long at, const float v[VEC]) {
-  if constexpr (VEC == 1) {
-    if (type == EXL3_F32)
-      static_cast<float*>(p)[at] = v[0];
-    else
-      static_cast<uint16_t*>(p)[at] =
-          type == EXL3_BF16 ? f32_to_bf16(v[0]) : __builtin_bit_cast(uint16_t, (_Float16)v[0]);
+__device__ __forceinline__ float an_value(const void* p, int type, long long at) {
+  if (type == EXL3_F32) return static_cast<const float*>(p)[at];
+  const uint16_t u = static_cast<const uint16_t*>(p)[at];
+  return type == EXL3_BF16 ? __builtin_bit_cast(float, (uint32_t)u << 16) : (float)__builtin_bit_cast(_Float16, u);
+}
+
+// values at .. at + 7 of a row, 0 past the first n (1 at least)
+__device__ __forceinline__ void an_load(const void* p, int type, long long at, int n, float v[8]) {
+  if (n < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = e < n ? an_value(p, type, at + e) : 0.f;
+  } else if (type == EXL3_F32) {
+    const an_f32x4_t* q = reinterpret_cast<const an_f32x4_t*>(static_cast<const float*>(p) + at);
+    const an_f32x4_t a = q[0], b = q[1];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
   } else {
-    if (type == EXL3_F32) {
-      float4_t* q = reinterpret_cast<float4_t*>(static_cast<float*>(p) + at);
-      q[0] = float4_t{v[0], v[1], v[2], v[3]}, q[1] = float4_t{v[4], v[5], v[6], v[7]};
-      return;
+    an_unpack(*reinterpret_cast<const an_u32x4_t*>(static_cast<const uint16_t*>(p) + at), type, v);
+  }
+}
+
+// two values in 16 bits, rounded to nearest even
+template <int TYPE>
+__device__ __forceinline__ uint32_t an_pair(float a, float b) {
+  if constexpr (TYPE == EXL3_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((an_f32x2_t{a, b}), an_bf16x2_t));
+  else
+    return __builtin_bit_cast(uint32_t, half2_t{(_Float16)a, (_Float16)b});
+}
+
+template <int TYPE>
+__device__ __forceinline__ void an_store(void* p, long long at, int n, const float v[8]) {
+  if (n < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (e >= n) continue;
+      if constexpr (TYPE == EXL3_F32)
+        static_cast<float*>(p)[at + e] = v[e];
+      else
+        static_cast<uint16_t*>(p)[at + e] = (uint16_t)an_pair<TYPE>(v[e], 0.f);
     }
+  } else if constexpr (TYPE == EXL3_F32) {
+    an_f32x4_t* q = reinterpret_cast<an_f32x4_t*>(static_cast<float*>(p) + at);
+    q[0] = an_f32x4_t{v[0], v[1], v[2], v[3]}, q[1] = an_f32x4_t{v[4], v[5], v[6], v[7]};
+  } else {
     an_u32x4_t r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (type == EXL3_BF16)
-        r[i] = (uint32_t)f32_to_bf16(v[2 * i]) | ((uint32_t)f32_to_bf16(v[2 * i + 1]) << 16);
-      else
-        r[i] = __builtin_bit_cast(uint32_t, half2_t{(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
-    }
+    for (int i = 0; i < 4; i++) r[i] = an_pair<TYPE>(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<an_u32x4_t*>(static_cast<uint16_t*>(p) + at) = r;
   }
 }
 
-// the sum over the workgroup, in every lane; `part`: LDS, a float a wave, of its own for each call
-__device__ __forceinline__ float an_sum(float v, float* part, int waves) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  if (waves == 1) return v;
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = 0.f;
-  for (int w = 0; w < waves; w++) s += part[w];
-  return s;
-}
+__device__ __forceinline__ float an_act(const AddNormArgs& a, float g) { return a.sigmoid ? 1.0f / (1.0f + expf(-g)) : g; }
 
-// VEC values at a time, R times a thread
-template <int VEC, int R>
-__global__ __launch_bounds__(1024) void add_norm_kernel(const AddNormArgs a) {
+// the sum over the workgroup, in every lane; `slot` alternates, so that one barrier a sum is enough
+struct AddNormSum {
+  float (*part)[16];
+  int waves, slot;
+  __device__ __forceinline__ float operator()(float v) {
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xF, 0xF, false));  // row_ror:4
+    v += lane_xor<8>(v);
+    v = sum_over_groups(v);
+    if (waves == 1) return v;
+    slot ^= 1;
+    if ((threadIdx.x & 63) == 0) part[slot][threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int w = 0; w < waves; w++) s += part[slot][w];
+    return s;
+  }
+};
+
+// Rows of any width, stride and alignment: a workgroup a row, R times 8 values a thread
+template <int R, int XT, int RT>
+__global__ __launch_bounds__(512) void add_norm_any_kernel(const AddNormArgs a) {
   __shared__ float part[2][16];
-  const long long row = blockIdx.x;
-  const int waves = blockDim.x >> 6;
-  const long long x0 = row * a.ld_x, r0 = row * a.ld_r, o0 = row * a.dim;
-  float u[R][VEC];
-  float ss = 0.f;
+  AddNormSum sum{part, (int)(blockDim.x >> 6), 0};
+  const long long row = blockIdx.x, o0 = row * a.dim;
+  float token = a.scale;
+  if (a.gate_kind == kGateToken) token *= an_act(a, an_value(a.gate, a.g_type, row * a.ld_g));
+  float u[R][8], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < R; i++) {
-    const int d = (threadIdx.x + i * blockDim.x) * VEC;
+    const int d = (threadIdx.x + i * blockDim.x) * 8;
 #pragma unroll
-    for (int e = 0; e < VEC; e++) u[i][e] = 0.f;
-    if (d < a.dim) an_load<VEC>(a.x, a.x_type, x0 + d, u[i]);
+    for (int e = 0; e < 8; e++) u[i][e] = 0.f;
+    if (d < a.dim) an_load(a.x, XT, row * a.ld_x + d, a.dim - d, u[i]);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) ss = __builtin_fmaf(u[i][e], u[i][e], ss);
+    for (int e = 0; e < 8; e++) ss = __builtin_fmaf(u[i][e], u[i][e], ss);
   }
   float post = 1.f;
-  if (a.post_weight) post = 1.0f / __builtin_sqrtf(an_sum(ss, part[0], waves) / (float)a.dim + a.eps);
-  float g_token = 1.f;
-  if (a.gate_kind == kGateToken) an_load<1>(a.gate, a.g_type, row * a.ld_g, &g_token);
-  auto act = [&](float g) { return a.sigmoid ? 1.0f / (1.0f + expf(-g)) : g; };
-  const float token = a.scale * (a.gate_kind == kGateToken ? act(g_token) : 1.f);
+  if (a.post_weight) post = 1.0f / __builtin_sqrtf(sum(ss) / (float)a.dim + a.eps);
   ss = 0.f;
 #pragma unroll
   for (int i = 0; i < R; i++) {
-    const int d = (threadIdx.x + i * blockDim.x) * VEC;
-    if (d >= a.dim) continue;
-    float w[VEC];
+    const int d = (threadIdx.x + i * blockDim.x) * 8, n = a.dim - d;
+    if (n <= 0) continue;
+    float w[8], r[8];
     if (a.post_weight) {
-      an_load<VEC>(a.post_weight, a.w_type, d, w);
+      an_load(a.post_weight, a.w_type, d, n, w);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) u[i][e] *= post * (w[e] + a.offset);
+      for (int e = 0; e < 8; e++) u[i][e] *= post * (w[e] + a.offset);
     }
-    if (a.gate_kind == kGateChannel || a.gate_kind == kGateFull) {
-      an_load<VEC>(a.gate, a.g_type, (a.gate_kind == kGateFull ? row * a.ld_g : 0) + d, w);
+    if (a.gate_kind == kGateFull || a.gate_kind == kGateChannel) {
+      an_load(a.gate, a.g_type, (a.gate_kind == kGateFull ? row * a.ld_g : 0) + d, n, w);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) u[i][e] *= act(w[e]);
+      for (int e = 0; e < 8; e++) u[i][e] *= an_act(a, w[e]);
     }
-    float r[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; e++) r[e] = 0.f;
-    if (a.residual) an_load<VEC>(a.residual, a.r_type, r0 + d, r);
+    for (int e = 0; e < 8; e++) r[e] = 0.f;
+    if (a.residual) an_load(a.residual, RT, row * a.ld_r + d, n, r);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
-      u[i][e] = __builtin_fmaf(u[i][e], token, r[e]);
+    for (int e = 0; e < 8; e++) {
+      u[i][e] = e < n ? __builtin_fmaf(u[i][e], token, r[e]) : 0.f;
       ss = __builtin_fmaf(u[i][e], u[i][e], ss);
     }
-    if (a.h) an_store<VEC>(a.h, a.r_type, o0 + d, u[i]);
+    if (a.h) an_store<RT>(a.h, o0 + d, n, u[i]);
   }
   if (!a.y) return;
-  const float pre = 1.0f / __builtin_sqrtf(an_sum(ss, part[1], waves) / (float)a.dim + a.eps);
+  const float pre = 1.0f / __builtin_sqrtf(sum(ss) / (float)a.dim + a.eps);
 #pragma unroll
   for (int i = 0; i < R; i++) {
-    const int d = (threadIdx.x + i * blockDim.x) * VEC;
-    if (d >= a.dim) continue;
-    float w[VEC];
-    an_load<VEC>(a.weight, a.w_type, d, w);
+    const int d = (threadIdx.x + i * blockDim.x) * 8, n = a.dim - d;
+    if (n <= 0) continue;
+    float w[8];
+    an_load(a.weight, a.w_type, d, n, w);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) w[e] = u[i][e] * pre * (w[e] + a.offset);
-    an_store<VEC>(a.y, a.x_type, o0 + d, w);
+    for (int e = 0; e < 8; e++) w[e] = u[i][e] * pre * (w[e] + a.offset);
+    an_store<XT>(a.y, o0 + d, n, w);
   }
 }
 
-constexpr int kAddNormMaxDim = 65536;
+// A row of n bytes as a buffer: what lies past it (all of it where p is null) reads as 0 and is not written
+struct AddNormBuffer {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ AddNormBuffer(const void* p, long long at, int n)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)(static_cast<const char*>(p) + (p ? at : 0)), (short)0, p ? n : 0,
+                                               0x00020000)) {}
+  __device__ __forceinline__ an_u32x4_t load(int at) const {
+    return __builtin_bit_cast(an_u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+  }
+  __device__ __forceinline__ void store(int at, an_u32x4_t v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(an_b128_t, v), rsrc, at, 0, 0);
+  }
+};
+template <int TYPE>
+__device__ __forceinline__ void an_unpack_row(const an_u32x4_t* r, float v[8]) {
+  if constexpr (TYPE == EXL3_F32) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const uint32_t u = r[e / 4][e & 3];
+      v[e] = __builtin_bit_cast(float, u);
+    }
+  } else {
+    an_unpack(r[0], TYPE, v);
+  }
+}
+template <int TYPE>
+__device__ __forceinline__ void an_put(const AddNormBuffer& to, int d, const float v[8]) {
+  an_u32x4_t r[2];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (TYPE == EXL3_F32)
+      r[0][i] = __builtin_bit_cast(uint32_t, v[i]), r[1][i] = __builtin_bit_cast(uint32_t, v[4 + i]);
+    else
+      r[0][i] = an_pair<TYPE>(v[2 * i], v[2 * i + 1]);
+  }
+  to.store(d * (TYPE == EXL3_F32 ? 4 : 2), r[0]);
+  if constexpr (TYPE == EXL3_F32) to.store(d * 4 + 16, r[1]);
+}
+
+// Rows of multiples of 8 values that lie at multiples of 16 bytes, up to 16 values a thread.  A workgroup takes rows blockIdx.x,
+// + gridDim.x, ..: the next row is loaded before this one is worked on; weights and a gate of one value a channel stay in
+// registers.  Loads and stores go through buffers, without a branch: the wait for a row's loads then leaves the stores behind them
+// out (with lane-conditional stores the compiler waits for everything: 112 us instead of TODO at 8192 rows of 5120).
+template <int R>
+constexpr int kAddNormThreads = R == 1 ? 1024 : 512;
+
+template <int R, int XT, int RT>
+__global__ __launch_bounds__(kAddNormThreads<R>) void add_norm_rows_kernel(const AddNormArgs a) {
+  constexpr int WIDE = RT == EXL3_F32 ? 2 : 1;
+  __shared__ float part[2][16];
+  AddNormSum sum{part, (int)(blockDim.x >> 6), 0};
+  const int x_bytes = a.dim * 2, r_bytes = a.dim * 2 * WIDE;
+  int d[R];
+  float w[R][8], p[R][8], g[R][8];  // weight, post_weight, gate a channel
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    d[i] = (threadIdx.x + i * blockDim.x) * 8;
+    const int n = a.dim - d[i];
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[i][e] = 0.f, p[i][e] = g[i][e] = 1.f;
+    if (n <= 0) continue;
+    if (a.weight) an_load(a.weight, a.w_type, d[i], n, w[i]);
+    if (a.post_weight) an_load(a.post_weight, a.w_type, d[i], n, p[i]);
+    if (a.gate_kind == kGateChannel) an_load(a.gate, a.g_type, d[i], n, g[i]);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      w[i][e] += a.offset;
+      if (a.post_weight) p[i][e] += a.offset;
+      if (a.gate_kind == kGateChannel) g[i][e] = an_act(a, g[i][e]);
+      p[i][e] *= g[i][e];
+    }
+  }
+  const bool full = a.gate_kind == kGateFull;  // (in 16 bits)
+  an_u32x4_t x[R], r[R][WIDE], f[R];
+  auto load = [&](long long row) {
+    const AddNormBuffer bx(a.x, row * a.ld_x * 2, x_bytes), br(a.residual, row * a.ld_r * 2 * WIDE, r_bytes),
+        bf(full ? a.gate : nullptr, row * a.ld_g * 2, x_bytes);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      x[i] = bx.load(2 * d[i]);
+#pragma unroll
+      for (int j = 0; j < WIDE; j++) r[i][j] = br.load(2 * WIDE * d[i] + 16 * j);
+      f[i] = bf.load(2 * d[i]);
+    }
+  };
+  const float inv_dim = 1.0f / (float)a.dim;
+  long long row = blockIdx.x;
+  load(row);
+  while (true) {
+    float u[R][8], h[R][8], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      an_unpack(x[i], XT, u[i]);
+#pragma unroll
+      for (int e = 0; e < 8; e++) ss = __builtin_fmaf(u[i][e], u[i][e], ss);
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[i][e] *= p[i][e];
+      if (full) {
+        float q[8];
+        an_unpack(f[i], a.g_type, q);
+#pragma unroll
+        for (int e = 0; e < 8; e++) u[i][e] *= an_act(a, q[e]);
+      }
+      an_unpack_row<RT>(r[i], h[i]);
+    }
+    const long long after = row + gridDim.x;
+    load(min(after, (long long)a.rows - 1));
+    float token = a.scale;
+    if (a.gate_kind == kGateToken) token *= an_act(a, an_value(a.gate, a.g_type, row * a.ld_g));
+    if (a.post_weight) token *= 1.0f / __builtin_sqrtf(sum(ss) * inv_dim + a.eps);
+    ss = 0.f;
+    const AddNormBuffer bh(a.h, row * r_bytes, r_bytes), by(a.y, row * x_bytes, x_bytes);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        h[i][e] = __builtin_fmaf(u[i][e], token, h[i][e]);
+        ss = __builtin_fmaf(h[i][e], h[i][e], ss);
+      }
+      an_put<RT>(bh, d[i], h[i]);
+    }
+    const float pre = 1.0f / __builtin_sqrtf(sum(ss) * inv_dim + a.eps);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) h[i][e] *= pre * w[i][e];
+      an_put<XT>(by, d[i], h[i]);
+    }
+    if (after >= a.rows) break;
+    row = after;
+  }
+}
+
+template <int XT, int RT>
+static void add_norm_launch(const AddNormArgs& a, bool even, int threads, int each, int grid, hipStream_t st) {
+  auto kern = even ? (each <= 1 ? add_norm_rows_kernel<1, XT, RT> : add_norm_rows_kernel<2, XT, RT>)
+                   : (each <= 1 ? add_norm_any_kernel<1, XT, RT> : each <= 4 ? add_norm_any_kernel<4, XT, RT> : add_norm_any_kernel<8, XT, RT>);
+  kern<<<grid, threads, 0, st>>>(a);
+}
+
+constexpr int kAddNormMaxDim = 32768;  // eight times 8 values of 512 threads
 
 }  // namespace exl3
 
@@ -202,21 +360,29 @@ extern "C" int exl3_add_norm(const void* x, int x_type, long long ld_x, const vo
   EXL3_CHECK_ARG(apart(all, 2), "exl3_add_norm: an output overlaps another tensor of the call");
   const AddNormArgs a{x, residual, weight, post_weight, gate, ld_x, ld_r, ld_g, x_type, r_type, w_type, g_type, gate_kind,
                       gate_sigmoid, weight_offset ? 1.f : 0.f, scale, eps, rows, dim, y, h};
-  // 8 values at a time where every row of every tensor starts at a multiple of 16 bytes
-  const bool vec = dim % 8 == 0 && ld_x % 8 == 0 && (!residual || ld_r % 8 == 0) && (gate_kind != kGateFull || ld_g % 8 == 0) &&
-                   (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)post_weight | (uintptr_t)y |
-                     (uintptr_t)h | (gate_kind == kGateToken ? 0 : (uintptr_t)gate)) & 15) == 0;
-  const int chunks = vec ? dim / 8 : dim;
-  const int threads = std::min(1024, (chunks + 63) / 64 * 64), each = (chunks + threads - 1) / threads;
-  hipStream_t st = as_stream(stream);
-  if (vec) {
-    auto kern = each <= 1 ? add_norm_kernel<8, 1> : each <= 2 ? add_norm_kernel<8, 2> : each <= 4 ? add_norm_kernel<8, 4>
-                                                                                            : add_norm_kernel<8, 8>;
-    kern<<<rows, threads, 0, st>>>(a);
-  } else {
-    auto kern = each <= 4 ? add_norm_kernel<1, 4> : each <= 16 ? add_norm_kernel<1, 16> : add_norm_kernel<1, 64>;
-    kern<<<rows, threads, 0, st>>>(a);
+  const int chunks = (dim + 7) / 8;
+  const bool even = dim % 8 == 0 && chunks <= 1024 && ld_x % 8 == 0 && (!residual || ld_r % 8 == 0) &&
+                    (gate_kind != kGateFull || (ld_g % 8 == 0 && g_type != EXL3_F32)) &&
+                    (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)h |
+                      (gate_kind == kGateFull ? (uintptr_t)gate : 0)) & 15) == 0;
+  // Few rows: as many threads as there are values to load.  Many: 16 values a thread, and workgroups that stay for several rows
+  // (as many each), six waves a SIMD.
+  const bool many = rows > 1024;
+  int threads = (std::min(chunks, even ? 1024 : 512) + 63) / 64 * 64, grid = rows;
+  if (even && many) {
+    if (chunks > 64) threads = (chunks + 127) / 128 * 64;
+    const int fit = 256 * std::max(1, 1536 / threads), rounds = (rows + fit - 1) / fit;
+    grid = (rows + rounds - 1) / rounds;
   }
+  const int each = (chunks + threads - 1) / threads;
+  hipStream_t st = as_stream(stream);
+  auto launch = x_type == EXL3_BF16 ? (r_type == EXL3_F32    ? add_norm_launch<EXL3_BF16, EXL3_F32>
+                                       : r_type == EXL3_BF16 ? add_norm_launch<EXL3_BF16, EXL3_BF16>
+                                                             : add_norm_launch<EXL3_BF16, EXL3_F16>)
+                                    : (r_type == EXL3_F32    ? add_norm_launch<EXL3_F16, EXL3_F32>
+                                       : r_type == EXL3_BF16 ? add_norm_launch<EXL3_F16, EXL3_BF16>
+                                                             : add_norm_launch<EXL3_F16, EXL3_F16>);
+  launch(a, even, threads, each, grid, st);
   EXL3_CHECK_LAUNCH();
   return EXL3_OK;
 }

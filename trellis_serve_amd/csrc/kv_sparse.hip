@@ -52,75 +52,57 @@ __device__ __forceinline__ uint32_t min_i16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(kv_i16x2_t, a),
                                                                 __builtin_bit_cast(kv_i16x2_t, b)));
 }
-// over the lanes that differ in the bits from FROM up (a lane of 16: bits 2 and 3; 16 and 32)
-template <int FROM>
-__device__ __forceinline__ uint32_t max_rows(uint32_t v) {
-  if constexpr (FROM <= 4) v = max_i16x2(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xF, 0xF, true));
-  v = max_i16x2(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true));
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = max_i16x2(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return max_i16x2(b[0], b[1]);
-}
-template <int FROM>
-__device__ __forceinline__ uint32_t min_rows(uint32_t v) {
-  if constexpr (FROM <= 4) v = min_i16x2(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xF, 0xF, true));
-  v = min_i16x2(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true));
-  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-  v = min_i16x2(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return min_i16x2(b[0], b[1]);
-}
-
+// Lanes of a token's row (16 bytes each) stay with one (page, kv head) and go through its 16 tokens, so that a wave has 16 of
+// them (8 bits: 8) and nothing crosses lanes: 44 (40) instructions a page, where a wave a page with its reductions took ten
+// times as many.
 template <int BITS>
-__global__ __launch_bounds__(256) void page_bounds_kernel(const PageBoundsArgs a) {
+__global__ __launch_bounds__(64) void page_bounds_kernel(const PageBoundsArgs a) {
   constexpr int ROW = BITS == 8 ? kHeadDim : kHeadDim / 2;
-  constexpr int PER = ROW / 16;       // lanes of a token's row, 16 bytes each
-  constexpr int LOADS = BITS == 8 ? 2 : 1;
+  constexpr int PER = ROW / 16;             // lanes of a token's row
   constexpr int PARTS = BITS == 8 ? 2 : 4;  // codes of a 16-bit half
-  const int lane = threadIdx.x & 63;
-  const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= a.items) return;
-  const long long at = item / a.Hkv;
-  const int hk = (int)(item - at * a.Hkv);
-  const int b = (int)(at / a.pages_each), pg = (int)(at - (long long)b * a.pages_each);
+  const int lane = threadIdx.x;
+  const unsigned item = blockIdx.x * (64u / PER) + lane / PER;
+  if (item >= (unsigned)a.items) return;
+  const unsigned at = item / (unsigned)a.Hkv;
+  const int hk = (int)(item - at * (unsigned)a.Hkv);
+  const int b = (int)(at / (unsigned)a.pages_each), pg = (int)(at - (unsigned)b * (unsigned)a.pages_each);
   const int len = min(a.seq_lens[b], a.max_pages * kPage);
   int from = a.first ? max(a.first[b], 0) : 0;
+  if (from >= len) return;
   if (len - from > a.max_new) from = len - a.max_new;
   const int lp = from / kPage + pg, first = lp * kPage;
-  if (first >= len || from >= len) return;
+  if (first >= len) return;
   const int page = a.page_table[(size_t)b * a.max_pages + lp];
   if (page < 0 || page >= a.num_pages) return;
   const int live = min(len - first, kPage);
   const size_t block = (size_t)page * a.Hkv + hk;
   const uint8_t* src = a.k_cache + block * (kPage * ROW) + (lane % PER) * 16;
-  uint32_t hi[4 * PARTS], lo[4 * PARTS];
+  kv_u32x4_t raw[kPage];
 #pragma unroll
-  for (int j = 0; j < LOADS; j++) {
-    const int token = min(lane / PER + j * (64 / PER), live - 1);  // the last live one for those that are not there
-    const kv_u32x4_t raw = *reinterpret_cast<const kv_u32x4_t*>(src + token * ROW);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int p = 0; p < PARTS; p++) {
-        const uint32_t v = BITS == 8 ? (raw[i] << (8 - 8 * p)) & 0xFF00FF00u : (raw[i] << (12 - 4 * p)) & 0xF000F000u;
-        uint32_t &h = hi[i * PARTS + p], &l = lo[i * PARTS + p];
-        h = j ? max_i16x2(h, v) : v;
-        l = j ? min_i16x2(l, v) : v;
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < 4 * PARTS; i++) hi[i] = max_rows<PER>(hi[i]), lo[i] = min_rows<PER>(lo[i]);
-  if (lane >= 2 * PER) return;
-  kv_u32x4_t o;
+  for (int t = 0; t < kPage; t++)  // the last live token for those that are not there
+    raw[t] = *reinterpret_cast<const kv_u32x4_t*>(src + min(t, live - 1) * ROW);
+  kv_u32x4_t hi, lo;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    uint32_t w = 0;
+    uint32_t out_hi = 0, out_lo = 0;
 #pragma unroll
-    for (int p = 0; p < PARTS; p++) w |= (lane < PER ? hi : lo)[i * PARTS + p] >> (BITS == 8 ? 8 - 8 * p : 12 - 4 * p);
-    o[i] = w;
+    for (int p = 0; p < PARTS; p++) {
+      // code p of both halves moves to their tops; what is below it does not change the order of the tops
+      constexpr uint32_t TOP = BITS == 8 ? 0xFF00FF00u : 0xF000F000u;
+      const int up = BITS == 8 ? 8 - 8 * p : 12 - 4 * p;
+      uint32_t h = raw[0][i] << up, l = h;
+#pragma unroll
+      for (int t = 1; t < kPage; t++) {
+        const uint32_t v = raw[t][i] << up;
+        h = max_i16x2(h, v), l = min_i16x2(l, v);
+      }
+      out_hi |= (h & TOP) >> up, out_lo |= (l & TOP) >> up;
+    }
+    hi[i] = out_hi, lo[i] = out_lo;
   }
-  *reinterpret_cast<kv_u32x4_t*>(a.bounds + block * (2 * ROW) + lane * 16) = o;
+  uint8_t* to = a.bounds + block * (2 * ROW) + (lane % PER) * 16;
+  *reinterpret_cast<kv_u32x4_t*>(to) = hi;
+  *reinterpret_cast<kv_u32x4_t*>(to + ROW) = lo;
 }
 
 // ---- worth and choice of pages -----------------------------------------------------------------------------------------
@@ -160,125 +142,180 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 
 constexpr int kWorthWaves = 4;
+constexpr int kWorthRows = 4;  // consecutive rows of a workgroup; those of one sequence share what it reads
 
+// A page group's bounds (16 pages, the lane's is n) as MFMA operands, and its page's scale
 template <int BITS>
-__global__ __launch_bounds__(64 * kWorthWaves) void page_worth_kernel(const SelectArgs a, int per_wave) {
-  constexpr int ROW = BITS == 8 ? kHeadDim : kHeadDim / 2;
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.y, row = blockIdx.z;
-  int b;
-  const int len = row_tokens(a.row_seq, a.seq_lens, a.batch, a.max_pages, row, b);
-  const int pages = (len + kPage - 1) / kPage;
-  if (pages <= a.top) return;  // all of them are read
-  const int wave = blockIdx.x * kWorthWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int p0 = wave * per_wave * 16, p1 = min(p0 + per_wave * 16, pages);
-  if (p0 >= p1) return;
-  const int G = a.Hq / a.Hkv;
-  // the lane's channels of head min(n, G - 1), in the order that the bounds' fragments have: 8 bits, 16 g .. + 15 and
-  // 64 + 16 g .. + 15; 4 bits, the even and the odd ones of 32 g .. + 31
-  const uint16_t* qrow = a.q + row * a.ld_q + (size_t)(hk * G + min(n, G - 1)) * kHeadDim;
-  kv_u32x4_t raw[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    raw[i] = *reinterpret_cast<const kv_u32x4_t*>(qrow + (BITS == 8 ? 64 * (i / 2) + 16 * g + 8 * (i & 1) : 32 * g + 8 * i));
-  float x[32];
-  float most = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const uint32_t u = raw[i / 4][i & 3];
-    const half2_t h = __builtin_bit_cast(half2_t, u);
-    x[2 * i] = (float)h[0], x[2 * i + 1] = (float)h[1];
-  }
-#pragma unroll
-  for (int i = 0; i < 32; i++) {
-    const float m = fabsf(x[i]);
-    most = m < __builtin_inff() ? fmaxf(most, m) : most;
-  }
-  most = max_over_groups(most);
-  const float inv = most > 0.f ? 1.f / most : 0.f;
-  kv_i32x4_t plus[2], minus[2];
-#pragma unroll
-  for (int c = 0; c < 2; c++)
-#pragma unroll
-    for (int d = 0; d < 4; d++) {
-      uint32_t p = 0, m = 0;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float v = BITS == 8 ? x[16 * c + 4 * d + e] : x[2 * (4 * d + e) + c];
-        int w = whole(fminf(fmaxf(v, -most), most), most, inv);  // infinities as the largest
-        w = v == v ? w : 0;
-        p |= (uint32_t)max(w, 0) << (8 * e);
-        m |= (uint32_t)(min(w, 0) & 0xFF) << (8 * e);
-      }
-      plus[c][d] = (int)p, minus[c][d] = (int)m;
-    }
-  const int* ptab = a.page_table + (size_t)b * a.max_pages;
-  uint32_t* to = a.worth + ((size_t)row * a.Hkv + hk) * a.stride;
-  for (int p = p0; p < p1; p += 16) {
-    const int page = min(max(ptab[min(p + n, pages - 1)], 0), a.num_pages - 1);
-    const size_t block = (size_t)page * a.Hkv + hk;
+struct WorthRegs {
+  kv_i32x4_t k[BITS == 8 ? 4 : 2];
+  uint32_t ks;
+  __device__ __forceinline__ void load(const SelectArgs& a, int page, int hk, int g) {
+    constexpr int ROW = BITS == 8 ? kHeadDim : kHeadDim / 2;
+    const size_t block = (size_t)min(max(page, 0), a.num_pages - 1) * a.Hkv + hk;
     const uint8_t* src = a.bounds + block * (2 * ROW) + 16 * g;
-    const float ks = (float)__builtin_bit_cast(_Float16, a.k_scale[block]);
+    ks = a.k_scale[block];
+#pragma unroll
+    for (int c = 0; c < (BITS == 8 ? 4 : 2); c++) k[c] = *reinterpret_cast<const kv_i32x4_t*>(src + 64 * c);
+  }
+  // products with the rounded queries of 16 heads (columns); 4 bits: 16 times that
+  __device__ __forceinline__ kv_i32x4_t times(const kv_i32x4_t plus[2], const kv_i32x4_t minus[2]) const {
     kv_i32x4_t s = {0, 0, 0, 0};
     if constexpr (BITS == 8) {
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const kv_i32x4_t k = *reinterpret_cast<const kv_i32x4_t*>(src + 64 * c);
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, c < 2 ? plus[c & 1] : minus[c & 1], s, 0, 0, 0);
-      }
+      for (int c = 0; c < 4; c++)
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[c], c < 2 ? plus[c & 1] : minus[c & 1], s, 0, 0, 0);
     } else {
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        const kv_i32x4_t k = *reinterpret_cast<const kv_i32x4_t*>(src + 64 * c);
-        kv_i32x4_t even, odd;  // 16 times the codes
+        kv_i32x4_t even, odd;
 #pragma unroll
-        for (int i = 0; i < 4; i++) even[i] = (int)(((uint32_t)k[i] << 4) & 0xF0F0F0F0u), odd[i] = (int)((uint32_t)k[i] & 0xF0F0F0F0u);
+        for (int i = 0; i < 4; i++)
+          even[i] = (int)(((uint32_t)k[c][i] << 4) & 0xF0F0F0F0u), odd[i] = (int)((uint32_t)k[c][i] & 0xF0F0F0F0u);
         s = __builtin_amdgcn_mfma_i32_16x16x64_i8(even, c ? minus[0] : plus[0], s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_i32_16x16x64_i8(odd, c ? minus[1] : plus[1], s, 0, 0, 0);
       }
     }
-    // lane: pages 4 g .. + 3 of head n
-    uint32_t out[4];
+    return s;
+  }
+};
+
+// A column's head, rounded: the lane's channels in the order that the bounds' operands have them: 8 bits, 16 g .. + 15 and
+// 64 + 16 g .. + 15; 4 bits, the even and the odd ones of 32 g .. + 31
+template <int BITS>
+struct WorthQuery {
+  kv_i32x4_t plus[2], minus[2];
+  float most;
+  __device__ __forceinline__ void load(const uint16_t* head, int g) {
+    kv_u32x4_t raw[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float scale = most * __shfl(ks, 4 * g + i);  // exact
-      const float total = (float)(BITS == 8 ? s[i] : s[i] / 16);
-      uint32_t v = ordered(total * scale);
-      v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true));
-      v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xF, 0xF, true));
-      v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xF, 0xF, true));
-      v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xF, 0xF, true));
-      out[i] = v;
+    for (int i = 0; i < 4; i++)
+      raw[i] = *reinterpret_cast<const kv_u32x4_t*>(head + (BITS == 8 ? 64 * (i / 2) + 16 * g + 8 * (i & 1) : 32 * g + 8 * i));
+    float x[32];
+    most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const uint32_t u = raw[i / 4][i & 3];
+      const half2_t h = __builtin_bit_cast(half2_t, u);
+      x[2 * i] = (float)h[0], x[2 * i + 1] = (float)h[1];
     }
-    if (n == 0) *reinterpret_cast<kv_u32x4_t*>(to + p + 4 * g) = kv_u32x4_t{out[0], out[1], out[2], out[3]};
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const float m = fabsf(x[i]);
+      most = m < __builtin_inff() ? fmaxf(most, m) : most;
+    }
+    most = max_over_groups(most);
+    const float inv = most > 0.f ? 1.f / most : 0.f;
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+      for (int d = 0; d < 4; d++) {
+        uint32_t p = 0, m = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float v = BITS == 8 ? x[16 * c + 4 * d + e] : x[2 * (4 * d + e) + c];
+          int w = whole(fminf(fmaxf(v, -most), most), most, inv);  // infinities as the largest
+          w = v == v ? w : 0;
+          p |= (uint32_t)max(w, 0) << (8 * e);
+          m |= (uint32_t)(min(w, 0) & 0xFF) << (8 * e);
+        }
+        plus[c][d] = (int)p, minus[c][d] = (int)m;
+      }
+  }
+};
+
+// the largest of lanes n .. n + G - 1 of each row of 16 (0 past its end)
+__device__ __forceinline__ uint32_t max_of_next(uint32_t v, int G, int lane) {
+  int w = 1;
+  if (G >= 2) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x101, 0xF, 0xF, true)), w = 2;  // row_shl:1
+  if (G >= 4) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x102, 0xF, 0xF, true)), w = 4;
+  if (G >= 8) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x104, 0xF, 0xF, true)), w = 8;
+  if (G >= 16) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x108, 0xF, 0xF, true)), w = 16;
+  if (w < G) v = max(v, (uint32_t)__shfl((int)v, min(lane + G - w, lane | 15)));
+  return v;
+}
+
+template <int BITS, int ROWS>
+__global__ __launch_bounds__(64 * kWorthWaves) void page_worth_kernel(const SelectArgs a, int rows, int per_wave) {
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int hk = blockIdx.y, row0 = blockIdx.z * ROWS;
+  const int G = a.Hq / a.Hkv, fit = 16 / G;  // rows of an MFMA's columns
+  const int wave = blockIdx.x * kWorthWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int p0 = wave * per_wave * 16;
+  int seq[ROWS], pages[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; r++) {
+    seq[r] = -1, pages[r] = 0;
+    if (row0 + r < rows) {
+      pages[r] = (row_tokens(a.row_seq, a.seq_lens, a.batch, a.max_pages, row0 + r, seq[r]) + kPage - 1) / kPage;
+      if (pages[r] <= a.top) pages[r] = 0;  // all of them are read
+    }
+  }
+  // runs of rows that share a sequence
+  for (int first = 0, count; first < ROWS; first += count) {
+    count = 1;
+    int most = pages[0], b = seq[0];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++)
+      if (r == first) b = seq[r], most = pages[r];
+#pragma unroll
+    for (int r = 1; r < ROWS; r++)
+      if (r == first + count && seq[r] == b) count++, most = max(most, pages[r]);
+    const int p1 = min(p0 + per_wave * 16, most);
+    if (p0 >= p1) continue;
+    // columns: row j of the run, of those that fit, head by head; sets of them
+    WorthQuery<BITS> q[ROWS];
+    const int sets = (count + fit - 1) / fit, column = min(n / G, fit - 1), head = hk * G + min(n - column * G, G - 1);
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+      if (i < sets) q[i].load(a.q + (row0 + first + min(i * fit + column, count - 1)) * a.ld_q + (size_t)head * kHeadDim, g);
+    const int* ptab = a.page_table + (size_t)b * a.max_pages;
+    WorthRegs<BITS> next;
+    next.load(a, ptab[min(p0 + n, most - 1)], hk, g);
+    int page = ptab[min(p0 + 16 + n, most - 1)];
+    for (int p = p0; p < p1; p += 16) {
+      const WorthRegs<BITS> now = next;
+      next.load(a, page, hk, g);
+      page = ptab[min(p + 32 + n, most - 1)];
+      const float ks = (float)__builtin_bit_cast(_Float16, (uint16_t)now.ks);
+      float scale[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) scale[i] = __shfl(ks, 4 * g + i);  // of the lane's result pages
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) {
+        if (i >= sets) continue;
+        const kv_i32x4_t s = now.times(q[i].plus, q[i].minus);
+        kv_u32x4_t out;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float total = (float)(BITS == 8 ? s[j] : s[j] >> 4);
+          out[j] = max_of_next(ordered(total * (q[i].most * scale[j])), G, lane);  // the scales' product is exact
+        }
+        const int r = i * fit + column;
+        if (n == column * G && r < count) {
+          uint32_t* to = a.worth + ((size_t)(row0 + first + r) * a.Hkv + hk) * a.stride;
+          *reinterpret_cast<kv_u32x4_t*>(to + p + 4 * g) = out;
+        }
+      }
+    }
   }
 }
 
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kSelectBins = 1024;
+constexpr int kSelectList = 64;
 
-// the sums over the workgroup of `v` before this thread's (exclusive) and in all; part: LDS, one int a wave
-__device__ __forceinline__ int select_scan(int v, int& total, int* part) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int s = wave_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) part[wave] = s;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kSelectWaves; w++) {
-    before += w < wave ? part[w] : 0;
-    total += part[w];
-  }
-  return before + s - v;
-}
+struct SelectShared {
+  int hist[kSelectBins], part[2][kSelectWaves], found[2][3], listed;
+  uint32_t range[2][kSelectWaves];
+  unsigned long long list[kSelectList];  // worth << 32 | ~page
+};
 
+// EACH consecutive pages a thread, in registers; longer sequences by tiles, loaded anew for each pass
+template <int EACH>
 __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const SelectArgs a) {
-  __shared__ int hist[kSelectBins], part[kSelectWaves];
-  __shared__ uint32_t range[2 * kSelectWaves];
-  __shared__ int found[2];
+  constexpr int TILE = EACH * kSelectThreads;
+  __shared__ SelectShared sh;
   const int hk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int b;
@@ -290,57 +327,117 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const Selec
     return;
   }
   const uint32_t* worth = a.worth + ((size_t)row * a.Hkv + hk) * a.stride;
-  const int p0 = a.first, p1 = pages - a.last;  // the pages that are chosen among
-  int need = a.top - a.first - a.last;          // of them, 0 <= need < p1 - p0
-  uint32_t lo = 0xFFFFFFFFu, hi = 0;
-  for (int p = p0 + tid; p < p1; p += kSelectThreads) lo = min(lo, worth[p]), hi = max(hi, worth[p]);
-  hi = wave_max_u32(hi), lo = ~wave_max_u32(~lo);
-  if (lane == 0) range[wave] = lo, range[kSelectWaves + wave] = hi;
+  const int p0 = a.first, p1 = pages - a.last;  // the pages that are chosen among; 0 for the others
+  const int tiles = (pages + TILE - 1) / TILE;
+  uint32_t v[EACH];
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < EACH; i += 4) {
+      const int p = tile * TILE + tid * EACH + i;
+      kv_u32x4_t r = {0, 0, 0, 0};
+      if (p < pages) r = *reinterpret_cast<const kv_u32x4_t*>(worth + p);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[i + e] = p + e >= p0 && p + e < p1 ? r[e] : 0;
+    }
+  };
+  load(0);
+  int need = a.top - a.first - a.last;  // of them, 0 <= need < p1 - p0
+  uint32_t lo = ~0u, hi = 0;
+  for (int tile = 0; tile < tiles; tile++) {
+    if (tiles > 1) load(tile);
+#pragma unroll
+    for (int i = 0; i < EACH; i++) lo = v[i] ? min(lo, v[i]) : lo, hi = max(hi, v[i]);
+  }
+  hi = wave_max_u32(hi), lo = wave_max_u32(~lo);
+  if (lane == 0) sh.range[0][wave] = lo, sh.range[1][wave] = hi;
+  if (tid == 0) sh.listed = 0;
+  for (int i = tid; i < kSelectBins; i += kSelectThreads) sh.hist[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; w++) lo = min(lo, range[w]), hi = max(hi, range[kSelectWaves + w]);
-  // the need-th largest is in [lo, hi], `need` counts from hi; it is found once the range is a single value
-  while (need > 0 && lo < hi) {
+  for (int w = 0; w < kSelectWaves; w++) lo = max(lo, sh.range[0][w]), hi = max(hi, sh.range[1][w]);
+  lo = ~lo;
+  // The need-th largest is in [lo, hi], `need` counts from hi.  The range narrows to one of 1024 parts of it until few are in it.
+  int here = p1 - p0;
+  for (int turn = 0; need > 0 && here > kSelectList && lo < hi; turn ^= 1) {
     const uint32_t span = hi - lo;
     const int shift = max(0, 32 - __builtin_clz(span) - 10);  // span >> shift is below 1024
-    for (int i = tid; i < kSelectBins; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    for (int p = p0 + tid; p < p1; p += kSelectThreads) {
-      const uint32_t v = worth[p];
-      if (v >= lo && v <= hi) atomicAdd(&hist[(hi - v) >> shift], 1);
+    for (int tile = 0; tile < tiles; tile++) {
+      if (tiles > 1) load(tile);
+#pragma unroll
+      for (int i = 0; i < EACH; i++)
+        if (v[i] >= lo && v[i] <= hi) atomicAdd(&sh.hist[(hi - v[i]) >> shift], 1);
     }
     __syncthreads();
-    int here[2], total;
-#pragma unroll
-    for (int i = 0; i < 2; i++) here[i] = hist[2 * tid + i];
-    int before = select_scan(here[0] + here[1], total, part);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      if (before < need && before + here[i] >= need) found[0] = 2 * tid + i, found[1] = before;
-      before += here[i];
-    }
+    const int h0 = sh.hist[2 * tid], h1 = sh.hist[2 * tid + 1];
+    const int upto = wave_scan(h0 + h1);
+    if (lane == 63) sh.part[turn][wave] = upto;
     __syncthreads();
-    const uint32_t bin = found[0];
-    need -= found[1];
-    const uint32_t top = hi - (bin << shift), size = (1u << shift) - 1;
-    hi = top;
-    lo = top - lo > size ? top - size : lo;
+    int before = upto - h0 - h1;
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; w++) before += w < wave ? sh.part[turn][w] : 0;
+    if (before < need && before + h0 >= need) sh.found[turn][0] = 2 * tid, sh.found[turn][1] = before, sh.found[turn][2] = h0;
+    if (before + h0 < need && before + h0 + h1 >= need)
+      sh.found[turn][0] = 2 * tid + 1, sh.found[turn][1] = before + h0, sh.found[turn][2] = h1;
+    sh.hist[2 * tid] = sh.hist[2 * tid + 1] = 0;
+    __syncthreads();
+    need -= sh.found[turn][1], here = sh.found[turn][2];
+    hi -= (uint32_t)sh.found[turn][0] << shift;
+    const uint32_t size = (1u << shift) - 1;
+    lo = hi - lo > size ? hi - size : lo;
+  }
+  // Above hi: chosen.  In [lo, hi]: the first `need` by worth and page, by their ranks in a list of them; a single worth held by
+  // more pages than it takes: the first `need` by page.
+  const bool ranked = need > 0 && here <= kSelectList;
+  if (ranked) {
+    for (int tile = 0; tile < tiles; tile++) {
+      if (tiles > 1) load(tile);
+#pragma unroll
+      for (int i = 0; i < EACH; i++)
+        if (v[i] && v[i] >= lo && v[i] <= hi)
+          sh.list[atomicAdd(&sh.listed, 1)] = (unsigned long long)v[i] << 32 | (uint32_t)~(tile * TILE + tid * EACH + i);
+    }
     __syncthreads();
   }
-  // above hi: chosen; at hi: the first `need`; none where nothing is needed
-  const bool none = need == 0;
-  int chosen = a.first, equal = 0;
+  const int listed = ranked ? sh.listed : 0;
+  int chosen = a.first, ties = 0;
   for (int i = tid; i < a.first; i += kSelectThreads) out[i] = i;
-  for (int base = p0; base < p1; base += kSelectThreads) {
-    const int p = base + tid;
-    const uint32_t v = p < p1 ? worth[p] : 0;
-    const int ties = !none && p < p1 && v == hi;
-    int all_ties, taken;
-    const int tie = equal + select_scan(ties, all_ties, part);
-    const int take = !none && p < p1 && (v > hi || (ties && tie < need));
-    const int at = chosen + select_scan(take, taken, part);
-    if (take) out[at] = p;
-    equal += all_ties, chosen += taken;
+  for (int tile = 0; tile < tiles; tile++) {
+    if (tiles > 1) load(tile);
+    unsigned take = 0, tie = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      if (need <= 0 || v[i] == 0) continue;
+      bool in = v[i] > hi;
+      if (v[i] >= lo && v[i] <= hi) {
+        if (ranked) {
+          const unsigned long long mine = (unsigned long long)v[i] << 32 | (uint32_t)~(tile * TILE + tid * EACH + i);
+          int rank = 0;
+          for (int j = 0; j < listed; j++) rank += sh.list[j] > mine;
+          in = rank < need;
+        } else {
+          tie |= 1u << i;
+        }
+      }
+      take |= (unsigned)in << i;
+    }
+    // counts of both, packed (at most 8192 of a tile)
+    const int mine = __builtin_popcount(take) | __builtin_popcount(tie) << 16;
+    const int upto = wave_scan(mine);
+    __syncthreads();
+    if (lane == 63) sh.part[0][wave] = upto;
+    __syncthreads();
+    int before = upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; w++) before += w < wave ? sh.part[0][w] : 0, all += sh.part[0][w];
+    int to = chosen + (before & 0xFFFF) + min(need, ties + (before >> 16)) - min(need, ties), rank = ties + (before >> 16);
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const bool is_tie = tie >> i & 1;
+      if ((take >> i & 1) || (is_tie && rank < need)) out[to++] = tile * TILE + tid * EACH + i;
+      rank += is_tie;
+    }
+    chosen += (all & 0xFFFF) + min(need, ties + (all >> 16)) - min(need, ties);
+    ties += all >> 16;
   }
   for (int i = tid; i < a.last; i += kSelectThreads) out[a.top - a.last + i] = p1 + i;
 }
@@ -443,13 +540,32 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
   const int* list = a.pages + ((size_t)row * a.Hkv + hk) * a.top;
   const int* ptab = a.page_table + (size_t)(L > 0 ? b : 0) * a.max_pages;
   const int end = min((part + 1) * a.per, a.top), table_pages = (L + kPage - 1) / kPage;
-  for (int i = part * a.per + w; i < end; i += W) {
-    const int lp = list[i];
-    if (lp < 0 || lp >= table_pages) continue;  // not a page of the row's
-    const size_t bi = (size_t)min(max(ptab[lp], 0), a.num_pages - 1) * a.Hkv + hk;
-    KvRegs<BITS> r;
-    r.load(a.kc + bi * (kPage * ROW), a.vc + bi * (kPage * ROW), a.ksc, a.vsc, bi, n, g);
-    s.page(r, qf, qsum, lp * kPage, L, a.qk_scale, g);
+  // One page's codes are in flight while the one before is worked on, and the list's entry after it.  Entries that are no page
+  // of the row's load its first one and are left out.
+  if (L > 0 && part * a.per + w < end) {
+    KvRegs<BITS> r[2];
+    auto entry = [&](int i) { return list[min(i, end - 1)]; };
+    auto load = [&](KvRegs<BITS>& to, int lp) {
+      const size_t bi = (size_t)min(max(ptab[min(max(lp, 0), table_pages - 1)], 0), a.num_pages - 1) * a.Hkv + hk;
+      to.load(a.kc + bi * (kPage * ROW), a.vc + bi * (kPage * ROW), a.ksc, a.vsc, bi, n, g);
+    };
+    int i = part * a.per + w, lp = entry(i), after = entry(i + W);
+    load(r[0], lp);
+    bool more = true;
+    while (more) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        if (more) {
+          load(r[j ^ 1], after);
+          const int then = entry(i + 2 * W);
+          issue_fence();
+          if (lp >= 0 && lp < table_pages) s.page(r[j], qf, qsum, lp * kPage, L, a.qk_scale, g);
+          lp = after, after = then;
+          i += W;
+          more = i < end;
+        }
+      }
+    }
   }
 
   // join the waves; lane (n, g) holds dims 32 g + 8 i + db of query n
@@ -494,20 +610,32 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
   if (td == 0) a.part_ml[slot * 2] = mx, a.part_ml[slot * 2 + 1] = lsum;
 }
 
-// One wave per (row, head): lane holds dims 2 l, 2 l + 1; parts in order
+// One wave per (row, head): lane c holds part c's maximum and sum (64 parts at most), then dims 2 l, 2 l + 1; parts in order
+constexpr int kSparseParts = 64;
+
 __global__ __launch_bounds__(256) void sparse_merge_kernel(const SparseArgs a, int heads) {
   const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
   if (head >= heads) return;
-  const float* ml = a.part_ml + (size_t)head * a.parts * 2;
-  float mx = -INFINITY;
-  for (int c = 0; c < a.parts; c++) mx = fmaxf(mx, ml[2 * c]);
+  const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[(size_t)head * a.parts + min(l, a.parts - 1)];
+  const float m = l < a.parts ? ml.x : -INFINITY;
+  float mx = fmaxf(m, lane_xor<1>(m));
+  mx = fmaxf(mx, lane_xor<2>(mx));
+  mx = fmaxf(mx, lane_xor<4>(mx));
+  mx = fmaxf(mx, lane_xor<8>(mx));
+  mx = max_over_groups(mx);
+  const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+  const float share = f == 0.f ? 0.f : ml.y * f;
   float lsum = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int c = 0; c < a.parts; c++) {
-    if (ml[2 * c] == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(ml[2 * c] - mx);
-    const float2 o = *reinterpret_cast<const float2*>(a.part_o + ((size_t)head * a.parts + c) * kHeadDim + 2 * l);
-    lsum += ml[2 * c + 1] * f;
-    a0 += o.x * f, a1 += o.y * f;
+  const float* from = a.part_o + (size_t)head * a.parts * kHeadDim + 2 * l;
+  for (int c0 = 0; c0 < a.parts; c0 += 8) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {  // past the last part the weight is 0
+      const int c = c0 + i;
+      const float fc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), c));
+      lsum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, share), c));
+      const float2 o = *reinterpret_cast<const float2*>(from + (size_t)min(c, a.parts - 1) * kHeadDim);
+      a0 = __builtin_fmaf(o.x, fc, a0), a1 = __builtin_fmaf(o.y, fc, a1);
+    }
   }
   const bool empty = mx == -INFINITY;
   *reinterpret_cast<half2_t*>(a.out + (size_t)head * kHeadDim + 2 * l) =
@@ -520,7 +648,7 @@ struct SparsePlan {
 // Enough workgroups for two a CU, each with a page a wave at least
 static SparsePlan sparse_plan(int rows, int Hkv, int top) {
   const long long pairs = (long long)rows * Hkv;
-  const int most = (top + kSparseWaves - 1) / kSparseWaves;
+  const int most = std::min(kSparseParts, (top + kSparseWaves - 1) / kSparseWaves);
   const int parts = (int)std::max<long long>(1, std::min<long long>(most, (512 + pairs - 1) / pairs));
   const int per = ((top + parts - 1) / parts + kSparseWaves - 1) / kSparseWaves * kSparseWaves;
   return SparsePlan{per, (top + per - 1) / per};
@@ -566,11 +694,12 @@ extern "C" int exl3_kv_page_bounds(const void* k_cache, int num_pages, const int
   EXL3_CHECK_ARG(apart(all, 1), "exl3_kv_page_bounds: the bounds overlap another tensor of the call");
   const int pages_each = (int)std::min<long long>(max_pages, ((long long)max_new + 2 * (kPage - 1)) / kPage);
   const long long items = (long long)batch * pages_each * num_kv_heads;
-  EXL3_CHECK_ARG(items < (1LL << 26), "exl3_kv_page_bounds: %d sequences of up to %d tokens", batch, max_new);
+  EXL3_CHECK_ARG(items < (1LL << 28), "exl3_kv_page_bounds: %d sequences of up to %d tokens", batch, max_new);
   const PageBoundsArgs a{static_cast<const uint8_t*>(k_cache), num_pages, page_table, max_pages, seq_lens, first, max_new,
                          num_kv_heads, pages_each, items, static_cast<uint8_t*>(bounds)};
   auto kern = bits == 8 ? page_bounds_kernel<8> : page_bounds_kernel<4>;
-  kern<<<(unsigned)((items + 3) / 4), 256, 0, as_stream(stream)>>>(a);
+  const int each = bits == 8 ? 8 : 16;
+  kern<<<(unsigned)((items + each - 1) / each), 64, 0, as_stream(stream)>>>(a);
   EXL3_CHECK_LAUNCH();
   return EXL3_OK;
 }
@@ -612,16 +741,21 @@ extern "C" int exl3_kv_select_pages(const void* q, long long ld_q, const void* k
                      num_q_heads, num_kv_heads, top, first, last, (int)select_stride(max_pages),
                      static_cast<uint32_t*>(workspace), pages_out};
   if (max_pages > top) {
+    // rows of one sequence share its bounds where row_seq says that there can be any (at 4 rows a sequence of up to 128k tokens
+    // 59 us apart, TODO together)
+    const int each = row_seq ? kWorthRows : 1, blocks_z = (rows + each - 1) / each;
     const int groups = (max_pages + 15) / 16;
-    const long long pairs = (long long)rows * num_kv_heads;
+    const long long pairs = (long long)blocks_z * num_kv_heads;
     const int per_wave = (int)std::max<long long>(1, std::min<long long>(16, groups * pairs / 8192));
     const int waves = (groups + per_wave - 1) / per_wave;
-    auto kern = bits == 8 ? page_worth_kernel<8> : page_worth_kernel<4>;
-    kern<<<dim3((waves + kWorthWaves - 1) / kWorthWaves, num_kv_heads, rows), 64 * kWorthWaves, 0, as_stream(stream)>>>(
-        a, per_wave);
+    const dim3 grid((waves + kWorthWaves - 1) / kWorthWaves, num_kv_heads, blocks_z);
+    auto kern = bits == 8 ? (row_seq ? page_worth_kernel<8, kWorthRows> : page_worth_kernel<8, 1>)
+                          : (row_seq ? page_worth_kernel<4, kWorthRows> : page_worth_kernel<4, 1>);
+    kern<<<grid, 64 * kWorthWaves, 0, as_stream(stream)>>>(a, rows, per_wave);
     EXL3_CHECK_LAUNCH();
   }
-  page_select_kernel<<<dim3(num_kv_heads, rows), kSelectThreads, 0, as_stream(stream)>>>(a);
+  auto pick = max_pages <= 4 * kSelectThreads ? page_select_kernel<4> : page_select_kernel<16>;
+  pick<<<dim3(num_kv_heads, rows), kSelectThreads, 0, as_stream(stream)>>>(a);
   EXL3_CHECK_LAUNCH();
   return EXL3_OK;
 }
