@@ -6,8 +6,9 @@
 // with 1 + w for w where the weights are offsets.  fp32 throughout; h and y are each rounded once to their types, and y comes
 // from the h before its rounding.
 //
-// A workgroup holds a row in registers between its sums.  Bound by memory at many rows, 8 bytes a value in 16 bits; by the
-// chain load -> sum -> sum -> store at few.
+// A workgroup holds a row in registers between its sums.  Bound by memory at many rows, 8 bytes a value in 16 bits: 8192 rows of
+// 5120 (336 MB, both norms, bf16) take 65 us, 5.1 TB/s, what a large copy reaches; by the chain load -> sum -> sum -> store at
+// few (one row 3.4 us).
 #include <algorithm>
 
 #include "exl3_api.hpp"
@@ -221,72 +222,63 @@ __device__ __forceinline__ void an_put(const AddNormBuffer& to, int d, const flo
   if constexpr (TYPE == EXL3_F32) to.store(d * 4 + 16, r[1]);
 }
 
-// Rows of multiples of 8 values that lie at multiples of 16 bytes, up to 16 values a thread.  A workgroup takes rows blockIdx.x,
+// Rows of multiples of 8 values that lie at multiples of 16 bytes, 8 values a thread.  A workgroup takes rows blockIdx.x,
 // + gridDim.x, ..: the next row is loaded before this one is worked on; weights and a gate of one value a channel stay in
 // registers.  Loads and stores go through buffers, without a branch: the wait for a row's loads then leaves the stores behind them
-// out (with lane-conditional stores the compiler waits for everything: 112 us instead of TODO at 8192 rows of 5120).
-template <int R>
-constexpr int kAddNormThreads = R == 1 ? 1024 : 512;
-
-template <int R, int XT, int RT>
-__global__ __launch_bounds__(kAddNormThreads<R>) void add_norm_rows_kernel(const AddNormArgs a) {
+// out (with lane-conditional stores the compiler waits for everything: 112 us instead of 65 at 8192 rows of 5120).
+template <int XT, int RT>
+__global__ __launch_bounds__(1024) void add_norm_rows_kernel(const AddNormArgs a) {
   constexpr int WIDE = RT == EXL3_F32 ? 2 : 1;
   __shared__ float part[2][16];
   AddNormSum sum{part, (int)(blockDim.x >> 6), 0};
   const int x_bytes = a.dim * 2, r_bytes = a.dim * 2 * WIDE;
-  int d[R];
-  float w[R][8], p[R][8], g[R][8];  // weight, post_weight, gate a channel
+  const int d = threadIdx.x * 8, n = a.dim - d;
+  float w[8], p[8];  // weight; post_weight times a channel's gate
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    d[i] = (threadIdx.x + i * blockDim.x) * 8;
-    const int n = a.dim - d[i];
+  for (int e = 0; e < 8; e++) w[e] = 0.f, p[e] = 1.f;
+  if (n > 0) {
+    float g[8];
+    if (a.post_weight) {
+      an_load(a.post_weight, a.w_type, d, n, p);
 #pragma unroll
-    for (int e = 0; e < 8; e++) w[i][e] = 0.f, p[i][e] = g[i][e] = 1.f;
-    if (n <= 0) continue;
-    if (a.weight) an_load(a.weight, a.w_type, d[i], n, w[i]);
-    if (a.post_weight) an_load(a.post_weight, a.w_type, d[i], n, p[i]);
-    if (a.gate_kind == kGateChannel) an_load(a.gate, a.g_type, d[i], n, g[i]);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      w[i][e] += a.offset;
-      if (a.post_weight) p[i][e] += a.offset;
-      if (a.gate_kind == kGateChannel) g[i][e] = an_act(a, g[i][e]);
-      p[i][e] *= g[i][e];
+      for (int e = 0; e < 8; e++) p[e] += a.offset;
     }
+    if (a.gate_kind == kGateChannel) {
+      an_load(a.gate, a.g_type, d, n, g);
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] *= an_act(a, g[e]);
+    }
+    if (a.weight) an_load(a.weight, a.w_type, d, n, w);
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] += a.offset;
   }
   const bool full = a.gate_kind == kGateFull;  // (in 16 bits)
-  an_u32x4_t x[R], r[R][WIDE], f[R];
+  an_u32x4_t x, r[WIDE], f;
   auto load = [&](long long row) {
     const AddNormBuffer bx(a.x, row * a.ld_x * 2, x_bytes), br(a.residual, row * a.ld_r * 2 * WIDE, r_bytes),
         bf(full ? a.gate : nullptr, row * a.ld_g * 2, x_bytes);
+    x = bx.load(2 * d);
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-      x[i] = bx.load(2 * d[i]);
-#pragma unroll
-      for (int j = 0; j < WIDE; j++) r[i][j] = br.load(2 * WIDE * d[i] + 16 * j);
-      f[i] = bf.load(2 * d[i]);
-    }
+    for (int j = 0; j < WIDE; j++) r[j] = br.load(2 * WIDE * d + 16 * j);
+    f = bf.load(2 * d);
   };
   const float inv_dim = 1.0f / (float)a.dim;
   long long row = blockIdx.x;
   load(row);
   while (true) {
-    float u[R][8], h[R][8], ss = 0.f;
+    float u[8], h[8], ss = 0.f;
+    an_unpack(x, XT, u);
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-      an_unpack(x[i], XT, u[i]);
+    for (int e = 0; e < 8; e++) ss = __builtin_fmaf(u[e], u[e], ss);
 #pragma unroll
-      for (int e = 0; e < 8; e++) ss = __builtin_fmaf(u[i][e], u[i][e], ss);
+    for (int e = 0; e < 8; e++) u[e] *= p[e];
+    if (full) {
+      float q[8];
+      an_unpack(f, a.g_type, q);
 #pragma unroll
-      for (int e = 0; e < 8; e++) u[i][e] *= p[i][e];
-      if (full) {
-        float q[8];
-        an_unpack(f[i], a.g_type, q);
-#pragma unroll
-        for (int e = 0; e < 8; e++) u[i][e] *= an_act(a, q[e]);
-      }
-      an_unpack_row<RT>(r[i], h[i]);
+      for (int e = 0; e < 8; e++) u[e] *= an_act(a, q[e]);
     }
+    an_unpack_row<RT>(r, h);
     const long long after = row + gridDim.x;
     load(min(after, (long long)a.rows - 1));
     float token = a.scale;
@@ -295,21 +287,15 @@ __global__ __launch_bounds__(kAddNormThreads<R>) void add_norm_rows_kernel(const
     ss = 0.f;
     const AddNormBuffer bh(a.h, row * r_bytes, r_bytes), by(a.y, row * x_bytes, x_bytes);
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        h[i][e] = __builtin_fmaf(u[i][e], token, h[i][e]);
-        ss = __builtin_fmaf(h[i][e], h[i][e], ss);
-      }
-      an_put<RT>(bh, d[i], h[i]);
+    for (int e = 0; e < 8; e++) {
+      h[e] = __builtin_fmaf(u[e], token, h[e]);
+      ss = __builtin_fmaf(h[e], h[e], ss);
     }
+    an_put<RT>(bh, d, h);
     const float pre = 1.0f / __builtin_sqrtf(sum(ss) * inv_dim + a.eps);
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) h[i][e] *= pre * w[i][e];
-      an_put<XT>(by, d[i], h[i]);
-    }
+    for (int e = 0; e < 8; e++) h[e] *= pre * w[e];
+    an_put<XT>(by, d, h);
     if (after >= a.rows) break;
     row = after;
   }
@@ -317,8 +303,10 @@ __global__ __launch_bounds__(kAddNormThreads<R>) void add_norm_rows_kernel(const
 
 template <int XT, int RT>
 static void add_norm_launch(const AddNormArgs& a, bool even, int threads, int each, int grid, hipStream_t st) {
-  auto kern = even ? (each <= 1 ? add_norm_rows_kernel<1, XT, RT> : add_norm_rows_kernel<2, XT, RT>)
-                   : (each <= 1 ? add_norm_any_kernel<1, XT, RT> : each <= 4 ? add_norm_any_kernel<4, XT, RT> : add_norm_any_kernel<8, XT, RT>);
+  auto kern = even ? add_norm_rows_kernel<XT, RT>
+              : each <= 1 ? add_norm_any_kernel<1, XT, RT>
+              : each <= 4 ? add_norm_any_kernel<4, XT, RT>
+                          : add_norm_any_kernel<8, XT, RT>;
   kern<<<grid, threads, 0, st>>>(a);
 }
 
@@ -365,15 +353,11 @@ extern "C" int exl3_add_norm(const void* x, int x_type, long long ld_x, const vo
                     (gate_kind != kGateFull || (ld_g % 8 == 0 && g_type != EXL3_F32)) &&
                     (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y | (uintptr_t)h |
                       (gate_kind == kGateFull ? (uintptr_t)gate : 0)) & 15) == 0;
-  // Few rows: as many threads as there are values to load.  Many: 16 values a thread, and workgroups that stay for several rows
-  // (as many each), six waves a SIMD.
-  const bool many = rows > 1024;
-  int threads = (std::min(chunks, even ? 1024 : 512) + 63) / 64 * 64, grid = rows;
-  if (even && many) {
-    if (chunks > 64) threads = (chunks + 127) / 128 * 64;
-    const int fit = 256 * std::max(1, 1536 / threads), rounds = (rows + fit - 1) / fit;
-    grid = (rows + rounds - 1) / rounds;
-  }
+  const int threads = (std::min(chunks, even ? 1024 : 512) + 63) / 64 * 64;
+  // Even rows: workgroups that stay for as many rows each, six waves a SIMD (16 values a thread, half the threads, took 73 us
+  // at 8192 rows of 5120, for fewer waves by their registers; 8 take 65)
+  const int fit = 256 * std::max(1, 1536 / threads), rounds = even ? (rows + fit - 1) / fit : 1;
+  const int grid = (rows + rounds - 1) / rounds;
   const int each = (chunks + threads - 1) / threads;
   hipStream_t st = as_stream(stream);
   auto launch = x_type == EXL3_BF16 ? (r_type == EXL3_F32    ? add_norm_launch<EXL3_BF16, EXL3_F32>

@@ -13,8 +13,8 @@
 // In integers the choice does not depend on any order of summation.
 //
 // page_bounds_kernel: a wave per (page, kv head).  Min and max in packed 16-bit integers that hold a code in their high bits.
-// page_worth_kernel: a wave per 16 pages.  16 x 256 codes against the group's 16 columns (q8+ | q8-) are four MFMA 16x16x64
-//   i8; the largest over the columns by DPP.  Worths are written as integers that order like them.
+// page_worth_kernel: waves take 16 pages at a time.  16 heads (q8+ | q8-) against 16 x 256 codes are four MFMA 16x16x64 i8; query
+//   rows of one sequence share the codes.  Worths are written as integers that order like them.
 // page_select_kernel: a workgroup per (row, kv head) narrows the range of the T-th largest by histograms of 1024 equal parts
 //   of it, then writes the pages in ascending order by prefix sums (no atomic decides an order).
 // sparse_attention_kernel: (parts of the list, kv heads, rows) workgroups, waves take pages, one 16-token page is one MFMA
@@ -157,13 +157,13 @@ struct WorthRegs {
 #pragma unroll
     for (int c = 0; c < (BITS == 8 ? 4 : 2); c++) k[c] = *reinterpret_cast<const kv_i32x4_t*>(src + 64 * c);
   }
-  // products with the rounded queries of 16 heads (columns); 4 bits: 16 times that
+  // products with the rounded queries of 16 heads: lane (n, g) has those of heads 4 g .. + 3 with page n; 4 bits: 16 times that
   __device__ __forceinline__ kv_i32x4_t times(const kv_i32x4_t plus[2], const kv_i32x4_t minus[2]) const {
     kv_i32x4_t s = {0, 0, 0, 0};
     if constexpr (BITS == 8) {
 #pragma unroll
       for (int c = 0; c < 4; c++)
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[c], c < 2 ? plus[c & 1] : minus[c & 1], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(c < 2 ? plus[c & 1] : minus[c & 1], k[c], s, 0, 0, 0);
     } else {
 #pragma unroll
       for (int c = 0; c < 2; c++) {
@@ -171,76 +171,75 @@ struct WorthRegs {
 #pragma unroll
         for (int i = 0; i < 4; i++)
           even[i] = (int)(((uint32_t)k[c][i] << 4) & 0xF0F0F0F0u), odd[i] = (int)((uint32_t)k[c][i] & 0xF0F0F0F0u);
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(even, c ? minus[0] : plus[0], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(odd, c ? minus[1] : plus[1], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(c ? minus[0] : plus[0], even, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(c ? minus[1] : plus[1], odd, s, 0, 0, 0);
       }
     }
     return s;
   }
 };
 
-// A column's head, rounded: the lane's channels in the order that the bounds' operands have them: 8 bits, 16 g .. + 15 and
-// 64 + 16 g .. + 15; 4 bits, the even and the odd ones of 32 g .. + 31
+// A head, rounded: the lane's channels in the order that the bounds' operands have them: 8 bits, 16 g .. + 15 and
+// 64 + 16 g .. + 15; 4 bits, the even and the odd ones of 32 g .. + 31.  Every wave of a workgroup needs the same, so each rounds
+// a quarter and the others take it from LDS.
+struct WorthShared {
+  uint32_t plus[kWorthRows][8][64], minus[kWorthRows][8][64];
+};
 template <int BITS>
 struct WorthQuery {
   kv_i32x4_t plus[2], minus[2];
-  float most;
-  __device__ __forceinline__ void load(const uint16_t* head, int g) {
-    kv_u32x4_t raw[4];
+  __device__ __forceinline__ static void load(const uint16_t* head, int g, kv_u32x4_t raw[4]) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
       raw[i] = *reinterpret_cast<const kv_u32x4_t*>(head + (BITS == 8 ? 64 * (i / 2) + 16 * g + 8 * (i & 1) : 32 * g + 8 * i));
-    float x[32];
-    most = 0.f;
+  }
+  // returns max |q| of the head
+  __device__ __forceinline__ static float round(const kv_u32x4_t raw[4], int lane, int wave, uint32_t plus[8][64],
+                                                uint32_t minus[8][64]) {
+    uint32_t most_bits = 0;  // magnitudes of halves order as integers; infinities and NaN take no part
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const uint32_t u = raw[i / 4][i & 3];
-      const half2_t h = __builtin_bit_cast(half2_t, u);
-      x[2 * i] = (float)h[0], x[2 * i + 1] = (float)h[1];
+      const uint32_t lo = u & 0x7FFFu, hi = u >> 16 & 0x7FFFu;
+      most_bits = max(most_bits, max(lo < 0x7C00u ? lo : 0, hi < 0x7C00u ? hi : 0));
     }
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      const float m = fabsf(x[i]);
-      most = m < __builtin_inff() ? fmaxf(most, m) : most;
-    }
-    most = max_over_groups(most);
+    const float most = max_over_groups((float)__builtin_bit_cast(_Float16, (uint16_t)most_bits));
     const float inv = most > 0.f ? 1.f / most : 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; c++)
+    for (int i = 0; i < 8; i++) {
+      if (i / 2 != wave) continue;
+      const int c = i / 4, d = i & 3;  // dword d of operand c: channels 4 d .. + 3 of it
+      uint32_t p = 0, m = 0;
 #pragma unroll
-      for (int d = 0; d < 4; d++) {
-        uint32_t p = 0, m = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float v = BITS == 8 ? x[16 * c + 4 * d + e] : x[2 * (4 * d + e) + c];
-          int w = whole(fminf(fmaxf(v, -most), most), most, inv);  // infinities as the largest
-          w = v == v ? w : 0;
-          p |= (uint32_t)max(w, 0) << (8 * e);
-          m |= (uint32_t)(min(w, 0) & 0xFF) << (8 * e);
-        }
-        plus[c][d] = (int)p, minus[c][d] = (int)m;
+      for (int e = 0; e < 4; e++) {
+        const int at = BITS == 8 ? 16 * c + 4 * d + e : 2 * (4 * d + e) + c;  // of the lane's 32 halves
+        const uint32_t u = raw[at / 8][at / 2 & 3];
+        const half2_t h = __builtin_bit_cast(half2_t, u);
+        const float v = (float)h[at & 1];
+        int w = whole(fminf(fmaxf(v, -most), most), most, inv);  // infinities as the largest
+        w = v == v ? w : 0;
+        p |= (uint32_t)max(w, 0) << (8 * e);
+        m |= (uint32_t)(min(w, 0) & 0xFF) << (8 * e);
       }
+      plus[i][lane] = p, minus[i][lane] = m;
+    }
+    return most;
+  }
+  __device__ __forceinline__ void take(int lane, const uint32_t p[8][64], const uint32_t m[8][64]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) plus[i / 4][i & 3] = (int)p[i][lane], minus[i / 4][i & 3] = (int)m[i][lane];
   }
 };
 
-// the largest of lanes n .. n + G - 1 of each row of 16 (0 past its end)
-__device__ __forceinline__ uint32_t max_of_next(uint32_t v, int G, int lane) {
-  int w = 1;
-  if (G >= 2) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x101, 0xF, 0xF, true)), w = 2;  // row_shl:1
-  if (G >= 4) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x102, 0xF, 0xF, true)), w = 4;
-  if (G >= 8) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x104, 0xF, 0xF, true)), w = 8;
-  if (G >= 16) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x108, 0xF, 0xF, true)), w = 16;
-  if (w < G) v = max(v, (uint32_t)__shfl((int)v, min(lane + G - w, lane | 15)));
-  return v;
-}
-
+// The MFMA's 16 head rows hold 4, 2 or 1 query rows of up to 4, 8 or 16 heads (the last one repeated), so that a query row's
+// maximum is one over a lane's own four values and at most two exchanges between lanes of one page.
 template <int BITS, int ROWS>
 __global__ __launch_bounds__(64 * kWorthWaves) void page_worth_kernel(const SelectArgs a, int rows, int per_wave) {
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.y, row0 = blockIdx.z * ROWS;
-  const int G = a.Hq / a.Hkv, fit = 16 / G;  // rows of an MFMA's columns
-  const int wave = blockIdx.x * kWorthWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int p0 = wave * per_wave * 16;
+  __shared__ WorthShared sh;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = blockIdx.x, row0 = blockIdx.z * ROWS;  // kv heads first: a page's bounds lie side by side
+  const int G = a.Hq / a.Hkv, wide = G <= 4 ? 4 : G <= 8 ? 8 : 16, fit = 16 / wide;
+  const int start = blockIdx.y * kWorthWaves * per_wave * 16, p0 = start + w * per_wave * 16;
   int seq[ROWS], pages[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; r++) {
@@ -260,41 +259,62 @@ __global__ __launch_bounds__(64 * kWorthWaves) void page_worth_kernel(const Sele
 #pragma unroll
     for (int r = 1; r < ROWS; r++)
       if (r == first + count && seq[r] == b) count++, most = max(most, pages[r]);
-    const int p1 = min(p0 + per_wave * 16, most);
-    if (p0 >= p1) continue;
-    // columns: row j of the run, of those that fit, head by head; sets of them
+    // sets of `fit` rows of the run
     WorthQuery<BITS> q[ROWS];
-    const int sets = (count + fit - 1) / fit, column = min(n / G, fit - 1), head = hk * G + min(n - column * G, G - 1);
+    float a4[ROWS][4];  // max |q| of the lane's result heads
+    const int sets = (count + fit - 1) / fit, head = hk * G + min(n % wide, G - 1);
+    // (asked for before the rows' lengths are known: entries past a length are not used)
+    const int* ptab = a.page_table + (size_t)min(max(b, 0), a.batch - 1) * a.max_pages;
+    int page = ptab[min(p0 + n, a.max_pages - 1)], then = ptab[min(p0 + 16 + n, a.max_pages - 1)];
+    kv_u32x4_t raw[4];
+    auto ask = [&](int i) {
+      WorthQuery<BITS>::load(a.q + min(row0 + first + min(i * fit + n / wide, count - 1), rows - 1) * a.ld_q +
+                                 (size_t)head * kHeadDim, g, raw);
+    };
+    ask(0);
+    if (start >= most) continue;  // (the whole workgroup)
+    if (first > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+      if (i >= sets) continue;
+      if (i > 0) ask(i);
+      const float largest = WorthQuery<BITS>::round(raw, lane, w, sh.plus[i], sh.minus[i]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) a4[i][j] = __shfl(largest, 4 * g + j);
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < ROWS; i++)
-      if (i < sets) q[i].load(a.q + (row0 + first + min(i * fit + column, count - 1)) * a.ld_q + (size_t)head * kHeadDim, g);
-    const int* ptab = a.page_table + (size_t)b * a.max_pages;
+      if (i < sets) q[i].take(lane, sh.plus[i], sh.minus[i]);
+    const int p1 = min(p0 + per_wave * 16, most);
+    if (p0 >= p1) continue;
     WorthRegs<BITS> next;
-    next.load(a, ptab[min(p0 + n, most - 1)], hk, g);
-    int page = ptab[min(p0 + 16 + n, most - 1)];
+    next.load(a, page, hk, g);
     for (int p = p0; p < p1; p += 16) {
       const WorthRegs<BITS> now = next;
-      next.load(a, page, hk, g);
-      page = ptab[min(p + 32 + n, most - 1)];
+      next.load(a, then, hk, g);
+      then = ptab[min(p + 32 + n, most - 1)];
       const float ks = (float)__builtin_bit_cast(_Float16, (uint16_t)now.ks);
-      float scale[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) scale[i] = __shfl(ks, 4 * g + i);  // of the lane's result pages
 #pragma unroll
       for (int i = 0; i < ROWS; i++) {
         if (i >= sets) continue;
         const kv_i32x4_t s = now.times(q[i].plus, q[i].minus);
-        kv_u32x4_t out;
+        float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float total = (float)(BITS == 8 ? s[j] : s[j] >> 4);
-          out[j] = max_of_next(ordered(total * (q[i].most * scale[j])), G, lane);  // the scales' product is exact
+        for (int j = 0; j < 4; j++) v[j] = (float)(BITS == 8 ? s[j] : s[j] >> 4) * (a4[i][j] * ks);  // a4 ks is exact
+        // (fmaxf passes a NaN by)
+        float worth = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        if (wide >= 8) {
+          const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(worth), __float_as_uint(worth), false, false);
+          worth = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
         }
-        const int r = i * fit + column;
-        if (n == column * G && r < count) {
-          uint32_t* to = a.worth + ((size_t)(row0 + first + r) * a.Hkv + hk) * a.stride;
-          *reinterpret_cast<kv_u32x4_t*>(to + p + 4 * g) = out;
+        if (wide == 16) {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(worth), __float_as_uint(worth), false, false);
+          worth = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
         }
+        const int r = i * fit + 4 * g / wide;
+        if (4 * g % wide == 0 && r < count)
+          a.worth[((size_t)(row0 + first + r) * a.Hkv + hk) * a.stride + p + n] = ordered(worth);
       }
     }
   }
@@ -318,6 +338,14 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const Selec
   __shared__ SelectShared sh;
   const int hk = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t* worth = a.worth + ((size_t)row * a.Hkv + hk) * a.stride;
+  kv_u32x4_t raw[EACH / 4];  // (asked for before the row's length is known)
+  auto ask = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < EACH / 4; i++)
+      raw[i] = *reinterpret_cast<const kv_u32x4_t*>(worth + min(tile * TILE + tid * EACH + 4 * i, a.stride - 4));
+  };
+  ask(0);
   int b;
   const int len = row_tokens(a.row_seq, a.seq_lens, a.batch, a.max_pages, row, b);
   const int pages = (len + kPage - 1) / kPage;
@@ -326,21 +354,18 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const Selec
     for (int i = tid; i < a.top; i += kSelectThreads) out[i] = i < pages ? i : -1;
     return;
   }
-  const uint32_t* worth = a.worth + ((size_t)row * a.Hkv + hk) * a.stride;
   const int p0 = a.first, p1 = pages - a.last;  // the pages that are chosen among; 0 for the others
   const int tiles = (pages + TILE - 1) / TILE;
   uint32_t v[EACH];
-  auto load = [&](int tile) {
+  auto keep = [&](int tile) {
 #pragma unroll
-    for (int i = 0; i < EACH; i += 4) {
+    for (int i = 0; i < EACH; i++) {
       const int p = tile * TILE + tid * EACH + i;
-      kv_u32x4_t r = {0, 0, 0, 0};
-      if (p < pages) r = *reinterpret_cast<const kv_u32x4_t*>(worth + p);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[i + e] = p + e >= p0 && p + e < p1 ? r[e] : 0;
+      v[i] = p >= p0 && p < p1 ? raw[i / 4][i & 3] : 0;
     }
   };
-  load(0);
+  auto load = [&](int tile) { ask(tile), keep(tile); };
+  keep(0);
   int need = a.top - a.first - a.last;  // of them, 0 <= need < p1 - p0
   uint32_t lo = ~0u, hi = 0;
   for (int tile = 0; tile < tiles; tile++) {
@@ -514,6 +539,11 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
   extern __shared__ float red[];  // [W][G][D + 1], then [W][G][2]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   const int part = blockIdx.x, hk = blockIdx.y, row = blockIdx.z, G = a.Hq / a.Hkv;
+  // (the list is asked for before the row's length is known)
+  const int* list = a.pages + ((size_t)row * a.Hkv + hk) * a.top;
+  const int end = min((part + 1) * a.per, a.top);
+  auto entry = [&](int i) { return list[min(i, end - 1)]; };
+  int i = part * a.per + w, lp = entry(i), after = entry(i + W);
   int b;
   const int L = row_tokens(a.row_seq, a.seq_lens, a.batch, a.max_pages, row, b);
 
@@ -537,19 +567,16 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
 #pragma unroll
   for (int db = 0; db < 8; db++) s.o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-  const int* list = a.pages + ((size_t)row * a.Hkv + hk) * a.top;
   const int* ptab = a.page_table + (size_t)(L > 0 ? b : 0) * a.max_pages;
-  const int end = min((part + 1) * a.per, a.top), table_pages = (L + kPage - 1) / kPage;
+  const int table_pages = (L + kPage - 1) / kPage;
   // One page's codes are in flight while the one before is worked on, and the list's entry after it.  Entries that are no page
   // of the row's load its first one and are left out.
-  if (L > 0 && part * a.per + w < end) {
+  if (L > 0 && i < end) {
     KvRegs<BITS> r[2];
-    auto entry = [&](int i) { return list[min(i, end - 1)]; };
     auto load = [&](KvRegs<BITS>& to, int lp) {
       const size_t bi = (size_t)min(max(ptab[min(max(lp, 0), table_pages - 1)], 0), a.num_pages - 1) * a.Hkv + hk;
       to.load(a.kc + bi * (kPage * ROW), a.vc + bi * (kPage * ROW), a.ksc, a.vsc, bi, n, g);
     };
-    int i = part * a.per + w, lp = entry(i), after = entry(i + W);
     load(r[0], lp);
     bool more = true;
     while (more) {
@@ -645,11 +672,12 @@ __global__ __launch_bounds__(256) void sparse_merge_kernel(const SparseArgs a, i
 struct SparsePlan {
   int per, parts;
 };
-// Enough workgroups for two a CU, each with a page a wave at least
+// Enough workgroups for four a CU, each with a page a wave at least (16 sequences of 128 pages, 8 bits, 8 kv heads: two a CU 19 us,
+// four 17, eight 19; 32 rows of 256 pages, 4 bits: 43, 32, 34)
 static SparsePlan sparse_plan(int rows, int Hkv, int top) {
   const long long pairs = (long long)rows * Hkv;
   const int most = std::min(kSparseParts, (top + kSparseWaves - 1) / kSparseWaves);
-  const int parts = (int)std::max<long long>(1, std::min<long long>(most, (512 + pairs - 1) / pairs));
+  const int parts = (int)std::max<long long>(1, std::min<long long>(most, (1024 + pairs - 1) / pairs));
   const int per = ((top + parts - 1) / parts + kSparseWaves - 1) / kSparseWaves * kSparseWaves;
   return SparsePlan{per, (top + per - 1) / per};
 }
@@ -724,7 +752,8 @@ extern "C" int exl3_kv_select_pages(const void* q, long long ld_q, const void* k
   EXL3_CHECK_ARG(k_scale && bounds && ((uintptr_t)bounds & 15) == 0,
                  "exl3_kv_select_pages: the bounds or the scales are null, or the bounds not 16-byte aligned");
   if (rows == 0) return EXL3_OK;
-  EXL3_CHECK_ARG(q && seq_lens && pages_out && (page_table || batch == 0), "exl3_kv_select_pages: null pointer");
+  EXL3_CHECK_ARG(batch >= 1, "exl3_kv_select_pages: %d rows of no sequence", rows);
+  EXL3_CHECK_ARG(q && seq_lens && pages_out && page_table, "exl3_kv_select_pages: null pointer");
   EXL3_CHECK_ARG(ld_q >= (long long)num_q_heads * head_dim && ld_q % 8 == 0 && ((uintptr_t)q & 15) == 0,
                  "exl3_kv_select_pages: row stride %lld (a multiple of 8, a row's heads at least; 16-byte aligned)", ld_q);
   const size_t need = exl3_kv_select_workspace_bytes(rows, num_kv_heads, max_pages);
@@ -741,14 +770,14 @@ extern "C" int exl3_kv_select_pages(const void* q, long long ld_q, const void* k
                      num_q_heads, num_kv_heads, top, first, last, (int)select_stride(max_pages),
                      static_cast<uint32_t*>(workspace), pages_out};
   if (max_pages > top) {
-    // rows of one sequence share its bounds where row_seq says that there can be any (at 4 rows a sequence of up to 128k tokens
-    // 59 us apart, TODO together)
+    // rows of one sequence share its bounds where row_seq says that there can be any (4 rows each of 8 sequences of up to 128k
+    // tokens, 4 bits: 59 us apart, 20 together)
     const int each = row_seq ? kWorthRows : 1, blocks_z = (rows + each - 1) / each;
     const int groups = (max_pages + 15) / 16;
     const long long pairs = (long long)blocks_z * num_kv_heads;
-    const int per_wave = (int)std::max<long long>(1, std::min<long long>(16, groups * pairs / 8192));
+    const int per_wave = (int)std::max<long long>(1, std::min<long long>(16, groups * pairs / 4096));
     const int waves = (groups + per_wave - 1) / per_wave;
-    const dim3 grid((waves + kWorthWaves - 1) / kWorthWaves, num_kv_heads, blocks_z);
+    const dim3 grid(num_kv_heads, (waves + kWorthWaves - 1) / kWorthWaves, blocks_z);
     auto kern = bits == 8 ? (row_seq ? page_worth_kernel<8, kWorthRows> : page_worth_kernel<8, 1>)
                           : (row_seq ? page_worth_kernel<4, kWorthRows> : page_worth_kernel<4, 1>);
     kern<<<grid, 64 * kWorthWaves, 0, as_stream(stream)>>>(a, rows, per_wave);
@@ -778,7 +807,8 @@ extern "C" int exl3_kv_sparse_attention(const void* q, long long ld_q, const voi
   EXL3_CHECK_ARG(k_cache && v_cache && k_scale && v_scale && (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0,
                  "exl3_kv_sparse_attention: a cache is null or not 16-byte aligned");
   if (rows == 0) return EXL3_OK;
-  EXL3_CHECK_ARG(q && seq_lens && pages && out && (page_table || batch == 0), "exl3_kv_sparse_attention: null pointer");
+  EXL3_CHECK_ARG(batch >= 1, "exl3_kv_sparse_attention: %d rows of no sequence", rows);
+  EXL3_CHECK_ARG(q && seq_lens && pages && out && page_table, "exl3_kv_sparse_attention: null pointer");
   EXL3_CHECK_ARG(ld_q >= (long long)num_q_heads * head_dim && ld_q % 8 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0,
                  "exl3_kv_sparse_attention: row stride %lld (a multiple of 8, a row's heads at least; 16-byte aligned)", ld_q);
   const size_t need = exl3_kv_sparse_workspace_bytes(rows, num_q_heads, num_kv_heads, top);
