@@ -39,16 +39,16 @@ typedef unsigned long long u64_t;
 typedef uint32_t sample_u32x4_t __attribute__((ext_vector_type(4), aligned(2)));  // rows start at any element
 
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kEach = 8;                          // elements of a chunk's thread
-constexpr int kLargeChunk = 8192;                 // 1024 threads
-constexpr int kSmallChunk = 4096;                 // 512
+constexpr int kChunkThreads = 512;
+constexpr int kLargeChunk = 16 * kChunkThreads;
+constexpr int kSmallChunk = 8 * kChunkThreads;
 constexpr int kMaxChunks = kMaxVocab / kSmallChunk;
 constexpr int kBins = 256;
 constexpr int kBorderThreads = 256;               // a bin each, and a chunk each
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kCrossBins = 1024;
-constexpr int kList = 4096;
+constexpr int kList = 3072;
 constexpr int kSliceRows = 1024;                  // rows of a workspace
 constexpr double kBinUnit = 0x1p-50;              // a bin's sum is in 2^-50 of the chunk's largest weight
 constexpr double kBinBase = 0x1p52 * kBinUnit;
@@ -64,7 +64,8 @@ struct SampleBorder {
   double sum;                 // of all weights
   double before_k, before_p;  // of those in the bins before k_bin, p_first
   double inv;                 // 1 / the sum of the kept weights (sample_row_kernel); 0: no logit above -inf
-  float m, top;               // the largest logit, its place
+  double scale, min_w;        // of SampleRules: scale, m
+  float m, top, bin_scale;    // the largest logit, its place; of SampleRules
   int first, last;            // the bins with elements that may be kept or not; before them all are, behind them none; first
                               // kBins: no rule
   int k_bin, k_left;          // the bin of the k-th element (-1: it does not matter), its rank there
@@ -87,6 +88,7 @@ struct SampleArgs {
   int chunks;
   SampleBorder* border;  // [rows]
   SampleChunk* chunk;    // [rows][chunks]
+  double* factor;        // [rows][chunks]: the weight of the chunk's largest logit
   u64_t* chunk_mass;     // [rows][chunks]: what lies before the border bins, in the row's units
   u64_t* bin_mass;       // [rows][chunks][kBins]
   int* bin_count;        // [rows][chunks][kBins], where there is a top-k
@@ -175,7 +177,7 @@ struct SampleRow {
       f = __builtin_bit_cast(float, bits << 16);
     else
       f = (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
-    return f == f ? f : -INFINITY;
+    return fmaxf(f, -INFINITY);  // NaN: -inf
   }
   __device__ __forceinline__ float at(int i) const { return value(row[i]); }
   // elements i .. i + VEC - 1, -inf past the row; `whole` (uniform): none is
@@ -190,14 +192,15 @@ struct SampleRow {
       for (int e = 0; e < VEC; e++) v[e] = i + e < vocab ? at(i + e) : -INFINITY;
     }
   }
-  // a thread's kEach elements of a chunk: VEC j 's at first + j * step
-  __device__ __forceinline__ void get_each(int first, int step, bool whole, float v[kEach]) const {
+  // a thread's EACH elements of a chunk: VEC j 's at first + j * step
+  template <int EACH>
+  __device__ __forceinline__ void get_each(int first, int step, bool whole, float v[EACH]) const {
     if (whole) {
 #pragma unroll
-      for (int j = 0; j < kEach / VEC; j++) get(first + j * step, true, v + j * VEC);
+      for (int j = 0; j < EACH / VEC; j++) get(first + j * step, true, v + j * VEC);
     } else {
 #pragma unroll
-      for (int j = 0; j < kEach / VEC; j++) get(first + j * step, false, v + j * VEC);
+      for (int j = 0; j < EACH / VEC; j++) get(first + j * step, false, v + j * VEC);
     }
   }
   // whole numbers that order like the logits, both zeros the same
@@ -256,9 +259,9 @@ __device__ __forceinline__ float wave_max_f32(float v) {  // of values that are 
 
 // ---- the chunks --------------------------------------------------------------------------------------------------------
 
-template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_chunk_kernel(const SampleArgs a) {
-  constexpr int VEC = SampleRow<TYPE>::VEC, WAVES = THREADS / 64, CHUNK = THREADS * kEach;
+template <int TYPE, int EACH>
+__global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const SampleArgs a) {
+  constexpr int VEC = SampleRow<TYPE>::VEC, THREADS = kChunkThreads, WAVES = THREADS / 64, CHUNK = THREADS * EACH;
   __shared__ u64_t mass[kBins];
   __shared__ int count[kBins], firsts[kBins];
   __shared__ float part[WAVES];
@@ -268,16 +271,17 @@ __global__ __launch_bounds__(THREADS) void sample_chunk_kernel(const SampleArgs 
   const SampleRow<TYPE> x = sample_row<TYPE>(a, row);
   const int first = c * CHUNK;
   const bool whole = first + CHUNK <= a.vocab;
-  float l[kEach];
-  x.get_each(first + tid * VEC, THREADS * VEC, whole, l);
+  float l[EACH];
+  x.template get_each<EACH>(first + tid * VEC, THREADS * VEC, whole, l);
   const SampleRules rules = sample_rules(a, row);
   const bool bins = rules.by_k || rules.by_p || rules.by_m;
-  // behind a chunk's k-th largest element, for k up to 512: bins of its threads' largest elements tell (others are more)
-  const bool by_firsts = rules.by_k && rules.k <= 512;
+  // behind a chunk's k-th largest element, for k up to half its threads: bins of its threads' largest elements tell (others are more)
+  const bool by_firsts = rules.by_k && rules.k <= THREADS / 2;
+  static_assert(THREADS >= kBins);
   if (bins && tid < kBins) mass[tid] = 0, count[tid] = 0, firsts[tid] = 0;
   float mine = l[0];
 #pragma unroll
-  for (int i = 1; i < kEach; i++) mine = fmaxf(mine, l[i]);
+  for (int i = 1; i < EACH; i++) mine = fmaxf(mine, l[i]);
   float m = wave_max_f32(mine);
   if (lane == 0) part[wave] = m;
   __syncthreads();
@@ -286,13 +290,23 @@ __global__ __launch_bounds__(THREADS) void sample_chunk_kernel(const SampleArgs 
   const size_t at = (size_t)row * a.chunks + c;
   const float top = sample_place(m, rules.bin_scale);
   const bool any = m > -INFINITY;
-  double w[kEach], sum = 0.0;
+  double w[EACH], sum = 0.0;
+  if (any && m < INFINITY && whole) {
+    const double m64 = (double)m;
 #pragma unroll
-  for (int i = 0; i < kEach; i++) {
-    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-    const bool in = any && (whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab);
-    w[i] = in ? sample_weight(l[i], m, rules.scale) : 0.0;
-    sum += w[i];
+    for (int i = 0; i < EACH; i++) {
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // a few chains at a time: all of them do not fit the registers
+      w[i] = exp2_f64(((double)l[i] - m64) * rules.scale);
+      sum += w[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+      const bool in = any && (whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab);
+      w[i] = in ? sample_weight(l[i], m, rules.scale) : 0.0;
+      sum += w[i];
+    }
   }
   sum = wave_scan_double(sum);
   if (lane == 63) sums[wave] = sum;
@@ -336,7 +350,7 @@ __global__ __launch_bounds__(THREADS) void sample_chunk_kernel(const SampleArgs 
   }
   if (any) {
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
+    for (int i = 0; i < EACH; i++) {
       const int bin = sample_bin(l[i], rules.bin_scale, top);
       const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
       if (in && bin <= deep) {
@@ -371,13 +385,13 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(const Sam
 #pragma unroll
   for (int w = 1; w < WAVES; w++) M = fmaxf(M, part[0][w]), top = fmaxf(top, part[1][w]);
   SampleBorder b{};
-  b.m = M, b.top = top, b.first = kBins, b.last = kBins - 1, b.k_bin = -1, b.p_last = -1, b.cut_at = a.vocab - 1;
+  b.m = M, b.top = top, b.scale = rules.scale, b.min_w = rules.m, b.bin_scale = rules.bin_scale, b.first = kBins, b.last = kBins - 1, b.k_bin = -1, b.p_last = -1, b.cut_at = a.vocab - 1;
   if (!(M > -INFINITY)) {  // nothing to draw from
     if (tid == 0) a.border[row] = b;
     return;
   }
   const double f = chunk.m > -INFINITY ? sample_weight(chunk.m, M, rules.scale) : 0.0;
-  if (tid < C) factor[tid] = f * kBinUnit, shift[tid] = (int)fminf(top - chunk.top, (float)kBins);
+  if (tid < C) a.factor[(size_t)row * C + tid] = f, factor[tid] = f * kBinUnit, shift[tid] = (int)fminf(top - chunk.top, (float)kBins);
   const double s = wave_scan_double(f * chunk.sum);
   if (lane == 63) sums[wave] = s;
   __syncthreads();
@@ -388,14 +402,22 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(const Sam
     // the bins of all chunks; the last one is what is not in the others
     double mass = 0.0;
     int count = 0;
-    if (tid < kBins - 1) {
-#pragma unroll 4
-      for (int c = 0; c < C; c++) {
-        const int bin = tid - shift[c];
-        if (bin < 0) continue;
-        const size_t at = ((size_t)row * C + c) * kBins + bin;
-        mass += factor[c] * (double)a.bin_mass[at];
-        if (rules.by_k) count += a.bin_count[at];
+    const u64_t* masses_of = a.bin_mass + (size_t)row * C * kBins;
+    const int* counts_of = a.bin_count + (size_t)row * C * kBins;
+    for (int c0 = 0; c0 < C; c0 += 8) {
+      u64_t m8[8];
+      int n8[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {  // all loads first
+        const int c = min(c0 + i, C - 1), at = c * kBins + max(tid - shift[c], 0);
+        m8[i] = masses_of[at];
+        n8[i] = rules.by_k ? counts_of[at] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const bool in = c0 + i < C && tid < kBins - 1 && tid >= shift[min(c0 + i, C - 1)];
+        mass += in ? factor[min(c0 + i, C - 1)] * (double)m8[i] : 0.0;
+        count += in ? n8[i] : 0;
       }
     }
     double mass_to = wave_scan_double(mass);
@@ -453,44 +475,38 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(const Sam
 
 // ---- their elements ----------------------------------------------------------------------------------------------------
 
-template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_list_kernel(const SampleArgs a) {
+template <int TYPE, int EACH>
+__global__ __launch_bounds__(kChunkThreads) void sample_list_kernel(const SampleArgs a) {
   using Row = SampleRow<TYPE>;
-  constexpr int VEC = Row::VEC, WAVES = THREADS / 64, CHUNK = THREADS * kEach;
+  constexpr int VEC = Row::VEC, THREADS = kChunkThreads, WAVES = THREADS / 64, CHUNK = THREADS * EACH;
   __shared__ int part[WAVES], base;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
   SampleBorder* border = a.border + row;
   const int g_first = border->first, g_last = border->last, k_bin = border->k_bin;
-  const float M = border->m, top = border->top;
-  if (!(M > -INFINITY)) return;
-  const SampleRules rules = sample_rules(a, row);
+  if (g_first == kBins) return;  // no rule, or nothing to draw from
+  const float top = border->top, bin_scale = border->bin_scale;
   const size_t at = (size_t)row * a.chunks + c;
-  const SampleChunk chunk = a.chunk[at];
-  const float ahead = top - chunk.top;  // bins
-  if (wave == 0) {
-    // its weights in the bins before the border
-    const double one = (double)(1ull << a.shift), f = chunk.m > -INFINITY ? sample_weight(chunk.m, M, rules.scale) : 0.0;
+  const float ahead = top - a.chunk[at].top;  // bins
+  if (wave == 0) {  // its weights in the bins before the border
+    const int end = g_first - (int)fminf(ahead, (float)kBins);
     double s = 0.0;
-    if (g_first == kBins) {
-      s = lane == 63 ? chunk.sum : 0.0;
-    } else {
-      const int end = g_first - (int)fminf(ahead, (float)kBins);
 #pragma unroll
-      for (int i = 0; i < kBins / 64; i++)
-        if (64 * i + lane < end) s += (double)a.bin_mass[at * kBins + 64 * i + lane];
-      s = wave_scan_double(s) * kBinUnit;
+    for (int i = 0; i < kBins / 64; i++) {
+      const double m = (double)a.bin_mass[at * kBins + 64 * i + lane];
+      s += 64 * i + lane < end ? m : 0.0;
     }
-    if (lane == 63) a.chunk_mass[at] = (u64_t)__builtin_rint(s * f * one);
+    s = wave_scan_double(s) * kBinUnit;
+    if (lane == 63) a.chunk_mass[at] = (u64_t)__builtin_rint(s * a.factor[at] * (double)(1ull << a.shift));
   }
-  if (g_first == kBins || ahead > (float)max(g_last, k_bin)) return;  // none listed
+  if (ahead > (float)max(g_last, k_bin)) return;  // none listed
   const int first = c * CHUNK;
   const bool whole = first + CHUNK <= a.vocab;
-  float l[kEach];
-  sample_row<TYPE>(a, row).get_each(first + tid * VEC, THREADS * VEC, whole, l);
+  float l[EACH];
+  sample_row<TYPE>(a, row).template get_each<EACH>(first + tid * VEC, THREADS * VEC, whole, l);
   unsigned take = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; i++) {
-    const int b = sample_bin(l[i], rules.bin_scale, top);
+  for (int i = 0; i < EACH; i++) {
+    const int b = sample_bin(l[i], bin_scale, top);
     const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
     take |= (unsigned)(in && ((b >= g_first && b <= g_last) || b == k_bin)) << i;
   }
@@ -506,7 +522,7 @@ __global__ __launch_bounds__(THREADS) void sample_list_kernel(const SampleArgs a
   int to = base + before;
   u64_t* list = a.list + (size_t)row * kList;
 #pragma unroll
-  for (int i = 0; i < kEach; i++)
+  for (int i = 0; i < EACH; i++)
     if (take >> i & 1) {
       if (to < kList) list[to] = (u64_t)Row::key(l[i]) << 32 | (uint32_t)~(first + (i / VEC * THREADS + tid) * VEC + i % VEC);
       to++;
@@ -515,15 +531,24 @@ __global__ __launch_bounds__(THREADS) void sample_list_kernel(const SampleArgs a
 
 // ---- the cut and the token ---------------------------------------------------------------------------------------------
 
+constexpr u64_t kNobody = ~(u64_t)0;  // (no key is that large)
+
 struct SampleFound {
-  u64_t before, here;
+  u64_t before;
   int bin;
 };
 struct SampleShared {
-  u64_t list[kList], hist[kCrossBins], part[2][kRowWaves], chunk_mass[kMaxChunks];
+  union {
+    struct {
+      u64_t list[kList], mass[kList];
+    };
+    int kept[kLargeChunk];
+  };
+  u64_t hist[kCrossBins], part[2][kRowWaves], chunk_mass[kMaxChunks];
+  u64_t few[64], few_mass[64], result;
   SampleFound found[2];
   uint32_t ends[2][kRowWaves];
-  int token, last;
+  int few_n;
 };
 
 // A workgroup's steps in LDS; `turn` alternates between two places, so that one barrier a step is enough
@@ -549,71 +574,86 @@ struct SampleGroup {
     return before + s - v;
   }
 
-  // Of the elements i < n with a value get(i, value, mass): the value at which their masses, summed from the largest value down,
-  // reach `target` (at least 1, at most their sum); target becomes what is left of it for that value, `here` that value's sum.
-  // Every pass leaves a range of 1/1024 of the one before.
+  // Elements get(i, key, index, mass) of i < n, keys in [lo, hi], indices below vocab, in order of falling keys and rising indices:
+  // the one (key << 32 | ~index) at which their running mass reaches `target` (at least 1, at most their sum).  Histograms narrow
+  // the keys' range to 1/1024 a pass, then, among equals, the indices'; one wave ranks the last 64.
   template <class Get>
-  __device__ uint32_t cross(int n, u64_t& target, u64_t& here, Get get) {
-    uint32_t lo = ~0u, hi = 0;
-    for (int i = threadIdx.x; i < n; i += kRowThreads) {
-      uint32_t v;
-      u64_t m;
-      if (get(i, v, m)) lo = min(lo, v), hi = max(hi, v);
-    }
-    hi = wave_max_u32(hi), lo = wave_max_u32(~lo);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.ends[0][threadIdx.x >> 6] = lo, sh.ends[1][threadIdx.x >> 6] = hi;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kRowWaves; w++) lo = max(lo, sh.ends[0][w]), hi = max(hi, sh.ends[1][w]);
-    lo = ~lo;
-    here = 0;
-    bool more = lo <= hi;
-    while (more) {
-      const uint32_t span = hi - lo;
-      const int shift = span ? max(0, 32 - __builtin_clz(span) - 10) : 0;
-      for (int i = threadIdx.x; i < kCrossBins; i += kRowThreads) sh.hist[i] = 0;
-      turn ^= 1;
-      SampleFound& found = sh.found[turn];
-      if (threadIdx.x == 0) found = SampleFound{0, 0, 0};
+  __device__ u64_t cross(int n, uint32_t lo, uint32_t hi, int vocab, u64_t target, Get get) {
+    bool by_index = false;
+    uint32_t key_at = 0;
+    auto in_range = [&](uint32_t key, int index, uint32_t& v) {
+      v = by_index ? ~(uint32_t)index : key;
+      return v >= lo && v <= hi && (!by_index || key == key_at);
+    };
+    bool narrow = n > 64;
+    while (true) {
       __syncthreads();
+      if (threadIdx.x == 0) sh.few_n = 0;
+      if (narrow) {
+        const uint32_t span = hi - lo;
+        const int shift = span ? max(0, 32 - __builtin_clz(span) - 10) : 0;
+        for (int i = threadIdx.x; i < kCrossBins; i += kRowThreads) sh.hist[i] = 0;
+        turn ^= 1;
+        SampleFound& found = sh.found[turn];
+        if (threadIdx.x == 0) found = SampleFound{0, 0};
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kRowThreads) {
+          uint32_t key, v;
+          int index;
+          u64_t m;
+          if (get(i, key, index, m) && in_range(key, index, v)) atomicAdd(&sh.hist[(hi - v) >> shift], m);
+        }
+        __syncthreads();
+        constexpr int PER = kCrossBins / kRowThreads;
+        u64_t bin[PER], all = 0, total;
+#pragma unroll
+        for (int i = 0; i < PER; i++) bin[i] = sh.hist[threadIdx.x * PER + i], all += bin[i];
+        turn ^= 1;  // (scan turns again: it does not touch what `found` refers to)
+        u64_t before = scan(all, total);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          if (before < target && before + bin[i] >= target) found = SampleFound{before, (int)threadIdx.x * PER + i};
+          before += bin[i];
+        }
+        __syncthreads();
+        target -= found.before;
+        hi -= min((uint32_t)found.bin, span >> shift) << shift;
+        const uint32_t size = (1u << shift) - 1;
+        lo = hi - lo > size ? hi - size : lo;
+      } else {
+        __syncthreads();
+      }
       for (int i = threadIdx.x; i < n; i += kRowThreads) {
-        uint32_t v;
+        uint32_t key, v;
+        int index;
         u64_t m;
-        if (get(i, v, m) && v >= lo && v <= hi) atomicAdd(&sh.hist[(hi - v) >> shift], m);
+        if (get(i, key, index, m) && in_range(key, index, v)) {
+          const int at = atomicAdd(&sh.few_n, 1);
+          if (at < 64) sh.few[at] = (u64_t)key << 32 | (uint32_t)~index, sh.few_mass[at] = m;
+        }
       }
       __syncthreads();
-      u64_t bin[kCrossBins / kRowThreads], all = 0, total;
-#pragma unroll
-      for (int i = 0; i < kCrossBins / kRowThreads; i++) {
-        bin[i] = sh.hist[threadIdx.x * (kCrossBins / kRowThreads) + i];
-        all += bin[i];
+      const int few = sh.few_n;
+      if (few <= 64) {
+        if (threadIdx.x < 64) {
+          const int lane = threadIdx.x;
+          const u64_t mine = lane < few ? sh.few[lane] : 0, m = lane < few ? sh.few_mass[lane] : 0;
+          u64_t before = 0, least = ~0ull;
+          for (int j = 0; j < few; j++) {
+            const u64_t other = sh.few[j];
+            before += other > mine ? sh.few_mass[j] : 0;
+            least = min(least, other);
+          }
+          const unsigned long long hit = __builtin_amdgcn_ballot_w64(lane < few && before < target && before + m >= target);
+          const int at = hit ? __builtin_ctzll(hit) : -1;
+          if (lane == 0) sh.result = few == 0 ? kNobody : at < 0 ? least : sh.few[at];
+        }
+        __syncthreads();
+        return sh.result;
       }
-      turn ^= 1;  // (scan turns again: it does not touch what `found` refers to)
-      u64_t before = scan(all, total);
-#pragma unroll
-      for (int i = 0; i < kCrossBins / kRowThreads; i++) {
-        if (before < target && before + bin[i] >= target)
-          found = SampleFound{before, bin[i], (int)threadIdx.x * (kCrossBins / kRowThreads) + i};
-        before += bin[i];
-      }
-      __syncthreads();
-      target -= found.before;
-      here = found.here;
-      hi -= min((uint32_t)found.bin, span >> shift) << shift;
-      const uint32_t size = (1u << shift) - 1;
-      lo = hi - lo > size ? hi - size : lo;
-      more = lo < hi;
+      narrow = true;
+      if (lo == hi && !by_index) by_index = true, key_at = hi, lo = ~(uint32_t)(vocab - 1), hi = ~0u;
     }
-    return hi;
-  }
-
-  template <class Get>
-  __device__ __forceinline__ u64_t sum(int n, Get get) {
-    u64_t s = 0, total;
-    for (int i = threadIdx.x; i < n; i += kRowThreads) s += get(i);
-    scan(s, total);
-    return total;
   }
 };
 
@@ -632,26 +672,32 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
   }
   const Row x = sample_row<TYPE>(a, row);
   const SampleRules rules = sample_rules(a, row);
-  const bool fast = b.listed <= kList;
+  const double one = (double)(1ull << a.shift), base = (double)(1ull << (52 - a.shift));
+  auto weight = [&](float l) { return sample_weight(l, b.m, b.scale); };
+  auto mass = [&](float l) { return sample_units(weight(l), base); };
+  auto bin_of = [&](uint32_t key) { return sample_bin(Row::logit(key), b.bin_scale, b.top); };
+  const bool ruled = b.first < kBins, fast = b.listed <= kList;
   const int n = fast ? b.listed : V;
+  uint32_t lo = ~0u, hi = 0;  // of the list's keys
   if (fast)
-    for (int i = tid; i < n; i += kRowThreads) sh.list[i] = a.list[(size_t)row * kList + i];
-  const bool ruled = b.first < kBins;
+    for (int i = tid; i < n; i += kRowThreads) {
+      const u64_t v = a.list[(size_t)row * kList + i];
+      const uint32_t key = (uint32_t)(v >> 32);
+      sh.list[i] = v, sh.mass[i] = mass(Row::logit(key));
+      lo = min(lo, key), hi = max(hi, key);
+    }
+  lo = wave_max_u32(~lo), hi = wave_max_u32(hi);
+  if ((tid & 63) == 0) sh.ends[0][tid >> 6] = lo, sh.ends[1][tid >> 6] = hi;
   for (int c = tid; c < C; c += kRowThreads) {
     const size_t at = (size_t)row * C + c;
-    if (ruled) {
-      sh.chunk_mass[c] = a.chunk_mass[at];
-    } else {
-      const SampleChunk chunk = a.chunk[at];
-      const double f = chunk.m > -INFINITY ? sample_weight(chunk.m, b.m, rules.scale) : 0.0;
-      sh.chunk_mass[c] = (u64_t)__builtin_rint(f * chunk.sum * (double)(1ull << a.shift));
-    }
+    sh.chunk_mass[c] = ruled && !fast ? 0
+                       : ruled        ? a.chunk_mass[at]
+                                      : (u64_t)__builtin_rint(a.factor[at] * a.chunk[at].sum * one);
   }
   __syncthreads();
-  const double one = (double)(1ull << a.shift), base = (double)(1ull << (52 - a.shift));
-  auto weight = [&](float l) { return sample_weight(l, b.m, rules.scale); };
-  auto mass = [&](float l) { return sample_units(weight(l), base); };
-  auto bin_of = [&](uint32_t key) { return sample_bin(Row::logit(key), rules.bin_scale, b.top); };
+#pragma unroll
+  for (int w = 0; w < kRowWaves; w++) lo = max(lo, sh.ends[0][w]), hi = max(hi, sh.ends[1][w]);
+  lo = fast ? ~lo : 0, hi = fast ? hi : Row::key(b.m);
   auto element = [&](int i, uint32_t& key, int& index) {
     if (fast) {
       const u64_t v = sh.list[i];
@@ -660,34 +706,19 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
       key = Row::key(x.at(i)), index = i;
     }
   };
+  auto mass_of = [&](int i, uint32_t key) { return fast ? sh.mass[i] : mass(Row::logit(key)); };
 
   // the last kept element
   uint32_t cut = 0;
   int cut_at = V - 1;
   auto before_cut = [&](uint32_t key, int i) { return key > cut || (key == cut && i <= cut_at); };
-  auto kept = [&](float l, int i) { return before_cut(Row::key(l), i) && (!rules.by_m || weight(l) >= rules.m); };
-  // the first `count` of the `ties` elements of key `at`, by index
-  auto cut_ties = [&](uint32_t at, u64_t count, u64_t ties) {
-    cut = at, cut_at = V - 1;
-    if (count >= ties) return;
-    u64_t here;
-    cut_at = (int)~group.cross(n, count, here, [&](int i, uint32_t& v, u64_t& m) {
-      uint32_t key;
-      int index;
-      element(i, key, index);
-      v = ~(uint32_t)index, m = 1;
-      return key == at;
-    });
-  };
   if (rules.by_k && (!fast || b.k_bin >= 0)) {
-    u64_t target = fast ? b.k_left : rules.k, ties;
-    const uint32_t at = group.cross(n, target, ties, [&](int i, uint32_t& v, u64_t& m) {
-      int index;
-      element(i, v, index);
+    const u64_t at = group.cross(n, lo, hi, V, fast ? b.k_left : rules.k, [&](int i, uint32_t& key, int& index, u64_t& m) {
+      element(i, key, index);
       m = 1;
-      return !fast || bin_of(v) == b.k_bin;
+      return !fast || bin_of(key) == b.k_bin;
     });
-    cut_ties(at, target, ties);
+    if (at != kNobody) cut = (uint32_t)(at >> 32), cut_at = (int)~(uint32_t)at;
   }
   if (rules.by_p) {
     auto in_p = [&](uint32_t key, int index) {
@@ -695,125 +726,131 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
       const int g = fast ? bin_of(key) : b.p_first;
       return g >= b.p_first && g <= b.p_last;
     };
-    auto mass_at = [&](int i) -> u64_t {
+    // the sums of the bins that its last element may be in, and of what top-k keeps of its last one
+    u64_t most = 0, at_k = 0, before;
+    for (int i = tid; i < n; i += kRowThreads) {
       uint32_t key;
       int index;
       element(i, key, index);
-      return in_p(key, index) ? mass(Row::logit(key)) : 0;
-    };
-    double total = b.sum;
-    const u64_t most = group.sum(n, mass_at);
-    if (!fast)
-      total = (double)most / one;
-    else if (rules.by_k)
-      total = b.before_k + (double)group.sum(n, [&](int i) -> u64_t {
-                uint32_t key;
-                int index;
-                element(i, key, index);
-                return bin_of(key) == b.k_bin && before_cut(key, index) ? mass(Row::logit(key)) : 0;
-              }) / one;
+      if (!before_cut(key, index)) continue;
+      const u64_t m = mass_of(i, key);
+      most += in_p(key, index) ? m : 0;
+      at_k += fast && bin_of(key) == b.k_bin ? m : 0;
+    }
+    group.scan(most, before), most = before;
+    double total = fast ? b.sum : (double)most / one;
+    if (fast && rules.by_k) {
+      group.scan(at_k, before);
+      total = b.before_k + (double)before / one;
+    }
     const double bar = __builtin_ceil((rules.p * total - (fast ? b.before_p : 0.0)) * one);
-    u64_t target = bar >= 1.0 ? min((u64_t)bar, most) : 1, here;
     if (most > 0) {
-      const uint32_t at = group.cross(n, target, here, [&](int i, uint32_t& v, u64_t& m) {
-        int index;
-        element(i, v, index);
-        if (!in_p(v, index)) return false;
-        m = mass(Row::logit(v));
+      const u64_t target = bar >= 1.0 ? min((u64_t)bar, most) : 1;
+      const u64_t at = group.cross(n, lo, hi, V, target, [&](int i, uint32_t& key, int& index, u64_t& m) {
+        element(i, key, index);
+        if (!in_p(key, index)) return false;
+        m = mass_of(i, key);
         return true;
       });
-      const u64_t each = mass(Row::logit(at));
-      if (each > 0) {
-        const u64_t count = (target + each - 1) / each;
-        // where the key is top-k's too, the ties are those that it keeps
-        if (at != cut || count < here / each) cut_ties(at, count, here / each);
-      }
+      if (at != kNobody) cut = (uint32_t)(at >> 32), cut_at = (int)~(uint32_t)at;
     }
   }
 
   // the kept sum of every chunk, and the token
-  u64_t total = 0;
-  if (!fast) {
-    for (int c = tid; c < C; c += kRowThreads) sh.chunk_mass[c] = 0;
-    __syncthreads();
-  }
-  for (int i = tid; i < n; i += kRowThreads) {
-    uint32_t key;
-    int index;
-    element(i, key, index);
-    const float l = Row::logit(key);
-    if ((!fast || bin_of(key) <= b.last) && kept(l, index)) atomicAdd(&sh.chunk_mass[index / CHUNK], mass(l));
-  }
+  if (ruled)
+    for (int i = tid; i < n; i += kRowThreads) {
+      uint32_t key;
+      int index;
+      element(i, key, index);
+      if ((fast && bin_of(key) > b.last) || !before_cut(key, index)) continue;
+      if (rules.by_m && !(weight(Row::logit(key)) >= rules.m)) continue;
+      atomicAdd(&sh.chunk_mass[index / CHUNK], mass_of(i, key));
+    }
   __syncthreads();
   const u64_t here = tid < C ? sh.chunk_mass[tid] : 0;
+  u64_t total;
   const u64_t before = group.scan(here, total);
   if (tid == 0) border->cut = cut, border->cut_at = cut_at, border->inv = one / (double)total;
   if (!a.tokens) return;
   const float u = a.uniform[row];
   const double bar = (u > 0.f ? (double)u : 0.0) * (double)total;  // the smallest whole number above it
   const u64_t target = bar < (double)total ? min((u64_t)bar + 1, total) : total;
-  if (tid == 0) sh.token = V, sh.last = -1, sh.found[0] = SampleFound{0, 0, 0};
+  if (here > 0 && before < target && before + here >= target) sh.found[0] = SampleFound{before, tid};
   __syncthreads();
-  if (here > 0 && before < target && before + here >= target) sh.found[0] = SampleFound{before, here, tid};
-  __syncthreads();
-  const u64_t left = target - sh.found[0].before;
-  const int i0 = sh.found[0].bin * CHUNK + tid * EACH;
-  u64_t w[EACH], sum = 0, all;
+  u64_t left = target - sh.found[0].before;
+  const int c = sh.found[0].bin;
+  // the chunk's kept elements, by index
+  unsigned flags = 0;
 #pragma unroll
   for (int j = 0; j < EACH / VEC; j++) {
+    const int i0 = c * CHUNK + tid * EACH + j * VEC;
     float l[VEC];
-    x.get(i0 + j * VEC, false, l);
+    x.get(i0, false, l);
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
-      const int i = i0 + j * VEC + e;
-      w[j * VEC + e] = i < V && kept(l[e], i) ? mass(l[e]) : 0;
-      sum += w[j * VEC + e];
-    }
+    for (int e = 0; e < VEC; e++)
+      flags |= (unsigned)(i0 + e < V && before_cut(Row::key(l[e]), i0 + e)) << (j * VEC + e);
   }
-  u64_t run = group.scan(sum, all);
-  int found = V, last = -1;
+  u64_t kept;
+  int to = (int)group.scan(__builtin_popcount(flags), kept);
+#pragma unroll
+  for (int j = 0; j < EACH; j++)
+    if (flags >> j & 1) sh.kept[to++] = c * CHUNK + tid * EACH + j;
+  __syncthreads();
+  const int per = ((int)kept + kRowThreads - 1) / kRowThreads, first = tid * per;
+  u64_t w[EACH], sum = 0, all;
 #pragma unroll
   for (int j = 0; j < EACH; j++) {
-    run += w[j];
-    if (w[j] > 0) {
-      last = i0 + j;
-      if (run >= left) found = min(found, i0 + j);
+    w[j] = 0;
+    if (j >= per) continue;  // (uniform)
+    if (first + j < (int)kept) {
+      const float l = x.at(sh.kept[first + j]);
+      const double v = weight(l);
+      w[j] = v >= b.min_w ? sample_units(v, base) : 0;
     }
+    sum += w[j];
   }
-  if (found < V && run - sum < left) atomicMin(&sh.token, found);
-  if (last >= 0) atomicMax(&sh.last, last);  // rounding may leave the threshold to nobody
-  __syncthreads();
-  if (tid == 0) a.tokens[row] = sh.token < V ? sh.token : sh.last;
+  u64_t run = group.scan(sum, all);
+  left = min(left, all);  // (the chunk's sum from its bins may be a rounding apart)
+  if (all == 0 && tid == 0) a.tokens[row] = kept > 0 ? sh.kept[0] : -1;
+  if (run < left && run + sum >= left) {
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; j++) {
+      if (w[j] > 0 && run < left) at = first + j;
+      run += w[j];
+    }
+    a.tokens[row] = sh.kept[at];
+  }
 }
 
-template <int TYPE, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_probs_kernel(const SampleArgs a) {
+template <int TYPE, int EACH>
+__global__ __launch_bounds__(kChunkThreads) void sample_probs_kernel(const SampleArgs a) {
   using Row = SampleRow<TYPE>;
-  constexpr int VEC = Row::VEC;
+  constexpr int VEC = Row::VEC, THREADS = kChunkThreads;
   typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
-  const int row = blockIdx.y, first = blockIdx.x * (THREADS * kEach);
-  const bool whole = first + THREADS * kEach <= a.vocab;
-  float l[kEach], p[kEach];
-  sample_row<TYPE>(a, row).get_each(first + (int)threadIdx.x * VEC, THREADS * VEC, whole, l);
+  const int row = blockIdx.y, first = blockIdx.x * (THREADS * EACH);
+  const bool whole = first + THREADS * EACH <= a.vocab;
+  float l[EACH], p[EACH];
+  sample_row<TYPE>(a, row).template get_each<EACH>(first + (int)threadIdx.x * VEC, THREADS * VEC, whole, l);
   const SampleBorder* border = a.border + row;
   const double inv = border->inv;
   const float m = border->m;
   const uint32_t cut = border->cut;
   const int cut_at = border->cut_at;
-  const SampleRules rules = sample_rules(a, row);
+  const double scale = border->scale, min_w = border->min_w;
   float* out = a.probs + (size_t)row * a.vocab;
 #pragma unroll
-  for (int i = 0; i < kEach; i++) {
+  for (int i = 0; i < EACH; i++) {
     const int at = first + (i / VEC * THREADS + (int)threadIdx.x) * VEC + i % VEC;
     const uint32_t key = Row::key(l[i]);
     p[i] = 0.f;
     if (inv > 0.0 && (key > cut || (key == cut && at <= cut_at))) {
-      const double w = sample_weight(l[i], m, rules.scale);
-      p[i] = w >= rules.m ? (float)(w * inv) : 0.f;
+      const double w = sample_weight(l[i], m, scale);
+      p[i] = w >= min_w ? (float)(w * inv) : 0.f;
     }
   }
 #pragma unroll
-  for (int j = 0; j < kEach / VEC; j++) {
+  for (int j = 0; j < EACH / VEC; j++) {
     const int at = first + (j * THREADS + (int)threadIdx.x) * VEC;
     const float* q = p + j * VEC;
     if (at + VEC <= a.vocab) {
@@ -831,17 +868,17 @@ __global__ __launch_bounds__(THREADS) void sample_probs_kernel(const SampleArgs 
 static int sample_chunk(int rows, int vocab) { return (long long)rows * vocab <= (1 << 19) ? kSmallChunk : kLargeChunk; }
 static size_t sample_bytes(int rows, int chunks) {
   return rows * (sizeof(SampleBorder) + kList * sizeof(u64_t) +
-                 chunks * (sizeof(SampleChunk) + sizeof(u64_t) + kBins * (sizeof(u64_t) + sizeof(int))));
+                 chunks * (sizeof(SampleChunk) + sizeof(double) + sizeof(u64_t) + kBins * (sizeof(u64_t) + sizeof(int))));
 }
 
-template <int TYPE, int THREADS>
+template <int TYPE, int EACH>
 static hipError_t sample_launch(const SampleArgs& a, bool ruled, hipStream_t st) {
   const dim3 grid(a.chunks, a.rows);
-  sample_chunk_kernel<TYPE, THREADS><<<grid, THREADS, 0, st>>>(a);
+  sample_chunk_kernel<TYPE, EACH><<<grid, kChunkThreads, 0, st>>>(a);
   sample_border_kernel<<<a.rows, kBorderThreads, 0, st>>>(a);
-  if (ruled) sample_list_kernel<TYPE, THREADS><<<grid, THREADS, 0, st>>>(a);
-  sample_row_kernel<TYPE, THREADS * kEach><<<a.rows, kRowThreads, 0, st>>>(a);
-  if (a.probs) sample_probs_kernel<TYPE, THREADS><<<grid, THREADS, 0, st>>>(a);
+  if (ruled) sample_list_kernel<TYPE, EACH><<<grid, kChunkThreads, 0, st>>>(a);
+  sample_row_kernel<TYPE, kChunkThreads * EACH><<<a.rows, kRowThreads, 0, st>>>(a);
+  if (a.probs) sample_probs_kernel<TYPE, EACH><<<grid, kChunkThreads, 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -891,13 +928,14 @@ extern "C" int exl3_sample(const void* logits, int type, long long ld, int rows,
     a.list = reinterpret_cast<u64_t*>(a.border + slice);
     a.bin_mass = a.list + (size_t)slice * kList;
     a.chunk_mass = a.bin_mass + (size_t)slice * chunks * kBins;
-    a.chunk = reinterpret_cast<SampleChunk*>(a.chunk_mass + (size_t)slice * chunks);
+    a.factor = reinterpret_cast<double*>(a.chunk_mass + (size_t)slice * chunks);
+    a.chunk = reinterpret_cast<SampleChunk*>(a.factor + (size_t)slice * chunks);
     a.bin_count = reinterpret_cast<int*>(a.chunk + (size_t)slice * chunks);
     const bool large = chunk == kLargeChunk;
     hipStream_t st = as_stream(stream);
-    EXL3_CHECK_HIP(type == EXL3_F32    ? (large ? sample_launch<EXL3_F32, 1024>(a, ruled, st) : sample_launch<EXL3_F32, 512>(a, ruled, st))
-                   : type == EXL3_BF16 ? (large ? sample_launch<EXL3_BF16, 1024>(a, ruled, st) : sample_launch<EXL3_BF16, 512>(a, ruled, st))
-                                       : (large ? sample_launch<EXL3_F16, 1024>(a, ruled, st) : sample_launch<EXL3_F16, 512>(a, ruled, st)));
+    EXL3_CHECK_HIP(type == EXL3_F32    ? (large ? sample_launch<EXL3_F32, 16>(a, ruled, st) : sample_launch<EXL3_F32, 8>(a, ruled, st))
+                   : type == EXL3_BF16 ? (large ? sample_launch<EXL3_BF16, 16>(a, ruled, st) : sample_launch<EXL3_BF16, 8>(a, ruled, st))
+                                       : (large ? sample_launch<EXL3_F16, 16>(a, ruled, st) : sample_launch<EXL3_F16, 8>(a, ruled, st)));
   }
   return EXL3_OK;
 }
