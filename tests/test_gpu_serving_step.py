@@ -527,7 +527,8 @@ def test_sample_odd_logits():
     x[12] *= 1e-30
     logits, u = _t(x), rng.random(14)
     for t, k, p, m in ((1.0, 0, 1.0, 0.0), (0.7, 30, 0.9, 0.0), (1e-30, 0, 0.9, 0.0), (1e30, 0, 0.5, 0.0), (1.0, 0, 1.0, 0.1),
-                       (0.0, 0, 1.0, 0.0), (1e-44, 5, 1.0, 0.0), (3e38, 100, 0.99, 0.9)):
+                       (0.0, 0, 1.0, 0.0), (1e-44, 5, 1.0, 0.0), (3e38, 100, 0.99, 0.9), (float("inf"), 0, 0.5, 0.0),
+                       (1e300, 0, 0.9, 0.0)):
         _check_sample(logits, u, t, k, p, m)
     tokens, probs = _ops().sample_tokens(logits, _t(u.astype(np.float32)), return_probs=True)
     assert tokens[3] == tokens[4] == -1 and not probs[3].any() and not probs[4].any()

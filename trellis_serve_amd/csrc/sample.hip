@@ -48,7 +48,7 @@ constexpr int kBorderThreads = 256;               // a bin each, and a chunk eac
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kCrossBins = 1024;
-constexpr int kList = 3072;
+constexpr int kList = 2560;
 constexpr int kSliceRows = 1024;                  // rows of a workspace
 constexpr double kBinUnit = 0x1p-50;              // a bin's sum is in 2^-50 of the chunk's largest weight
 constexpr double kBinBase = 0x1p52 * kBinUnit;
@@ -143,8 +143,13 @@ struct Exp2Term<0> {
 __device__ __forceinline__ double exp2_f64(double t) {
   t = fmax(t, -1000.0);  // NaN (-inf at a scale of 0) too
   const double k = __builtin_rint(t), r = t - k;
-  double p = Exp2Term<12>::value;
-#define EXL3_TERM(i) p = __builtin_fma(p, r, Exp2Term<i>::value);
+  // (in scalar registers: as literals the compiler moves each into the accumulator, two instructions a term)
+  auto term = [](double c) {
+    asm("" : "+s"(c));
+    return c;
+  };
+  double p = term(Exp2Term<12>::value);
+#define EXL3_TERM(i) p = __builtin_fma(p, r, term(Exp2Term<i>::value));
   EXL3_TERM(11) EXL3_TERM(10) EXL3_TERM(9) EXL3_TERM(8) EXL3_TERM(7) EXL3_TERM(6) EXL3_TERM(5) EXL3_TERM(4) EXL3_TERM(3)
   EXL3_TERM(2) EXL3_TERM(1) EXL3_TERM(0)
 #undef EXL3_TERM
@@ -264,7 +269,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   constexpr int VEC = SampleRow<TYPE>::VEC, THREADS = kChunkThreads, WAVES = THREADS / 64, CHUNK = THREADS * EACH;
   __shared__ u64_t mass[kBins];
   __shared__ int count[kBins], firsts[kBins];
-  __shared__ float part[WAVES];
+  __shared__ float part[WAVES], coarse[WAVES];
   __shared__ double sums[WAVES];
   __shared__ int deepest;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
@@ -290,43 +295,36 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   const size_t at = (size_t)row * a.chunks + c;
   const float top = sample_place(m, rules.bin_scale);
   const bool any = m > -INFINITY;
-  double w[EACH], sum = 0.0;
-  if (any && m < INFINITY && whole) {
-    const double m64 = (double)m;
+  // Elements of bins past `deep` take no part in any rule.  By weight that holds with bins to spare while places are exact to a
+  // small part of one; exponents stand for logarithms (bins of 8 times floor(log2), up to 7 more than needed), and for top-p a sum
+  // in 32 bits is good enough.
+  int deep = bins ? kBins - 2 : -1;
+  const bool near = any && fabsf(top) < 0x1p16f;
+  auto bins_to = [](double w) { return 11 - 8 * __builtin_amdgcn_frexp_exp(w); };
+  if (near && rules.by_m && !(rules.by_k && rules.by_p)) deep = min(deep, bins_to(rules.m));
+  const bool by_sum = near && rules.by_p && !rules.by_k;
+  if (by_sum) {
+    const float scale = (float)rules.scale;
+    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < EACH; i++) {
-      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // a few chains at a time: all of them do not fit the registers
-      w[i] = exp2_f64(((double)l[i] - m64) * rules.scale);
-      sum += w[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < EACH; i++) {
-      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-      const bool in = any && (whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab);
-      w[i] = in ? sample_weight(l[i], m, rules.scale) : 0.0;
-      sum += w[i];
-    }
+    for (int i = 0; i < EACH; i++) s += __builtin_amdgcn_exp2f((l[i] - m) * scale);  // (0 for those past the row)
+    s += lane_xor<1>(s);
+    s += lane_xor<2>(s);
+    s += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, s), 0x124, 0xF, 0xF, false));
+    s += lane_xor<8>(s);
+    s = sum_over_groups(s);
+    if (lane == 0) coarse[wave] = s;
   }
-  sum = wave_scan_double(sum);
-  if (lane == 63) sums[wave] = sum;
   if (any && by_firsts) {
     const int bin = sample_bin(mine, rules.bin_scale, top);
     if (bin < kBins - 1) atomicAdd(&firsts[bin], 1);
   }
-  __syncthreads();
-  sum = 0.0;
+  if (by_sum || by_firsts) __syncthreads();
+  if (by_sum) {
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < WAVES; i++) sum += sums[i];
-  if (tid == 0) a.chunk[at] = SampleChunk{sum, m, top};
-  if (!bins) return;
-  // Elements of bins past `deep` take no part in any rule.  By weight that holds with bins to spare while places are exact to a
-  // small part of one; exponents stand for logarithms (bins of 8 times floor(log2), up to 7 more than needed).
-  int deep = kBins - 2;
-  if (any && fabsf(top) < 0x1p16f) {
-    auto bins_to = [](double w) { return 11 - 8 * __builtin_amdgcn_frexp_exp(w); };
-    if (rules.by_m && !(rules.by_k && rules.by_p)) deep = min(deep, bins_to(rules.m));
-    if (rules.by_p && !rules.by_k) deep = min(deep, bins_to((1.0 - rules.p) * sum / (double)a.vocab));
+    for (int i = 0; i < WAVES; i++) s += coarse[i];
+    if (s > 0.5f) deep = min(deep, bins_to((1.0 - rules.p) * (double)s / (double)a.vocab));  // (NaN: -inf at a scale of 0)
   }
   if (any && by_firsts) {
     if (wave == 0) {
@@ -348,19 +346,39 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
     __syncthreads();
     deep = min(deep, deepest);
   }
-  if (any) {
+  double sum = 0.0;
+  auto add = [&](int i, bool in, double w) {
+    sum += in ? w : 0.0;
+    const int bin = sample_bin(l[i], rules.bin_scale, top);
+    if (in && bin <= deep) {
+      atomicAdd(&mass[bin], sample_units(w, kBinBase));
+      if (rules.by_k) atomicAdd(&count[bin], 1);
+    }
+  };
+  if (any && m < INFINITY && whole) {
+    const double m64 = (double)m;
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
-      const int bin = sample_bin(l[i], rules.bin_scale, top);
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // a few chains at a time: all of them do not fit the registers
+      add(i, true, exp2_f64(((double)l[i] - m64) * rules.scale));
+    }
+  } else if (any) {
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
-      if (in && bin <= deep) {
-        atomicAdd(&mass[bin], sample_units(w[i], kBinBase));
-        if (rules.by_k) atomicAdd(&count[bin], 1);
-      }
+      add(i, in, sample_weight(l[i], m, rules.scale));
     }
   }
+  sum = wave_scan_double(sum);
+  if (lane == 63) sums[wave] = sum;
   __syncthreads();
-  if (tid < kBins) {
+  if (tid == 0) {
+    sum = 0.0;
+    for (int w = 0; w < WAVES; w++) sum += sums[w];
+    a.chunk[at] = SampleChunk{sum, m, top};
+  }
+  if (bins && tid < kBins) {
     a.bin_mass[at * kBins + tid] = mass[tid];
     if (rules.by_k) a.bin_count[at * kBins + tid] = count[tid];
   }
@@ -830,41 +848,46 @@ __global__ __launch_bounds__(kChunkThreads) void sample_probs_kernel(const Sampl
   typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));
   const int row = blockIdx.y, first = blockIdx.x * (THREADS * EACH);
   const bool whole = first + THREADS * EACH <= a.vocab;
-  float l[EACH], p[EACH];
-  sample_row<TYPE>(a, row).template get_each<EACH>(first + (int)threadIdx.x * VEC, THREADS * VEC, whole, l);
+  const Row x = sample_row<TYPE>(a, row);
+  float l[EACH];
+  x.template get_each<EACH>(first + (int)threadIdx.x * VEC, THREADS * VEC, whole, l);
   const SampleBorder* border = a.border + row;
-  const double inv = border->inv;
+  const double inv = border->inv, scale = border->scale, min_w = border->min_w;
   const float m = border->m;
   const uint32_t cut = border->cut;
   const int cut_at = border->cut_at;
-  const double scale = border->scale, min_w = border->min_w;
   float* out = a.probs + (size_t)row * a.vocab;
+  auto index = [&](int i) { return first + (i / VEC * THREADS + (int)threadIdx.x) * VEC + i % VEC; };
+  unsigned kept = 0;
 #pragma unroll
   for (int i = 0; i < EACH; i++) {
-    const int at = first + (i / VEC * THREADS + (int)threadIdx.x) * VEC + i % VEC;
     const uint32_t key = Row::key(l[i]);
-    p[i] = 0.f;
-    if (inv > 0.0 && (key > cut || (key == cut && at <= cut_at))) {
-      const double w = sample_weight(l[i], m, scale);
-      p[i] = w >= min_w ? (float)(w * inv) : 0.f;
-    }
+    kept |= (unsigned)((whole || index(i) < a.vocab) && (key > cut || (key == cut && index(i) <= cut_at))) << i;
   }
+  if (!(inv > 0.0)) kept = 0;
+  // zeros everywhere, then the few kept ones, each lane's in turn: a wave computes as many as its fullest lane has
 #pragma unroll
   for (int j = 0; j < EACH / VEC; j++) {
-    const int at = first + (j * THREADS + (int)threadIdx.x) * VEC;
-    const float* q = p + j * VEC;
-    if (at + VEC <= a.vocab) {
+    const int at = index(j * VEC);
+    if (whole || at + VEC <= a.vocab) {
 #pragma unroll
-      for (int e = 0; e < VEC; e += 4) *reinterpret_cast<f4_t*>(out + at + e) = f4_t{q[e], q[e + 1], q[e + 2], q[e + 3]};
+      for (int e = 0; e < VEC; e += 4) *reinterpret_cast<f4_t*>(out + at + e) = f4_t{0.f, 0.f, 0.f, 0.f};
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; e++)
-        if (at + e < a.vocab) out[at + e] = q[e];
+        if (at + e < a.vocab) out[at + e] = 0.f;
     }
+  }
+  while (kept) {
+    const int at = index(__builtin_ctz(kept));
+    kept &= kept - 1;
+    const double w = sample_weight(x.at(at), m, scale);
+    if (w >= min_w) out[at] = (float)(w * inv);
   }
 }
 
-// Chunks of 8192 elements, or 4096 for more workgroups where there are few elements in all (one row of 32003 fp32: TODO us)
+// Chunks of 8192 elements, or 4096 for more workgroups where there are few elements in all (one row of 32003 fp32: the chunks'
+// kernel takes 7.0 us with 4 chunks, 5.0 with 8)
 static int sample_chunk(int rows, int vocab) { return (long long)rows * vocab <= (1 << 19) ? kSmallChunk : kLargeChunk; }
 static size_t sample_bytes(int rows, int chunks) {
   return rows * (sizeof(SampleBorder) + kList * sizeof(u64_t) +
