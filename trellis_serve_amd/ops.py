@@ -1189,17 +1189,22 @@ def kv_step_plan(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: tor
             return kv_step_plan(page_table, seq_lens, new_lens, free_pages, free_state, rows, state_out)
     # one allocation, the workspace at its end
     buf = page_table.new_empty(5 * rows + 4 * B + 3)
-    slots, row_start, counts, after, positions, row_lens, row_seq, ws = buf.split(
-        (2 * rows, B + 1, B, B, rows, rows, rows, B + 2))
-    slots = slots.view(torch.int64)
-    if B == 0:
-        row_start.zero_()
+    at_slots = buf.data_ptr()
+    at_start = at_slots + 8 * rows
+    at_counts = at_start + 4 * B + 4
+    at_after = at_counts + 4 * B
+    at_pos = at_after + 4 * B
+    at_lens = at_pos + 4 * rows
+    at_seq = at_lens + 4 * rows
     _lib.check(_lib.load().exl3_kv_step_plan(
         page_table.data_ptr(), max_pages, seq_lens.data_ptr(), new_lens.data_ptr(), B, 16, free_pages.data_ptr(),
-        free_pages.numel(), free_state.data_ptr(), state_out.data_ptr(), rows, row_start.data_ptr(), counts.data_ptr(),
-        after.data_ptr(), positions.data_ptr(), row_lens.data_ptr(), row_seq.data_ptr(), slots.data_ptr(), ws.data_ptr(),
-        4 * (B + 2), torch._C._cuda_getCurrentRawStream(index)), "kv_step_plan")
-    return StepPlan(row_start, counts, after, positions, row_lens, row_seq, slots)
+        free_pages.numel(), free_state.data_ptr(), state_out.data_ptr(), rows, at_start, at_counts, at_after, at_pos, at_lens,
+        at_seq, at_slots, at_seq + 4 * rows, 4 * (B + 2), torch._C._cuda_getCurrentRawStream(index)), "kv_step_plan")
+    slots, row_start, counts, after, positions, row_lens, row_seq, _ = buf.split_with_sizes(
+        (2 * rows, B + 1, B, B, rows, rows, rows, B + 2))
+    if B == 0:
+        row_start.zero_()
+    return StepPlan(row_start, counts, after, positions, row_lens, row_seq, slots.view(torch.int64))
 
 
 def _row_stride(t: torch.Tensor, name: str, shape: tuple, dtypes) -> int:
@@ -1224,9 +1229,9 @@ def add_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tenso
     [T, dim] (taken through a sigmoid with gate_sigmoid); weights and gate fp16|bf16|fp32, weights of one type, as 1 + w with
     unit_offset.  fp32 inside, y from the h before its rounding.  out: (y, h) to write to; h may be the residual itself where
     that is contiguous."""
-    if x.dim() != 2:
-        raise ValueError(f"x must be [T, dim], got {tuple(x.shape)}")
     shape, dtype = x.shape, x.dtype
+    if len(shape) != 2:
+        raise ValueError(f"x must be [T, dim], got {tuple(shape)}")
     T, dim = shape
     ld_x = _row_stride(x, "x", shape, _HALVES)
     r_dtype, ld_r = dtype, dim
