@@ -569,6 +569,12 @@ struct SampleShared {
   int few_n;
 };
 
+template <int XOR>
+__device__ __forceinline__ u64_t add_lane_xor(u64_t v) {
+  const float lo = lane_xor<XOR>(__builtin_bit_cast(float, (uint32_t)v)), hi = lane_xor<XOR>(__builtin_bit_cast(float, (uint32_t)(v >> 32)));
+  return v + ((u64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo));
+}
+
 // A workgroup's steps in LDS; `turn` alternates between two places, so that one barrier a step is enough
 struct SampleGroup {
   SampleShared& sh;
@@ -594,7 +600,7 @@ struct SampleGroup {
 
   // Elements get(i, key, index, mass) of i < n, keys in [lo, hi], indices below vocab, in order of falling keys and rising indices:
   // the one (key << 32 | ~index) at which their running mass reaches `target` (at least 1, at most their sum).  Histograms narrow
-  // the keys' range to 1/1024 a pass, then, among equals, the indices'; one wave ranks the last 64.
+  // the keys' range to 1/1024 a pass, then, among equals, the indices'; the last 64 are ranked.
   template <class Get>
   __device__ u64_t cross(int n, uint32_t lo, uint32_t hi, int vocab, u64_t target, Get get) {
     bool by_index = false;
@@ -606,7 +612,7 @@ struct SampleGroup {
     bool narrow = n > 64;
     while (true) {
       __syncthreads();
-      if (threadIdx.x == 0) sh.few_n = 0;
+      if (threadIdx.x == 0) sh.few_n = 0, sh.result = kNobody;
       if (narrow) {
         const uint32_t span = hi - lo;
         const int shift = span ? max(0, 32 - __builtin_clz(span) - 10) : 0;
@@ -653,19 +659,18 @@ struct SampleGroup {
       __syncthreads();
       const int few = sh.few_n;
       if (few <= 64) {
-        if (threadIdx.x < 64) {
-          const int lane = threadIdx.x;
-          const u64_t mine = lane < few ? sh.few[lane] : 0, m = lane < few ? sh.few_mass[lane] : 0;
-          u64_t before = 0, least = ~0ull;
-          for (int j = 0; j < few; j++) {
-            const u64_t other = sh.few[j];
-            before += other > mine ? sh.few_mass[j] : 0;
-            least = min(least, other);
-          }
-          const unsigned long long hit = __builtin_amdgcn_ballot_w64(lane < few && before < target && before + m >= target);
-          const int at = hit ? __builtin_ctzll(hit) : -1;
-          if (lane == 0) sh.result = few == 0 ? kNobody : at < 0 ? least : sh.few[at];
+        // 8 lanes an element, each sums what an eighth of the others puts before it
+        constexpr int LANES = kRowThreads / 64;
+        const int e = threadIdx.x / LANES, part = threadIdx.x % LANES;
+        const u64_t mine = sh.few[e], m = sh.few_mass[e];
+        u64_t before = 0;
+#pragma unroll
+        for (int j = 0; j < 64; j += LANES) {
+          const u64_t other = sh.few[j + part], mass = sh.few_mass[j + part];
+          before += j + part < few && other > mine ? mass : 0;
         }
+        before = add_lane_xor<1>(before), before = add_lane_xor<2>(before), before = add_lane_xor<4>(before);
+        if (e < few && part == 0 && before < target && before + m >= target) sh.result = mine;
         __syncthreads();
         return sh.result;
       }
