@@ -55,13 +55,13 @@ constexpr double kBinBase = 0x1p52 * kBinUnit;
 static_assert(kMaxChunks <= kBorderThreads && kBins == kBorderThreads);
 
 struct SampleChunk {
-  double sum;    // of exp((l - m) / t)
+  double sum;    // of exp((l - m) / t); with a top-k of at least those of the first k
   float m, top;  // the largest logit, its place on the bins' scale
 };
 
 // What a row's kernels know of it
 struct SampleBorder {
-  double sum;                 // of all weights
+  double sum;                 // of all weights; with a top-k of at least the first k's
   double before_k, before_p;  // of those in the bins before k_bin, p_first
   double inv;                 // 1 / the sum of the kept weights (sample_row_kernel); 0: no logit above -inf
   double scale, min_w;        // of SampleRules: scale, m
@@ -347,27 +347,41 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
     deep = min(deep, deepest);
   }
   double sum = 0.0;
-  auto add = [&](int i, bool in, double w) {
+  auto add = [&](float l, bool in, double w) {
     sum += in ? w : 0.0;
-    const int bin = sample_bin(l[i], rules.bin_scale, top);
+    const int bin = sample_bin(l, rules.bin_scale, top);
     if (in && bin <= deep) {
       atomicAdd(&mass[bin], sample_units(w, kBinBase));
       if (rules.by_k) atomicAdd(&count[bin], 1);
     }
   };
-  if (any && m < INFINITY && whole) {
+  if (any && by_firsts && deepest < kBins) {
+    // the first k's weights are all that is asked for: the few that may be theirs, each lane's in turn
+    unsigned take = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+      const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
+      take |= (unsigned)(in && sample_bin(l[i], rules.bin_scale, top) <= deep) << i;
+    }
+    while (take) {
+      const int i = __builtin_ctz(take);
+      take &= take - 1;
+      const float one = x.at(first + (i / VEC * THREADS + tid) * VEC + i % VEC);
+      add(one, true, sample_weight(one, m, rules.scale));
+    }
+  } else if (any && m < INFINITY && whole) {
     const double m64 = (double)m;
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
       if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // a few chains at a time: all of them do not fit the registers
-      add(i, true, exp2_f64(((double)l[i] - m64) * rules.scale));
+      add(l[i], true, exp2_f64(((double)l[i] - m64) * rules.scale));
     }
   } else if (any) {
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
       if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       const bool in = whole || first + (i / VEC * THREADS + tid) * VEC + i % VEC < a.vocab;
-      add(i, in, sample_weight(l[i], m, rules.scale));
+      add(l[i], in, sample_weight(l[i], m, rules.scale));
     }
   }
   sum = wave_scan_double(sum);
