@@ -48,7 +48,7 @@ constexpr int kBorderThreads = 256;               // a bin each, and a chunk eac
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kCrossBins = 1024;
-constexpr int kList = 2560;
+constexpr int kList = 2560;                       // (1024 at least: sample_row_kernel reads two a thread ahead)
 constexpr int kSliceRows = 1024;                  // rows of a workspace
 constexpr double kBinUnit = 0x1p-50;              // a bin's sum is in 2^-50 of the chunk's largest weight
 constexpr double kBinBase = 0x1p52 * kBinUnit;
@@ -613,33 +613,33 @@ struct SampleGroup {
   }
 
   // Elements get(i, key, index, mass) of i < n, keys in [lo, hi], indices below vocab, in order of falling keys and rising indices:
-  // the one (key << 32 | ~index) at which their running mass reaches `target` (at least 1, at most their sum).  Histograms narrow
-  // the keys' range to 1/1024 a pass, then, among equals, the indices'; the last 64 are ranked.
+  // the one (key << 32 | ~index) at which their running mass reaches `target` (at least 1, at most their sum).  An element's place
+  // in that order is one number, (hi - key, index); histograms narrow its range to 1/1024 a pass, the last 64 are ranked.  (Few keys
+  // leave bits of the first histogram to the indices, so that equal logits do not all add to one place of it.)
   template <class Get>
   __device__ u64_t cross(int n, uint32_t lo, uint32_t hi, int vocab, u64_t target, Get get) {
-    bool by_index = false;
-    uint32_t key_at = 0;
-    auto in_range = [&](uint32_t key, int index, uint32_t& v) {
-      v = by_index ? ~(uint32_t)index : key;
-      return v >= lo && v <= hi && (!by_index || key == key_at);
-    };
+    const int low = vocab > 1 ? 32 - __builtin_clz(vocab - 1) : 0;
+    int bits = low + (hi > lo ? 32 - __builtin_clz(hi - lo) : 0);
+    u64_t from = 0;
+    auto offset = [&](uint32_t key, int index) { return ((u64_t)(hi - key) << low | (uint32_t)index) - from; };
     bool narrow = n > 64;
     while (true) {
       __syncthreads();
       if (threadIdx.x == 0) sh.few_n = 0, sh.result = kNobody;
       if (narrow) {
-        const uint32_t span = hi - lo;
-        const int shift = span ? max(0, 32 - __builtin_clz(span) - 10) : 0;
+        const int shift = max(0, bits - 10);
         for (int i = threadIdx.x; i < kCrossBins; i += kRowThreads) sh.hist[i] = 0;
         turn ^= 1;
         SampleFound& found = sh.found[turn];
         if (threadIdx.x == 0) found = SampleFound{0, 0};
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += kRowThreads) {
-          uint32_t key, v;
+          uint32_t key;
           int index;
           u64_t m;
-          if (get(i, key, index, m) && in_range(key, index, v)) atomicAdd(&sh.hist[(hi - v) >> shift], m);
+          if (!get(i, key, index, m)) continue;
+          const u64_t v = offset(key, index);
+          if (v >> bits == 0) atomicAdd(&sh.hist[v >> shift], m);
         }
         __syncthreads();
         constexpr int PER = kCrossBins / kRowThreads;
@@ -655,19 +655,20 @@ struct SampleGroup {
         }
         __syncthreads();
         target -= found.before;
-        hi -= min((uint32_t)found.bin, span >> shift) << shift;
-        const uint32_t size = (1u << shift) - 1;
-        lo = hi - lo > size ? hi - size : lo;
+        from += (u64_t)found.bin << shift;
+        bits = shift;
       } else {
         __syncthreads();
       }
       for (int i = threadIdx.x; i < n; i += kRowThreads) {
-        uint32_t key, v;
+        uint32_t key;
         int index;
         u64_t m;
-        if (get(i, key, index, m) && in_range(key, index, v)) {
+        if (!get(i, key, index, m)) continue;
+        const u64_t v = offset(key, index);
+        if (v >> bits == 0) {
           const int at = atomicAdd(&sh.few_n, 1);
-          if (at < 64) sh.few[at] = (u64_t)key << 32 | (uint32_t)~index, sh.few_mass[at] = m;
+          if (at < 64) sh.few[at] = v, sh.few_mass[at] = m;
         }
       }
       __syncthreads();
@@ -681,15 +682,17 @@ struct SampleGroup {
 #pragma unroll
         for (int j = 0; j < 64; j += LANES) {
           const u64_t other = sh.few[j + part], mass = sh.few_mass[j + part];
-          before += j + part < few && other > mine ? mass : 0;
+          before += j + part < few && other < mine ? mass : 0;
         }
         before = add_lane_xor<1>(before), before = add_lane_xor<2>(before), before = add_lane_xor<4>(before);
-        if (e < few && part == 0 && before < target && before + m >= target) sh.result = mine;
+        if (e < few && part == 0 && before < target && before + m >= target) {
+          const u64_t v = mine + from;
+          sh.result = (u64_t)(hi - (uint32_t)(v >> low)) << 32 | ~((uint32_t)v & ((1u << low) - 1));
+        }
         __syncthreads();
         return sh.result;
       }
       narrow = true;
-      if (lo == hi && !by_index) by_index = true, key_at = hi, lo = ~(uint32_t)(vocab - 1), hi = ~0u;
     }
   }
 };
@@ -702,6 +705,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
   SampleGroup group{sh};
   const int row = blockIdx.x, tid = threadIdx.x, V = a.vocab, C = a.chunks;
   SampleBorder* border = a.border + row;
+  const u64_t* list = a.list + (size_t)row * kList;
+  // (before their number is known: what the list does not hold is not looked at)
+  constexpr int AHEAD = 2;
+  u64_t ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; j++) ahead[j] = list[tid + j * kRowThreads];
   const SampleBorder b = *border;
   if (!(b.m > -INFINITY)) {
     if (tid == 0 && a.tokens) a.tokens[row] = -1;
@@ -716,13 +725,17 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
   const bool ruled = b.first < kBins, fast = b.listed <= kList;
   const int n = fast ? b.listed : V;
   uint32_t lo = ~0u, hi = 0;  // of the list's keys
-  if (fast)
-    for (int i = tid; i < n; i += kRowThreads) {
-      const u64_t v = a.list[(size_t)row * kList + i];
+  if (fast) {
+    auto take = [&](int i, u64_t v) {
       const uint32_t key = (uint32_t)(v >> 32);
       sh.list[i] = v, sh.mass[i] = mass(Row::logit(key));
       lo = min(lo, key), hi = max(hi, key);
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++)
+      if (tid + j * kRowThreads < n) take(tid + j * kRowThreads, ahead[j]);
+    for (int i = tid + AHEAD * kRowThreads; i < n; i += kRowThreads) take(i, list[i]);
+  }
   lo = wave_max_u32(~lo), hi = wave_max_u32(hi);
   if ((tid & 63) == 0) sh.ends[0][tid >> 6] = lo, sh.ends[1][tid >> 6] = hi;
   for (int c = tid; c < C; c += kRowThreads) {
@@ -817,21 +830,18 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
   u64_t left = target - sh.found[0].before;
   const int c = sh.found[0].bin;
   // the chunk's kept elements, by index
+  const int i0 = c * CHUNK + tid * EACH;
+  float l[EACH];
+  x.template get_each<EACH>(i0, VEC, (c + 1) * CHUNK <= V, l);
   unsigned flags = 0;
 #pragma unroll
-  for (int j = 0; j < EACH / VEC; j++) {
-    const int i0 = c * CHUNK + tid * EACH + j * VEC;
-    float l[VEC];
-    x.get(i0, false, l);
-#pragma unroll
-    for (int e = 0; e < VEC; e++)
-      flags |= (unsigned)(i0 + e < V && before_cut(Row::key(l[e]), i0 + e)) << (j * VEC + e);
-  }
+  for (int j = 0; j < EACH; j++)
+    flags |= (unsigned)(i0 + j < V && before_cut(Row::key(l[j]), i0 + j) && sample_bin(l[j], b.bin_scale, b.top) <= b.last) << j;
   u64_t kept;
   int to = (int)group.scan(__builtin_popcount(flags), kept);
 #pragma unroll
   for (int j = 0; j < EACH; j++)
-    if (flags >> j & 1) sh.kept[to++] = c * CHUNK + tid * EACH + j;
+    if (flags >> j & 1) sh.kept[to++] = i0 + j;
   __syncthreads();
   const int per = ((int)kept + kRowThreads - 1) / kRowThreads, first = tid * per;
   u64_t w[EACH], sum = 0, all;
