@@ -452,7 +452,7 @@ size_t exl3_kv_select_workspace_bytes(int rows, int num_kv_heads, int max_pages)
  *   worth = max over the group's heads of fp32(S * (a * k_scale)),  a = max |q|,  S = sum_d q8_d (q8_d > 0 ? hi_d : lo_d),
  *   q8 = rint(127 q / a) to nearest even (infinities +-127 and NaN 0, neither counts for a),
  * an upper bound of the page's logits but for the rounding of q8 and the (positive) scale of the softmax.  NaN worths come
- * last.  Two launches; deterministic; calls that share a workspace must not overlap. */
+ * last.  One or two launches; deterministic; calls that share a workspace must not overlap. */
 int exl3_kv_select_pages(const void* q, long long ld_q, const void* k_scale, const void* bounds, int num_pages,
                          const int* page_table, int batch, int max_pages, const int* row_seq, const int* seq_lens, int rows,
                          int num_q_heads, int num_kv_heads, int head_dim, int page_size, int bits, int top, int first,
@@ -470,7 +470,7 @@ int exl3_kv_sparse_attention(const void* q, long long ld_q, const void* k_cache,
 
 /* Workspace bytes of exl3_sample.  No zero-fill needed. */
 size_t exl3_sample_workspace_bytes(int rows, int vocab);
-/* Tokens from logits [rows][vocab] (fp16 | bf16 | fp32, row stride ld; NaN as -inf; vocab up to 2^24): with w = exp((l - max l) /
+/* Tokens from logits [rows][vocab] (fp16 | bf16 | fp32, row stride ld; NaN as -inf; vocab up to 2^20): with w = exp((l - max l) /
  * temperature) and the elements in order of falling logits (ties by rising index), kept is the shortest of
  *   the first top_k (<= 0: all);  those whose predecessors have less than top_p of the sum of w over the first top_k (>= 1 or
  *   NaN: all);  those with w >= min_p (<= 0 or NaN: all; above 1 as 1);
