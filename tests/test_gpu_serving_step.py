@@ -571,3 +571,39 @@ def test_sample_shapes_and_strides():
     assert _ops().sample_tokens(logits[:0], u[:0]).shape == (0,)
     out = torch.empty((12, 777), device="cuda")
     assert _ops().sampling_probs(logits, 0.9, 10, out=out) is out
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_sample_flat_rows(dtype):
+    """Rows so flat that a rule's last element may be any of them."""
+    rng = np.random.default_rng(5)
+    B, V = 3, 60013
+    logits = _t(5 + np.array([[0.0], [0.003], [0.05]]) * rng.standard_normal((B, V))).to(T_OF[dtype])
+    for t, k, p, m in ((1.0, 0, 0.9, 0.0), (0.7, 30000, 1.0, 0.0), (1.0, 45001, 0.6, 0.97), (2.0, 0, 1.0, 0.99), (1.0, 60012, 0.999, 0.0),
+                       (1.0, 0, 1e-6, 0.0), (1.0, 5000, 0.5, 0.0)):
+        _check_sample(logits, rng.random(B), t, k, p, m)
+
+
+def test_sample_many_rows_of_own_settings():
+    rng = np.random.default_rng(6)
+    B, V = 1030, 70
+    some = lambda a, b: np.where(rng.random(B) < 0.3, a, b)   # noqa: E731
+    _check_sample(_logits(rng, B, V, "fp32"), rng.random(B), some(0.0, rng.uniform(0.2, 2, B)), some(0, rng.integers(-1, 2 * V, B)),
+                  some(1.0, rng.uniform(0, 1.1, B)), some(0.0, rng.uniform(0, 0.3, B)))
+
+
+def test_sample_largest_vocabulary():
+    rng = np.random.default_rng(7)
+    B, V = 2, 1 << 20
+    logits = _logits(rng, B, V, "fp32")
+    u = rng.random(B).astype(np.float32)
+    x = _n(logits)
+    for t, k, p, m in ((1.0, 0, 0.9, 0.0), (0.8, 1000, 0.97, 0.0), (1.0, 0, 1.0, 0.01), (1.0, 0, 1.0, 0.0)):
+        tokens, probs = _ops().sample_tokens(logits, _t(u), t, k, p, m, return_probs=True)
+        for b in range(B):
+            token, want = ref.sample(x[b], float(u[b]), t, k, p, m)
+            assert int(tokens[b]) == token
+            # the kept weights, of which the largest is 1, are summed in units of 2^-42: half a unit each, and one rounding to fp32
+            d = np.abs(_n(probs[b]).astype(np.float64) - want)
+            kept = int((want > 0).sum())
+            assert (d <= want * (2.0 ** -24 + kept * 2.0 ** -43 + 2.0 ** -38) + 2.0 ** -149).all()

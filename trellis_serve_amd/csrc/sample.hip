@@ -12,7 +12,7 @@
 //
 // Weights are 64-bit.  Where atomics sum them (in LDS) they are integers, so that no result depends on an order, in units of
 // 2^-50 of a chunk's largest weight or 2^-42 to 2^-52 of the row's: another summation decides differently only where a
-// threshold lies within some 10^-12 of the total of an edge.
+// threshold lies within some 10^-12 of the total (131072 elements) of an edge.
 //
 // sample_chunk_kernel: (chunks, rows) workgroups.  A chunk's largest logit m, its sum of exp((l - m) / t), and counts and sums
 //   in 256 bins an eighth of an octave of w wide.  An element's bin is a monotone function of its logit alone, so the chunks'

@@ -1250,9 +1250,9 @@ def add_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tenso
         if gate.dtype not in _WEIGHT_TYPE:
             raise ValueError(f"gate must be fp16, bf16 or fp32, got {gate.dtype}")
         g_type, g_shape = _WEIGHT_TYPE[gate.dtype], gate.shape
-        if g_shape == (dim,) and (gate.is_contiguous()):
+        if g_shape == (dim,) and gate.is_contiguous():
             kind = 1
-        elif g_shape == shape and (dim > 1):
+        elif g_shape == shape and dim > 1:
             kind, ld_g = 3, _row_stride(gate, "gate", shape, _WEIGHT_TYPE)
         elif g_shape == (T, 1):
             kind, ld_g = 2, gate.stride(0) if T > 1 else 1
