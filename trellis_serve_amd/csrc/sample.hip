@@ -22,8 +22,13 @@
 // sample_list_kernel: (chunks, rows) workgroups list those bins' elements (some hundreds a row) and sum what lies before them.
 // sample_row_kernel: a workgroup per row finds the cut in the list, by histograms of ever smaller ranges; then the chunk, and in
 //   it the element, where the running sum passes the threshold.  Rows so flat that their border bins hold more than the list
-//   takes go through the same search over the whole row.
+//   takes go through the same search over the whole row, in one workgroup (131072 logits with a deviation of 0.1 t, top-p 0.9:
+//   470 us, where a deviation of t takes 41).
 // sample_probs_kernel: (chunks, rows) workgroups write the probabilities.
+//
+// Latency bounds it: each kernel waits for the whole of the one before, and a row's search is a chain of barriers.  In us, chunks,
+// border, list, row, probabilities:  one row of 32003 fp32  5.3 + 3.9 + 5.1 + 8.2;  48 of 100352 fp16  14.3 + 5.5 + 7.7 + 13.5
+// + 10.5;  64 of 131072 bf16  16.6 + 6.6 + 8.3 + 16.3.  (48 x 100352 half-precision logits read once are 1.9 us.)
 #include <math.h>
 
 #include <algorithm>
@@ -48,8 +53,8 @@ constexpr int kBorderThreads = 256;               // a bin each, and a chunk eac
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kCrossBins = 1024;
-constexpr int kList = 2560;                       // (1024 at least: sample_row_kernel reads two a thread ahead)
-constexpr int kSliceRows = 1024;                  // rows of a workspace
+constexpr int kList = 8192;                       // of a row; in LDS two workgroups a CU fit (1024 at least: sample_row_kernel reads ahead)
+constexpr int kSliceRows = 512;                   // rows of a workspace
 constexpr double kBinUnit = 0x1p-50;              // a bin's sum is in 2^-50 of the chunk's largest weight
 constexpr double kBinBase = 0x1p52 * kBinUnit;
 static_assert(kMaxChunks <= kBorderThreads && kBins == kBorderThreads);
@@ -571,9 +576,7 @@ struct SampleFound {
 };
 struct SampleShared {
   union {
-    struct {
-      u64_t list[kList], mass[kList];
-    };
+    u64_t list[kList];
     int kept[kLargeChunk];
   };
   u64_t hist[kCrossBins], part[2][kRowWaves], chunk_mass[kMaxChunks];
@@ -612,12 +615,13 @@ struct SampleGroup {
     return before + s - v;
   }
 
-  // Elements get(i, key, index, mass) of i < n, keys in [lo, hi], indices below vocab, in order of falling keys and rising indices:
-  // the one (key << 32 | ~index) at which their running mass reaches `target` (at least 1, at most their sum).  An element's place
-  // in that order is one number, (hi - key, index); histograms narrow its range to 1/1024 a pass, the last 64 are ranked.  (Few keys
-  // leave bits of the first histogram to the indices, so that equal logits do not all add to one place of it.)
-  template <class Get>
-  __device__ u64_t cross(int n, uint32_t lo, uint32_t hi, int vocab, u64_t target, Get get) {
+  // Elements that each(f) calls f(key, index, mass()) for (a thread has its own; n of all threads at most), keys in [lo, hi],
+  // indices below vocab, in order of falling keys and rising indices: the one (key << 32 | ~index) at which their running mass
+  // reaches `target` (at least 1, at most their sum).  An element's place in that order is one number, (hi - key, index);
+  // histograms narrow its range to 1/1024 a pass, the last 64 are ranked.  (Few keys leave bits of the first histogram to the
+  // indices, so that equal logits do not all add to one place of it.)
+  template <class Each>
+  __device__ __forceinline__ u64_t cross(int n, uint32_t lo, uint32_t hi, int vocab, u64_t target, Each each) {
     const int low = vocab > 1 ? 32 - __builtin_clz(vocab - 1) : 0;
     int bits = low + (hi > lo ? 32 - __builtin_clz(hi - lo) : 0);
     u64_t from = 0;
@@ -633,14 +637,10 @@ struct SampleGroup {
         SampleFound& found = sh.found[turn];
         if (threadIdx.x == 0) found = SampleFound{0, 0};
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kRowThreads) {
-          uint32_t key;
-          int index;
-          u64_t m;
-          if (!get(i, key, index, m)) continue;
+        each([&](uint32_t key, int index, auto mass) {
           const u64_t v = offset(key, index);
-          if (v >> bits == 0) atomicAdd(&sh.hist[v >> shift], m);
-        }
+          if (v >> bits == 0) atomicAdd(&sh.hist[v >> shift], mass());
+        });
         __syncthreads();
         constexpr int PER = kCrossBins / kRowThreads;
         u64_t bin[PER], all = 0, total;
@@ -660,17 +660,13 @@ struct SampleGroup {
       } else {
         __syncthreads();
       }
-      for (int i = threadIdx.x; i < n; i += kRowThreads) {
-        uint32_t key;
-        int index;
-        u64_t m;
-        if (!get(i, key, index, m)) continue;
+      each([&](uint32_t key, int index, auto mass) {
         const u64_t v = offset(key, index);
         if (v >> bits == 0) {
           const int at = atomicAdd(&sh.few_n, 1);
-          if (at < 64) sh.few[at] = v, sh.few_mass[at] = m;
+          if (at < 64) sh.few[at] = v, sh.few_mass[at] = mass();
         }
-      }
+      });
       __syncthreads();
       const int few = sh.few_n;
       if (few <= 64) {
@@ -728,7 +724,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
   if (fast) {
     auto take = [&](int i, u64_t v) {
       const uint32_t key = (uint32_t)(v >> 32);
-      sh.list[i] = v, sh.mass[i] = mass(Row::logit(key));
+      sh.list[i] = v;
       lo = min(lo, key), hi = max(hi, key);
     };
 #pragma unroll
@@ -748,25 +744,33 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
 #pragma unroll
   for (int w = 0; w < kRowWaves; w++) lo = max(lo, sh.ends[0][w]), hi = max(hi, sh.ends[1][w]);
   lo = fast ? ~lo : 0, hi = fast ? hi : Row::key(b.m);
-  auto element = [&](int i, uint32_t& key, int& index) {
+  // f(key, index, mass()) of the list's elements, or of the row's
+  auto each = [&](auto f) {
     if (fast) {
-      const u64_t v = sh.list[i];
-      key = (uint32_t)(v >> 32), index = (int)~(uint32_t)v;
+      for (int i = tid; i < n; i += kRowThreads) {
+        const u64_t v = sh.list[i];
+        f((uint32_t)(v >> 32), (int)~(uint32_t)v, [&] { return mass(Row::logit((uint32_t)(v >> 32))); });
+      }
     } else {
-      key = Row::key(x.at(i)), index = i;
+      for (int i = tid * VEC; i < V; i += kRowThreads * VEC) {
+        float l[VEC];
+        x.get(i, false, l);
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+          if (i + e < V) f(Row::key(l[e]), i + e, [&] { return mass(l[e]); });
+      }
     }
   };
-  auto mass_of = [&](int i, uint32_t key) { return fast ? sh.mass[i] : mass(Row::logit(key)); };
 
   // the last kept element
   uint32_t cut = 0;
   int cut_at = V - 1;
   auto before_cut = [&](uint32_t key, int i) { return key > cut || (key == cut && i <= cut_at); };
   if (rules.by_k && (!fast || b.k_bin >= 0)) {
-    const u64_t at = group.cross(n, lo, hi, V, fast ? b.k_left : rules.k, [&](int i, uint32_t& key, int& index, u64_t& m) {
-      element(i, key, index);
-      m = 1;
-      return !fast || bin_of(key) == b.k_bin;
+    const u64_t at = group.cross(n, lo, hi, V, fast ? b.k_left : rules.k, [&](auto f) {
+      each([&](uint32_t key, int index, auto) {
+        if (!fast || bin_of(key) == b.k_bin) f(key, index, [] { return (u64_t)1; });
+      });
     });
     if (at != kNobody) cut = (uint32_t)(at >> 32), cut_at = (int)~(uint32_t)at;
   }
@@ -778,15 +782,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
     };
     // the sums of the bins that its last element may be in, and of what top-k keeps of its last one
     u64_t most = 0, at_k = 0, before;
-    for (int i = tid; i < n; i += kRowThreads) {
-      uint32_t key;
-      int index;
-      element(i, key, index);
-      if (!before_cut(key, index)) continue;
-      const u64_t m = mass_of(i, key);
+    each([&](uint32_t key, int index, auto mass_of) {
+      if (!before_cut(key, index)) return;
+      const u64_t m = mass_of();
       most += in_p(key, index) ? m : 0;
       at_k += fast && bin_of(key) == b.k_bin ? m : 0;
-    }
+    });
     group.scan(most, before), most = before;
     double total = fast ? b.sum : (double)most / one;
     if (fast && rules.by_k) {
@@ -796,11 +797,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
     const double bar = __builtin_ceil((rules.p * total - (fast ? b.before_p : 0.0)) * one);
     if (most > 0) {
       const u64_t target = bar >= 1.0 ? min((u64_t)bar, most) : 1;
-      const u64_t at = group.cross(n, lo, hi, V, target, [&](int i, uint32_t& key, int& index, u64_t& m) {
-        element(i, key, index);
-        if (!in_p(key, index)) return false;
-        m = mass_of(i, key);
-        return true;
+      const u64_t at = group.cross(n, lo, hi, V, target, [&](auto f) {
+        each([&](uint32_t key, int index, auto mass_of) {
+          if (in_p(key, index)) f(key, index, mass_of);
+        });
       });
       if (at != kNobody) cut = (uint32_t)(at >> 32), cut_at = (int)~(uint32_t)at;
     }
@@ -808,14 +808,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_row_kernel(const SampleArg
 
   // the kept sum of every chunk, and the token
   if (ruled)
-    for (int i = tid; i < n; i += kRowThreads) {
-      uint32_t key;
-      int index;
-      element(i, key, index);
-      if ((fast && bin_of(key) > b.last) || !before_cut(key, index)) continue;
-      if (rules.by_m && !(weight(Row::logit(key)) >= rules.m)) continue;
-      atomicAdd(&sh.chunk_mass[index / CHUNK], mass_of(i, key));
-    }
+    each([&](uint32_t key, int index, auto mass_of) {
+      if ((fast && bin_of(key) > b.last) || !before_cut(key, index)) return;
+      if (rules.by_m && !(weight(Row::logit(key)) >= rules.m)) return;
+      atomicAdd(&sh.chunk_mass[index / CHUNK], mass_of());
+    });
   __syncthreads();
   const u64_t here = tid < C ? sh.chunk_mass[tid] : 0;
   u64_t total;
