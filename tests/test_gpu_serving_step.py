@@ -607,3 +607,22 @@ def test_sample_largest_vocabulary():
             d = np.abs(_n(probs[b]).astype(np.float64) - want)
             kept = int((want > 0).sum())
             assert (d <= want * (2.0 ** -24 + kept * 2.0 ** -43 + 2.0 ** -38) + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("top", [3, 70])   # one part a head, and several
+def test_sparse_attention_of_a_query_that_is_no_number(bits, top):
+    """NaN in a head's query: NaN in its output, and in no other's."""
+    rng = np.random.default_rng(bits)
+    L, Hq, Hkv = 1500, 8, 2
+    P = (L + PAGE - 1) // PAGE
+    cache = [_t(x) for x in _random_cache(rng, P, Hkv, bits)]
+    q = _t(rng.standard_normal((1, Hq, D))).half()
+    table, seen = _i([list(range(P))]), _i([L])
+    pages = _i(np.sort([rng.permutation(P)[:top] for _ in range(Hkv)], 1)[None])
+    clean = _ops().kv_sparse_attention(q, *cache, table, seen, bits, pages)
+    q[0, 5, 77] = float("nan")
+    got = _ops().kv_sparse_attention(q, *cache, table, seen, bits, pages)
+    assert got[0, 5].isnan().all()
+    others = [h for h in range(Hq) if h != 5]
+    assert torch.equal(got[0, others], clean[0, others])

@@ -599,6 +599,8 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
     }
   }
 
+  // (logits that are NaN move no reference: without this a query of them alone would count as one that sees nothing)
+  if (s.m == -INFINITY && s.l != 0.f) s.m = 0.f;
   // join the waves; lane (n, g) holds dims 32 g + 8 i + db of query n
   float* red_ml = red + W * G * (kHeadDim + 1);
   if (n < G) {
