@@ -626,3 +626,24 @@ def test_sparse_attention_of_a_query_that_is_no_number(bits, top):
     assert got[0, 5].isnan().all()
     others = [h for h in range(Hq) if h != 5]
     assert torch.equal(got[0, others], clean[0, others])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("top,first,last", [(50, 1, 2), (9000, 3, 4), (1, 0, 1)])
+def test_choice_among_tens_of_thousands_of_pages(bits, top, first, last):
+    """One sequence whose table names few pages again and again, so that thousands of equal worths lie at the border."""
+    rng = np.random.default_rng(bits + top)
+    L, Hq, Hkv, P = 300001, 6, 2, 300
+    cache = _random_cache(rng, P, Hkv, bits)
+    pages = (L + PAGE - 1) // PAGE
+    edge = ref.bounds(cache[0], np.zeros((P, Hkv, 2, 16 * bits), cache[0].dtype), np.arange(P, dtype=np.int32)[None], [P * PAGE],
+                      None, bits)
+    q = rng.standard_normal((2, Hq, D)).astype(np.float16)
+    for names in (P, 3):
+        table = rng.integers(0, names, (1, pages + 5)).astype(np.int32)
+        seen, row_seq = [L, L - 40000], [0, 0]
+        got = _ops().kv_select_pages(_t(q), _t(edge), _t(cache[2]), _t(table), _i(seen), bits, top, first, last, row_seq=_i(row_seq))
+        want = ref.select(q, edge, cache[2], table, seen, bits, top, first, last, row_seq)
+        assert np.array_equal(_n(got), want)
+    out = _ops().kv_sparse_attention(_t(q), *[_t(c) for c in cache], _t(table), _i(seen), bits, got, row_seq=_i(row_seq))
+    _check_sparse(out, q, cache, table, seen, bits, want, row_seq=row_seq)
