@@ -647,3 +647,21 @@ def test_choice_among_tens_of_thousands_of_pages(bits, top, first, last):
         assert np.array_equal(_n(got), want)
     out = _ops().kv_sparse_attention(_t(q), *[_t(c) for c in cache], _t(table), _i(seen), bits, got, row_seq=_i(row_seq))
     _check_sparse(out, q, cache, table, seen, bits, want, row_seq=row_seq)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_sample_rows_flat_in_places(dtype):
+    """Flat rows with a few peaks, with masked places, with one value in every sixteen of them, of large values."""
+    rng = np.random.default_rng(8)
+    V = 40007
+    x = 0.03 * rng.standard_normal((6, V))
+    x[0, rng.integers(0, V, 5)] += 9
+    x[1, ::3] = -np.inf
+    x[2, V // 2:] = torch.finfo(torch.float32).min / 2
+    x[3, : V // 32 * 31] = 0.5
+    x[3, V // 32 * 31 + 16:] -= rng.uniform(0, 30, V - V // 32 * 31 - 16)
+    x[4] = x[4] * 1e-4 + 3000
+    x[5, ::2] -= 40
+    logits = _t(x).to(T_OF[dtype])
+    for t, k, p, m in ((1.0, 0, 0.9, 0.0), (1.0, 100, 1.0, 0.0), (0.9, 20000, 0.7, 0.0), (3.0, 0, 1.0, 0.98), (0.02, 0, 0.99, 0.001)):
+        _check_sample(logits, rng.random(6), t, k, p, m)

@@ -15,20 +15,20 @@
 // threshold lies within some 10^-12 of the total (131072 elements) of an edge.
 //
 // sample_chunk_kernel: (chunks, rows) workgroups.  A chunk's largest logit m, its sum of exp((l - m) / t), and counts and sums
-//   in 256 bins an eighth of an octave of w wide.  An element's bin is a monotone function of its logit alone, so the chunks'
+//   in 256 bins an eighth of an octave of w wide (less where the row is flat).  An element's bin is a monotone function of its logit alone, so the chunks'
 //   bins match, and an element of a lower bin comes before every one of a higher.  Elements that the chunk alone shows to be cut
 //   (less than (1 - p) / vocab of its sum, behind its k-th, below m of its largest) stay out of the bins.
 // sample_border_kernel: a workgroup per row adds the bins up and so knows the bins that each rule's last element is in.
 // sample_list_kernel: (chunks, rows) workgroups list those bins' elements (some hundreds a row) and sum what lies before them.
 // sample_row_kernel: a workgroup per row finds the cut in the list, by histograms of ever smaller ranges; then the chunk, and in
-//   it the element, where the running sum passes the threshold.  Rows so flat that their border bins hold more than the list
-//   takes go through the same search over the whole row, in one workgroup (131072 logits with a deviation of 0.1 t, top-p 0.9:
-//   470 us, where a deviation of t takes 41).
+//   it the element, where the running sum passes the threshold.  Rows of which the border bins hold more than the list takes (most
+//   of the row equal; a top-k of half of 131072 with a top-p) go through the same search over the whole row, in one workgroup
+//   (131072 equal logits, top-p 0.9: 970 us).
 // sample_probs_kernel: (chunks, rows) workgroups write the probabilities.
 //
 // Latency bounds it: each kernel waits for the whole of the one before, and a row's search is a chain of barriers.  In us, chunks,
-// border, list, row, probabilities:  one row of 32003 fp32  5.3 + 3.9 + 5.1 + 8.2;  48 of 100352 fp16  14.3 + 5.5 + 7.7 + 13.5
-// + 10.5;  64 of 131072 bf16  16.6 + 6.6 + 8.3 + 16.3.  (48 x 100352 half-precision logits read once are 1.9 us.)
+// border, list, row, probabilities:  one row of 32003 fp32  5.5 + 3.9 + 5.1 + 8.2;  48 of 100352 fp16  14.4 + 5.5 + 7.7 + 13.5
+// + 10.5;  64 of 131072 bf16  16.7 + 6.6 + 8.3 + 16.3.  (48 x 100352 half-precision logits read once are 1.9 us.)
 #include <math.h>
 
 #include <algorithm>
@@ -62,6 +62,7 @@ static_assert(kMaxChunks <= kBorderThreads && kBins == kBorderThreads);
 struct SampleChunk {
   double sum;    // of exp((l - m) / t); with a top-k of at least those of the first k
   float m, top;  // the largest logit, its place on the bins' scale
+  float bin_scale, unused;  // of the row
 };
 
 // What a row's kernels know of it
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   constexpr int VEC = SampleRow<TYPE>::VEC, THREADS = kChunkThreads, WAVES = THREADS / 64, CHUNK = THREADS * EACH;
   __shared__ u64_t mass[kBins];
   __shared__ int count[kBins], firsts[kBins];
-  __shared__ float part[WAVES], coarse[WAVES];
+  __shared__ float part[WAVES], ends[2], coarse[WAVES];
   __shared__ double sums[WAVES];
   __shared__ int deepest;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
@@ -283,7 +284,13 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   const bool whole = first + CHUNK <= a.vocab;
   float l[EACH];
   x.template get_each<EACH>(first + tid * VEC, THREADS * VEC, whole, l);
-  const SampleRules rules = sample_rules(a, row);
+  // Each chunk looks at the same 64 elements of the row: one that is flat there has finer bins (by a power of two, so that they still
+  // reach over four times the range of these), or its border bins would hold more than the list takes (131072 logits whose
+  // deviation is a tenth of t, top-p 0.9: 38 us for 463; the kernel takes 0.3 us more)
+  constexpr int SIDE = 16;  // elements side by side
+  const bool probed = a.vocab > kList && wave == 0;
+  const float probe = probed ? x.at(lane / SIDE * (a.vocab / (64 / SIDE)) + lane % SIDE) : 0.f;
+  SampleRules rules = sample_rules(a, row);
   const bool bins = rules.by_k || rules.by_p || rules.by_m;
   // behind a chunk's k-th largest element, for k up to half its threads: bins of its threads' largest elements tell (others are more)
   const bool by_firsts = rules.by_k && rules.k <= THREADS / 2;
@@ -294,9 +301,17 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   for (int i = 1; i < EACH; i++) mine = fmaxf(mine, l[i]);
   float m = wave_max_f32(mine);
   if (lane == 0) part[wave] = m;
+  if (wave == 0) {
+    const float high = wave_max_f32(probe), low = wave_max_f32(probe > -INFINITY ? -probe : -INFINITY);
+    if (lane == 0) ends[0] = high, ends[1] = low;
+  }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; w++) m = fmaxf(m, part[w]);
+  int finer = 0;
+  const float range = (ends[0] + ends[1]) * (float)rules.scale;  // (0 where none were looked at)
+  if (range > 0.f && range < 8.f) finer = min(max(5 - __builtin_amdgcn_frexp_expf(4.f * range), 0), 10);
+  rules.bin_scale = __builtin_amdgcn_ldexpf(rules.bin_scale, finer);
   const size_t at = (size_t)row * a.chunks + c;
   const float top = sample_place(m, rules.bin_scale);
   const bool any = m > -INFINITY;
@@ -305,7 +320,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   // in 32 bits is good enough.
   int deep = bins ? kBins - 2 : -1;
   const bool near = any && fabsf(top) < 0x1p16f;
-  auto bins_to = [](double w) { return 11 - 8 * __builtin_amdgcn_frexp_exp(w); };
+  auto bins_to = [=](double w) { return (8 - 8 * __builtin_amdgcn_frexp_exp(w)) * (1 << finer) + 3; };
   if (near && rules.by_m && !(rules.by_k && rules.by_p)) deep = min(deep, bins_to(rules.m));
   const bool by_sum = near && rules.by_p && !rules.by_k;
   if (by_sum) {
@@ -395,7 +410,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   if (tid == 0) {
     sum = 0.0;
     for (int w = 0; w < WAVES; w++) sum += sums[w];
-    a.chunk[at] = SampleChunk{sum, m, top};
+    a.chunk[at] = SampleChunk{sum, m, top, rules.bin_scale, 0.f};
   }
   if (bins && tid < kBins) {
     a.bin_mass[at * kBins + tid] = mass[tid];
@@ -411,8 +426,9 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(const Sam
   __shared__ float part[2][WAVES];
   __shared__ int shift[kMaxChunks], counts[WAVES], k_at[2], below[2][WAVES];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, C = a.chunks;
-  const SampleRules rules = sample_rules(a, row);
-  SampleChunk chunk{0.0, -INFINITY, -INFINITY};
+  SampleRules rules = sample_rules(a, row);
+  rules.bin_scale = a.chunk[(size_t)row * C].bin_scale;
+  SampleChunk chunk{0.0, -INFINITY, -INFINITY, 0.f, 0.f};
   if (tid < C) chunk = a.chunk[(size_t)row * C + tid];
   const float m = wave_max_f32(chunk.m), t = wave_max_f32(chunk.top);
   if (lane == 0) part[0][wave] = m, part[1][wave] = t;
