@@ -15,7 +15,8 @@
 // threshold lies within some 10^-12 of the total (131072 elements) of an edge.
 //
 // sample_chunk_kernel: (chunks, rows) workgroups.  A chunk's largest logit m, its sum of exp((l - m) / t), and counts and sums
-//   in 256 bins an eighth of an octave of w wide (less where the row is flat).  An element's bin is a monotone function of its logit alone, so the chunks'
+//   in 256 bins an eighth of an octave of w wide (less where the row is flat).  An element's bin is a monotone function of its
+//   logit alone (and of the row's scale), so the chunks'
 //   bins match, and an element of a lower bin comes before every one of a higher.  Elements that the chunk alone shows to be cut
 //   (less than (1 - p) / vocab of its sum, behind its k-th, below m of its largest) stay out of the bins.
 // sample_border_kernel: a workgroup per row adds the bins up and so knows the bins that each rule's last element is in.
@@ -53,7 +54,7 @@ constexpr int kBorderThreads = 256;               // a bin each, and a chunk eac
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kCrossBins = 1024;
-constexpr int kList = 8192;                       // of a row; in LDS two workgroups a CU fit (1024 at least: sample_row_kernel reads ahead)
+constexpr int kList = 8192;                       // (two workgroups' fit a CU's LDS; sample_row_kernel reads 1024 ahead)
 constexpr int kSliceRows = 512;                   // rows of a workspace
 constexpr double kBinUnit = 0x1p-50;              // a bin's sum is in 2^-50 of the chunk's largest weight
 constexpr double kBinBase = 0x1p52 * kBinUnit;
@@ -438,7 +439,8 @@ __global__ __launch_bounds__(kBorderThreads) void sample_border_kernel(const Sam
 #pragma unroll
   for (int w = 1; w < WAVES; w++) M = fmaxf(M, part[0][w]), top = fmaxf(top, part[1][w]);
   SampleBorder b{};
-  b.m = M, b.top = top, b.scale = rules.scale, b.min_w = rules.m, b.bin_scale = rules.bin_scale, b.first = kBins, b.last = kBins - 1, b.k_bin = -1, b.p_last = -1, b.cut_at = a.vocab - 1;
+  b.m = M, b.top = top, b.scale = rules.scale, b.min_w = rules.m, b.bin_scale = rules.bin_scale;
+  b.first = kBins, b.last = kBins - 1, b.k_bin = -1, b.p_last = -1, b.cut_at = a.vocab - 1;
   if (!(M > -INFINITY)) {  // nothing to draw from
     if (tid == 0) a.border[row] = b;
     return;
@@ -604,7 +606,8 @@ struct SampleShared {
 
 template <int XOR>
 __device__ __forceinline__ u64_t add_lane_xor(u64_t v) {
-  const float lo = lane_xor<XOR>(__builtin_bit_cast(float, (uint32_t)v)), hi = lane_xor<XOR>(__builtin_bit_cast(float, (uint32_t)(v >> 32)));
+  const float lo = lane_xor<XOR>(__builtin_bit_cast(float, (uint32_t)v));
+  const float hi = lane_xor<XOR>(__builtin_bit_cast(float, (uint32_t)(v >> 32)));
   return v + ((u64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo));
 }
 
