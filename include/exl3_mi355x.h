@@ -404,7 +404,9 @@ size_t exl3_kv_step_plan_workspace_bytes(int batch);
  *   free_pages int32 [num_free]: a ring of free page ids; free_state int32 [2]: the place of its first live entry, and how
  *     many are live.  Pages are taken from its beginning, in order of b, and written behind the others of the sequence into
  *     page_table int32 [batch][max_pages]; pages that a shrinking sequence gives up go to its end.  free_state_out gets the
- *     state after the step (it may be free_state itself).  A page is in the ring or in one table row, never in both.
+ *     state after the step (it may be free_state itself).  A page is in the ring or in one table row, never in both.  A page
+ *     given up may take the place of one taken in the same step.  num_free is at least the pages that are live after any step;
+ *     where the given-up ones are more than its places, the last of them, in order of b, are left out.
  *   A sequence gets all of its tokens or none: none when its table row is too short, when its rows pass `rows`, or when the
  *     pages asked for so far, its own among them, are more than there are (one that needs no page still gets its tokens).
  *   row_start int32 [batch + 1]: the running sums of the tokens asked for (at most `rows`); counts int32 [batch]: the tokens

@@ -14,6 +14,9 @@
 // step_plan_kernel: one workgroup scans the sequences, 1024 at a time, and, where the step is small, fills the rows too.
 // Otherwise step_fill_kernel does: waves of one sequence write its rows, its new table entries and its returned pages.  The
 // ring's state may be updated in place, since only the first kernel reads it.
+// A returned page may go to the place of one that is taken in the same step, where the ring has fewer places than there are pages
+// (live + given back > ring_pages): all that is taken is read before anything is put back.  step_plan_kernel has a barrier
+// between the two; before step_fill_kernel it then writes the taken pages into the table, and the fill reads them there.
 #include <algorithm>
 
 #include "exl3_api.hpp"
@@ -35,9 +38,18 @@ struct StepPlanArgs {
   int rows;
   int *row_start, *counts, *lens_after, *positions, *row_lens, *row_seq;
   long long* slots;
-  int* base;  // [batch + 2]: a sequence's first taken (or returned) page; then the ring's head and count before the step
+  int* base;  // [batch]: a sequence's first taken (or returned) page; then PlanRing
   int slices; // waves per sequence of the fill
 };
+
+// The step's view of the ring, behind `base`
+struct PlanRing {
+  int head, live;  // before the step
+  int places;      // for returned pages: those of no live entry after the step's pages are taken; pages past them are left out
+  int early;       // the table has the taken pages before the fill
+};
+constexpr int kPlanRingInts = sizeof(PlanRing) / sizeof(int);
+__device__ __forceinline__ PlanRing& plan_ring(const StepPlanArgs& a) { return *reinterpret_cast<PlanRing*>(a.base + a.batch); }
 
 // sums stop at kMost, which leaves room for one more number in 32 bits
 constexpr int kMost = (1 << 30) - 1;
@@ -78,41 +90,58 @@ __device__ __forceinline__ void plan_scan(int (&v)[N], int (&carry)[N], int (&pa
 
 __device__ __forceinline__ int plan_pages(int tokens) { return (int)(((unsigned)tokens + kPage - 1) / kPage); }
 
-// Slice `slice` of sequence b's rows, table entries and returned pages, or (b == batch) of the rows behind the last sequence
-__device__ __forceinline__ void plan_fill(const StepPlanArgs& a, int b, int slice) {
-  const int lane = threadIdx.x & 63, first = slice * 64 + lane, step = a.slices * 64;
+// What the scans say of sequence b
+struct PlanSequence {
+  int len, asked, have, base;
+  int* row;
+};
+__device__ __forceinline__ PlanSequence plan_sequence(const StepPlanArgs& a, int b) {
+  const int len = min(max(a.lens[b], 0), a.max_pages * kPage);
+  return PlanSequence{len, a.new_lens[b], plan_pages(len), a.base[b], a.table + (size_t)b * a.max_pages};
+}
+
+// The pages that sequence b takes, into its table row, and its rows; or (b == batch) the rows behind the last sequence.
+// in_table: the taken pages are there
+__device__ __forceinline__ void plan_fill(const StepPlanArgs& a, int b, const PlanSequence& s, int first, int step, bool take,
+                                          bool rows, bool in_table) {
   if (b == a.batch) {
+    if (!rows) return;
     for (int r = a.row_start[b] + first; r < a.rows; r += step)
       a.positions[r] = -1, a.row_lens[r] = 0, a.row_seq[r] = -1, a.slots[r] = -1;
     return;
   }
-  const int len = min(max(a.lens[b], 0), a.max_pages * kPage), asked = a.new_lens[b], have = plan_pages(len);
-  const int base = a.base[b];
-  const unsigned head = a.base[a.batch], P = a.ring_pages;
-  int* row = a.table + (size_t)b * a.max_pages;
-  if (asked < 0) {
-    const unsigned to = head + (unsigned)a.base[a.batch + 1] + (unsigned)base;
-    const int keep = plan_pages(a.lens_after[b]);
-    for (int j = first; j < have - keep; j += step) a.ring[(to + j) % P] = row[keep + j];
-    return;
-  }
-  const int r0 = a.row_start[b], n = a.row_start[b + 1] - r0, count = a.counts[b];
-  const int need = plan_pages(len + count) - have;
+  if (s.asked < 0) return;
+  const unsigned head = plan_ring(a).head, P = a.ring_pages;
   auto taken = [&](int j) {  // base + j is below the live pages
-    const unsigned at = head + base + j;
+    const unsigned at = head + s.base + j;
     return a.ring[at < P ? at : at - P];
   };
-  for (int j = first; j < need; j += step) row[have + j] = taken(j);
+  const int count = a.counts[b];
+  if (take) {
+    const int need = plan_pages(s.len + count) - s.have;
+    for (int j = first; j < need; j += step) s.row[s.have + j] = taken(j);
+  }
+  if (!rows) return;
+  const int r0 = a.row_start[b], n = a.row_start[b + 1] - r0;
   for (int i = first; i < n; i += step) {
-    const int r = r0 + i, pos = len + i, lp = pos / kPage;
+    const int r = r0 + i, pos = s.len + i, lp = pos / kPage;
     const bool live = i < count;
     int page = 0;
-    if (live) page = lp < have ? row[lp] : taken(lp - have);
+    if (live) page = in_table || lp < s.have ? s.row[lp] : taken(lp - s.have);
     a.positions[r] = live ? pos : -1;
     a.row_lens[r] = live ? pos + 1 : 0;
     a.row_seq[r] = live ? b : -1;
     a.slots[r] = live ? (long long)page * kPage + pos % kPage : -1;
   }
+}
+
+// The pages that sequence b gives up, to the ring's end
+__device__ __forceinline__ void plan_give(const StepPlanArgs& a, int b, const PlanSequence& s, int first, int step) {
+  if (s.asked >= 0) return;
+  const PlanRing ring = plan_ring(a);
+  const int keep = plan_pages(a.lens_after[b]), give = min(s.have - keep, ring.places - s.base);
+  const unsigned to = (unsigned)ring.head + (unsigned)ring.live + (unsigned)s.base;
+  for (int j = first; j < give; j += step) a.ring[(to + j) % (unsigned)a.ring_pages] = s.row[keep + j];
 }
 
 template <bool FILL>
@@ -148,24 +177,32 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(const StepPlanA
     }
   }
   __syncthreads();
+  const bool early = live + ends[1] > a.ring_pages;
   if (threadIdx.x == 0) {
     a.row_start[0] = 0;
-    a.base[a.batch] = head, a.base[a.batch + 1] = live;
+    plan_ring(a) = PlanRing{head, live, a.ring_pages - (live - popped), early};
     const unsigned at = (unsigned)head + (unsigned)popped;
     a.state_out[0] = (int)(at % (unsigned)a.ring_pages);
     a.state_out[1] = min(live - popped + ends[1], a.ring_pages);
   }
-  if constexpr (FILL) {
-    __syncthreads();
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int i = wave; i < (a.batch + 1) * a.slices; i += kPlanThreads / 64) plan_fill(a, i / a.slices, i % a.slices);
-  }
+  if (!FILL && !early) return;
+  __syncthreads();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int b = wave; b <= a.batch; b += kPlanThreads / 64)
+    plan_fill(a, b, plan_sequence(a, min(b, a.batch - 1)), lane, 64, true, FILL, false);
+  if (!FILL || ends[1] == 0) return;
+  __syncthreads();
+  for (int b = wave; b < a.batch; b += kPlanThreads / 64) plan_give(a, b, plan_sequence(a, b), lane, 64);
 }
 
 __global__ __launch_bounds__(256) void step_fill_kernel(const StepPlanArgs a) {
   const long long i = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= (long long)(a.batch + 1) * a.slices) return;
-  plan_fill(a, (int)(i / a.slices), (int)(i % a.slices));
+  const int b = (int)(i / a.slices), first = (int)(i % a.slices) * 64 + (threadIdx.x & 63), step = a.slices * 64;
+  const PlanSequence s = plan_sequence(a, min(b, a.batch - 1));
+  const bool early = plan_ring(a).early;
+  plan_fill(a, b, s, first, step, !early, true, early);
+  if (b < a.batch) plan_give(a, b, s, first, step);
 }
 
 }  // namespace exl3
@@ -173,7 +210,7 @@ __global__ __launch_bounds__(256) void step_fill_kernel(const StepPlanArgs a) {
 using namespace exl3;
 
 extern "C" size_t exl3_kv_step_plan_workspace_bytes(int batch) {
-  return batch <= 0 ? 0 : ((size_t)batch + 2) * sizeof(int);
+  return batch <= 0 ? 0 : ((size_t)batch + kPlanRingInts) * sizeof(int);
 }
 
 extern "C" int exl3_kv_step_plan(int* page_table, int max_pages, const int* seq_lens, const int* new_lens, int batch,

@@ -1162,7 +1162,8 @@ def kv_step_plan(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: tor
     seq_lens[b] tokens and asks for new_lens[b] more (int32 [B]), or, below 0, gives its last -new_lens[b] ones up.  free_pages
     int32 is a ring of free page ids, free_state int32 [2] the place of its first live entry and how many are live: pages are
     taken from its beginning in order of b and written into page_table int32 [B, max_pages]; pages given up go to its end;
-    state_out (None: free_state itself) gets its state after the step.  A sequence gets all of its tokens or none: none when its
+    state_out (None: free_state itself) gets its state after the step.  The ring is to have a place for every page that is ever
+    live in it: given-up pages past its places are left out.  A sequence gets all of its tokens or none: none when its
     table row is too short, its rows pass `rows`, or the pages asked for so far are more than there are.
     Returns, for the step's `rows` rows (new token i of b is row row_start[b] + i): row_start (kv_append's), counts (the tokens
     got; kv_append's), lens_after, positions (qk_norm_rope's), row_lens and row_seq (kv_select_pages' and
@@ -1188,7 +1189,7 @@ def kv_step_plan(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: tor
         with torch.cuda.device(index):
             return kv_step_plan(page_table, seq_lens, new_lens, free_pages, free_state, rows, state_out)
     # one allocation, the workspace at its end
-    buf = page_table.new_empty(5 * rows + 4 * B + 3)
+    buf = page_table.new_empty(5 * rows + 4 * B + 5)
     at_slots = buf.data_ptr()
     at_start = at_slots + 8 * rows
     at_counts = at_start + 4 * B + 4
@@ -1199,9 +1200,9 @@ def kv_step_plan(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: tor
     _lib.check(_lib.load().exl3_kv_step_plan(
         page_table.data_ptr(), max_pages, seq_lens.data_ptr(), new_lens.data_ptr(), B, 16, free_pages.data_ptr(),
         free_pages.numel(), free_state.data_ptr(), state_out.data_ptr(), rows, at_start, at_counts, at_after, at_pos, at_lens,
-        at_seq, at_slots, at_seq + 4 * rows, 4 * (B + 2), torch._C._cuda_getCurrentRawStream(index)), "kv_step_plan")
+        at_seq, at_slots, at_seq + 4 * rows, 4 * (B + 4), torch._C._cuda_getCurrentRawStream(index)), "kv_step_plan")
     slots, row_start, counts, after, positions, row_lens, row_seq, _ = buf.split_with_sizes(
-        (2 * rows, B + 1, B, B, rows, rows, rows, B + 2))
+        (2 * rows, B + 1, B, B, rows, rows, rows, B + 4))
     if B == 0:
         row_start.zero_()
     return StepPlan(row_start, counts, after, positions, row_lens, row_seq, slots.view(torch.int64))
