@@ -414,8 +414,8 @@ size_t exl3_kv_step_plan_workspace_bytes(int batch);
  *   Per row r of the step's `rows` (row_start[b] + i is new token i of b): positions int32, its position; row_lens int32, the
  *     tokens that it sees (position + 1); row_seq int32, b; slots int64, page * 16 + position % 16.  -1, 0, -1, -1 for rows
  *     of refused sequences and behind the last one.
- * Deterministic; one or two launches; batch * max_pages below 2^30, rows below 2^28.  Calls that share a workspace must not
- * overlap. */
+ * Deterministic; one or two launches; batch * max_pages below 2^30, rows below 2^28.  A batch of 0 goes with 0 rows and writes
+ * nothing, row_start[0] and free_state_out included.  Calls that share a workspace must not overlap. */
 int exl3_kv_step_plan(int* page_table, int max_pages, const int* seq_lens, const int* new_lens, int batch, int page_size,
                       int* free_pages, int num_free, const int* free_state, int* free_state_out, int rows, int* row_start,
                       int* counts, int* lens_after, int* positions, int* row_lens, int* row_seq, long long* slots,

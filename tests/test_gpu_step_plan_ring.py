@@ -104,3 +104,11 @@ def test_pages_circulate_through_a_short_ring():
         held = [int(p) for b, n in enumerate(_n(lens_t)) for p in _n(table_t)[b, :-(-int(n) // PAGE)]]
         head, live = _n(state_t)
         assert sorted(held + [int(_n(ring_t)[(head + j) % P]) for j in range(live)]) == list(range(B * 10 + free))
+
+
+def test_an_empty_step_passes_the_state_on():
+    state, state_out, ring = _i([3, 2]), _i([99, 98]), _i([5, 6, 7, 8])
+    none = _i(np.zeros(0))
+    plan = _ops().kv_step_plan(_i(np.zeros((0, 4))), none, none, ring, state, 0, state_out)
+    assert _n(state_out).tolist() == _n(state).tolist() == [3, 2] and _n(ring).tolist() == [5, 6, 7, 8]
+    assert plan.row_start.tolist() == [0] and plan.counts.numel() == plan.slots.numel() == 0

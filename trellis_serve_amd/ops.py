@@ -1203,8 +1203,10 @@ def kv_step_plan(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: tor
         at_seq, at_slots, at_seq + 4 * rows, 4 * (B + 4), torch._C._cuda_getCurrentRawStream(index)), "kv_step_plan")
     slots, row_start, counts, after, positions, row_lens, row_seq, _ = buf.split_with_sizes(
         (2 * rows, B + 1, B, B, rows, rows, rows, B + 4))
-    if B == 0:
+    if B == 0:  # (the library writes nothing)
         row_start.zero_()
+        if state_out is not free_state:
+            state_out.copy_(free_state)
     return StepPlan(row_start, counts, after, positions, row_lens, row_seq, slots.view(torch.int64))
 
 
