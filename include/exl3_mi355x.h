@@ -446,7 +446,7 @@ int exl3_kv_page_bounds(const void* k_cache, int num_pages, const int* page_tabl
 /* Rows of the two calls below: row r is a query of sequence row_seq[r] (int32 [rows]; NULL: sequence r, rows = batch) that sees
  * its first seq_lens[r] tokens (int32 [rows]).  A row of another sequence than 0 .. batch - 1 sees none.  q fp16
  * [rows][num_q_heads][128], row stride ld_q. */
-/* Workspace bytes of exl3_kv_select_pages.  No zero-fill needed. */
+/* Workspace bytes of exl3_kv_select_pages for up to `rows` rows.  No zero-fill needed. */
 size_t exl3_kv_select_workspace_bytes(int rows, int num_kv_heads, int max_pages);
 /* pages_out int32 [rows][num_kv_heads][top]: the pages (numbers within the sequence, ascending, -1 behind the last) that a row
  * reads: all where it sees at most `top`, else its first `first` and last `last` ones (last >= 1, first + last <= top), and of
@@ -459,7 +459,7 @@ int exl3_kv_select_pages(const void* q, long long ld_q, const void* k_scale, con
                          const int* page_table, int batch, int max_pages, const int* row_seq, const int* seq_lens, int rows,
                          int num_q_heads, int num_kv_heads, int head_dim, int page_size, int bits, int top, int first,
                          int last, int* pages_out, void* workspace, size_t workspace_bytes, void* stream);
-/* Workspace bytes of exl3_kv_sparse_attention (0 where it needs none).  No zero-fill needed. */
+/* Workspace bytes of exl3_kv_sparse_attention for up to `rows` rows (0 where none of them need one).  No zero-fill needed. */
 size_t exl3_kv_sparse_workspace_bytes(int rows, int num_q_heads, int num_kv_heads, int top);
 /* out fp16 [rows][num_q_heads][128] = softmax(sm_scale q . K^T) V over those tokens of the pages pages[r][kv head][0 .. top)
  * that the row sees; entries that are no page of what it sees are left out, the others are distinct.  A row that sees nothing

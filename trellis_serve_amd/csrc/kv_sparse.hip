@@ -680,10 +680,11 @@ struct SparsePlan {
 };
 // Enough workgroups for four a CU, each with a page a wave at least (16 sequences of 128 pages, 8 bits, 8 kv heads: two a CU 19 us,
 // four 17, eight 19; 32 rows of 256 pages, 4 bits: 43, 32, 34)
+constexpr int kSparseGroups = 1024;
+static int sparse_most_parts(int top) { return std::min(kSparseParts, (top + kSparseWaves - 1) / kSparseWaves); }
 static SparsePlan sparse_plan(int rows, int Hkv, int top) {
   const long long pairs = (long long)rows * Hkv;
-  const int most = std::min(kSparseParts, (top + kSparseWaves - 1) / kSparseWaves);
-  const int parts = (int)std::max<long long>(1, std::min<long long>(most, (1024 + pairs - 1) / pairs));
+  const int parts = (int)std::max<long long>(1, std::min<long long>(sparse_most_parts(top), (kSparseGroups + pairs - 1) / pairs));
   const int per = ((top + parts - 1) / parts + kSparseWaves - 1) / kSparseWaves * kSparseWaves;
   return SparsePlan{per, (top + per - 1) / per};
 }
@@ -797,8 +798,13 @@ extern "C" int exl3_kv_select_pages(const void* q, long long ld_q, const void* k
 
 extern "C" size_t exl3_kv_sparse_workspace_bytes(int rows, int num_q_heads, int num_kv_heads, int top) {
   if (rows <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || top <= 0) return 0;
-  const SparsePlan plan = sparse_plan(rows, num_kv_heads, top);
-  return plan.parts == 1 ? 0 : (size_t)rows * num_q_heads * plan.parts * (kHeadDim + 2) * sizeof(float);
+  // rows times parts of any number of rows up to `rows`, or a little more: from kSparseGroups (row, kv head) pairs on there is one
+  // part, below that r rows have at most (kSparseGroups - 1) / (r heads) + 1 parts
+  const long long split = std::min(rows, (kSparseGroups - 1) / num_kv_heads);
+  const int most = sparse_most_parts(top);
+  if (split == 0 || most == 1) return 0;
+  const long long parts = std::min(split * most, (kSparseGroups - 1) / num_kv_heads + split);
+  return (size_t)parts * num_q_heads * (kHeadDim + 2) * sizeof(float);
 }
 
 extern "C" int exl3_kv_sparse_attention(const void* q, long long ld_q, const void* k_cache, const void* v_cache,
@@ -817,7 +823,8 @@ extern "C" int exl3_kv_sparse_attention(const void* q, long long ld_q, const voi
   EXL3_CHECK_ARG(q && seq_lens && pages && out && page_table, "exl3_kv_sparse_attention: null pointer");
   EXL3_CHECK_ARG(ld_q >= (long long)num_q_heads * head_dim && ld_q % 8 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0,
                  "exl3_kv_sparse_attention: row stride %lld (a multiple of 8, a row's heads at least; 16-byte aligned)", ld_q);
-  const size_t need = exl3_kv_sparse_workspace_bytes(rows, num_q_heads, num_kv_heads, top);
+  const SparsePlan plan = sparse_plan(rows, num_kv_heads, top);
+  const size_t need = plan.parts == 1 ? 0 : exl3_kv_sparse_workspace_bytes(rows, num_q_heads, num_kv_heads, top);
   EXL3_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                  "exl3_kv_sparse_attention: workspace %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
   const size_t blocks = (size_t)num_pages * num_kv_heads, ints = sizeof(int), code_bytes = blocks * page_size * head_dim * bits / 8;
@@ -827,7 +834,6 @@ extern "C" int exl3_kv_sparse_attention(const void* q, long long ld_q, const voi
                       {page_table, (size_t)batch * max_pages * ints}, {row_seq, rows * ints}, {seq_lens, rows * ints},
                       {pages, (size_t)rows * num_kv_heads * top * ints}};
   EXL3_CHECK_ARG(apart(all, 2), "exl3_kv_sparse_attention: the output or the workspace overlaps another tensor of the call");
-  const SparsePlan plan = sparse_plan(rows, num_kv_heads, top);
   float* part_o = static_cast<float*>(workspace);
   const int G = num_q_heads / num_kv_heads, all_heads = rows * num_q_heads;
   const SparseArgs a{static_cast<const _Float16*>(q), ld_q, static_cast<const uint8_t*>(k_cache),

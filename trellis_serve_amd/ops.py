@@ -1339,7 +1339,7 @@ def _check_rows(q: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tenso
 
 
 def kv_select_workspace_bytes(rows: int, num_kv_heads: int, max_pages: int) -> int:
-    """Bytes of a `workspace` for kv_select_pages at this shape."""
+    """Bytes of a `workspace` for kv_select_pages of up to `rows` rows."""
     return _lib.load().exl3_kv_select_workspace_bytes(rows, num_kv_heads, max_pages)
 
 
@@ -1383,7 +1383,7 @@ def kv_select_pages(q: torch.Tensor, bounds: torch.Tensor, k_scale: torch.Tensor
 
 
 def kv_sparse_workspace_bytes(rows: int, num_q_heads: int, num_kv_heads: int, top: int) -> int:
-    """Bytes of a `workspace` for kv_sparse_attention at this shape (0: it needs none)."""
+    """Bytes of a `workspace` for kv_sparse_attention of up to `rows` rows (0: none of them need one)."""
     return _lib.load().exl3_kv_sparse_workspace_bytes(rows, num_q_heads, num_kv_heads, top)
 
 
