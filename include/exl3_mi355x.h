@@ -470,7 +470,7 @@ int exl3_kv_sparse_attention(const void* q, long long ld_q, const void* k_cache,
                              int head_dim, int page_size, int bits, const int* pages, int top, float sm_scale, void* out,
                              void* workspace, size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of exl3_sample.  No zero-fill needed. */
+/* Workspace bytes of exl3_sample for up to `rows` rows; no more for more than 512.  No zero-fill needed. */
 size_t exl3_sample_workspace_bytes(int rows, int vocab);
 /* Tokens from logits [rows][vocab] (fp16 | bf16 | fp32, row stride ld; NaN as -inf; vocab up to 2^20): with w = exp((l - max l) /
  * temperature) and the elements in order of falling logits (ties by rising index), kept is the shortest of

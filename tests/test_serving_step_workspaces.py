@@ -37,3 +37,15 @@ def test_sparse_attention_workspace_for_the_most_rows_serves_fewer(lib, hq, hkv,
 def test_choice_workspace_for_the_most_rows_serves_fewer(lib, hkv, width):
     sizes = [lib.exl3_kv_select_workspace_bytes(r, hkv, width) for r in range(1, 300)]
     assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("vocab", [1, 5, 8, 70, 777, 1023, 1024, 1025, 4097, 32003, 131072, 1 << 20])
+def test_sampling_workspace_is_one_slice_of_rows(lib, vocab):
+    """Rows are worked on 512 at a time: more of them take no more, and a workspace for the most serves fewer."""
+    rows = [*range(1, 530), 1030, 16384, 65536, 100000, (1 << 26) - 1]
+    sizes = [lib.exl3_sample_workspace_bytes(r, vocab) for r in rows]
+    assert sizes == sorted(sizes)
+    assert sizes[-1] == sizes[511]
+    chunks = -(-vocab // 4096)
+    # a row's state (256 bytes at most), its list of 8192 numbers of 8 bytes, and 256 bins of 12 bytes and some sums a chunk
+    assert sizes[-1] <= 512 * (256 + 8192 * 8 + chunks * (256 * 12 + 64))

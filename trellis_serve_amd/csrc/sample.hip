@@ -933,7 +933,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_probs_kernel(const Sampl
 
 // Chunks of 8192 elements, or 4096 for more workgroups where there are few elements in all (one row of 32003 fp32: the chunks'
 // kernel takes 7.0 us with 4 chunks, 5.0 with 8)
-static int sample_chunk(int rows, int vocab) { return (long long)rows * vocab <= (1 << 19) ? kSmallChunk : kLargeChunk; }
+constexpr int kFewElements = 1 << 19;
+static int sample_chunk(int rows, int vocab) { return (long long)rows * vocab <= kFewElements ? kSmallChunk : kLargeChunk; }
 static size_t sample_bytes(int rows, int chunks) {
   return rows * (sizeof(SampleBorder) + kList * sizeof(u64_t) +
                  chunks * (sizeof(SampleChunk) + sizeof(double) + sizeof(u64_t) + kBins * (sizeof(u64_t) + sizeof(int))));
@@ -956,9 +957,9 @@ using namespace exl3;
 
 extern "C" size_t exl3_sample_workspace_bytes(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab) return 0;
-  // the most that up to `rows` rows need: fewer may take smaller chunks
+  // the most that up to `rows` rows need, of which a slice is there at a time: fewer may take smaller chunks
   const int slice = std::min(rows, kSliceRows), chunk = sample_chunk(rows, vocab);
-  const int few = std::min(rows, (1 << 19) / vocab);
+  const int few = std::min(slice, kFewElements / vocab);
   return std::max(sample_bytes(slice, (vocab + chunk - 1) / chunk), sample_bytes(few, (vocab + kSmallChunk - 1) / kSmallChunk));
 }
 

@@ -1440,7 +1440,7 @@ def kv_sparse_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
 
 
 def sample_workspace_bytes(rows: int, vocab: int) -> int:
-    """Bytes of a `workspace` for sample_tokens and sampling_probs at this shape."""
+    """Bytes of a `workspace` for sample_tokens and sampling_probs of up to `rows` rows (no more for more than 512)."""
     return _lib.load().exl3_sample_workspace_bytes(rows, vocab)
 
 
