@@ -463,7 +463,7 @@ int exl3_kv_select_pages(const void* q, long long ld_q, const void* k_scale, con
 size_t exl3_kv_sparse_workspace_bytes(int rows, int num_q_heads, int num_kv_heads, int top);
 /* out fp16 [rows][num_q_heads][128] = softmax(sm_scale q . K^T) V over those tokens of the pages pages[r][kv head][0 .. top)
  * that the row sees; entries that are no page of what it sees are left out, the others are distinct.  A row that sees nothing
- * gives zeros.  One or two launches; deterministic; calls that share a workspace must not overlap. */
+ * gives zeros.  Probabilities times value scales keep 2^-21 of themselves, sums are in 32 bits.  One or two launches; deterministic; calls that share a workspace must not overlap. */
 int exl3_kv_sparse_attention(const void* q, long long ld_q, const void* k_cache, const void* v_cache, const void* k_scale,
                              const void* v_scale, int num_pages, const int* page_table, int batch, int max_pages,
                              const int* row_seq, const int* seq_lens, int rows, int num_q_heads, int num_kv_heads,

@@ -28,6 +28,28 @@ def test_sparse_attention_with_one_workspace_for_all_batches(bits):
         _check_sparse(got, q[:rows], cache, table[:rows], lens[:rows], bits, _n(pages))
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("Hq,Hkv,top", [(5, 1, 3), (8, 1, 40), (9, 1, 40), (32, 2, 64), (40, 8, 17)])
+def test_sparse_attention_keeps_probabilities_past_sixteen_bits(bits, Hq, Hkv, top):
+    """Queries of zeros: every key has the same probability, so outputs are means of values of every scale.  A product loses 2^-21,
+    fp32 sums some 64 roundings (a wave's pages, the waves, the parts) of 2^-24 of the mean |v|, and the output half a step of fp16
+    (2^-25 where it is subnormal); the same probabilities rounded to fp16 would be up to another half a step off."""
+    lens = [16 * top, 16 * top - 7, 900, 33, 1]
+    rng, cache, table, edge, q = _rows_case(top + bits, lens, Hq, Hkv, bits)
+    cache[3] = (rng.uniform(1, 2, cache[3].shape) * 2.0 ** rng.integers(-6, 3, (cache[3].shape[0], 1))).astype(np.float16)
+    q[:] = 0
+    pages = np.full((len(lens), Hkv, top), -1, np.int32)
+    for r, n in enumerate(lens):
+        for h in range(Hkv):
+            take = rng.permutation(-(-n // 16))[:top]
+            pages[r, h, :len(take)] = np.sort(take)
+    got = _ops().kv_sparse_attention(_t(q), *[_t(x) for x in cache], _t(table), _i(lens), bits, _t(pages))
+    out, mean, _ = ref.sparse_attention(q, cache, table, lens, bits, pages, 128 ** -0.5)
+    d = np.abs(got.double().cpu().numpy() - out)
+    tol = np.maximum(np.abs(out) * 2.0 ** -11, 2.0 ** -25) + mean * (2.0 ** -21 + 64 * 2.0 ** -24)
+    assert (d <= tol).all(), ((d / tol).max(), (d > tol).mean())
+
+
 # ---- sampling of more than 2^19 logits in all, which are worked on in chunks of 8192 -------------------------------------
 
 def _check_large(logits, u, t=1.0, k=0, p=1.0, m=0.0):

@@ -491,16 +491,33 @@ struct SparseArgs {
 
 constexpr int kSparseWaves = 4;
 
-// A wave's online softmax of the group's heads over pages.  P' = p * v_scale is rounded to fp16, so the reference m lies 11
-// (base 2) below the largest p * v_scale so far, and moves when a page passes it by 15: probabilities keep fp16's normal
-// range whatever the values' scale.  l sums p itself, at most 2^39 a key.
-template <int BITS>
+// P' = p * v_scale enters the product as two halves, its first 11 bits and the next 11, so that it loses no more than 2^-21 of
+// itself.  (By one half, rounded, outputs were 2.3e-4 of their norm off, of which fp16 outputs cannot but be 2.1e-4; by both they
+// are 2.1e-4.)
+constexpr uint32_t kFirstHalf = 0xFFFFE000u;  // of a float
+
+// four values, each cut to 11 bits
+__device__ __forceinline__ half4_t cut_to_halves(const float x[4]) {
+  return __builtin_bit_cast(half4_t, kv_u32x2_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1])),
+                                                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]))});
+}
+__device__ __forceinline__ float without(float x, uint32_t bits) {
+  return x - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & bits);
+}
+
+// A wave's online softmax of the group's heads over pages.  Groups of up to 8 heads have each head in columns n and n + 8 of the
+// product, with the first halves in the one and the second in the other: one MFMA, as for the first alone (the pair of calls then
+// takes 1.5 % longer; by an MFMA for each, rounded halves, 5 %).  WIDE groups take two.  The reference m lies 11 (base 2) below the
+// largest p * v_scale so far, and moves when a page passes it by 15: probabilities keep fp16's normal range whatever the values'
+// scale.  l sums p itself, at most 2^39 a key.
+template <int BITS, bool WIDE>
 struct SparseState {
   float m = -INFINITY, l = 0.f;
   float4_t o[8];
 
+  // left_out: not WIDE: kFirstHalf in columns 8 .. 15, 0 in the others
   __device__ __forceinline__ void page(const KvRegs<BITS>& r, const half8_t qf[4], float qsum, int key0, int L,
-                                       float qk_scale, int g) {
+                                       float qk_scale, int g, uint32_t left_out) {
     constexpr float kBias = BITS == 8 ? 1152.0f : 1032.0f;
     float4_t st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -520,24 +537,34 @@ struct SparseState {
 #pragma unroll
       for (int db = 0; db < 8; db++) o[db] *= alpha;
     }
-    float psum = 0.f;
-    half4_t pf;
+    float psum = 0.f, x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const float p = __builtin_amdgcn_exp2f(sv[i] - m);
       psum += p;
-      pf[i] = (_Float16)(p * vs);
+      x[i] = p * vs;
+      if constexpr (!WIDE) x[i] = without(x[i], left_out);
+    }
+    const half4_t first = cut_to_halves(x);
+    half4_t second;
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = without(x[i], kFirstHalf);
+      second = cut_to_halves(x);
     }
     l += sum_over_groups(psum);
     uint32_t vt[8];
     r.vtrans(vt);
 #pragma unroll
-    for (int db = 0; db < 8; db++)
-      o[db] = __builtin_amdgcn_mfma_f32_16x16x16f16(codes_f16(vt[db], (_Float16)kBias), pf, o[db], 0, 0, 0);
+    for (int db = 0; db < 8; db++) {
+      const half4_t v = codes_f16(vt[db], (_Float16)kBias);
+      o[db] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, first, o[db], 0, 0, 0);
+      if constexpr (WIDE) o[db] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, second, o[db], 0, 0, 0);
+    }
   }
 };
 
-template <int BITS>
+template <int BITS, bool WIDE>
 __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(const SparseArgs a) {
   constexpr int ROW = KvRegs<BITS>::ROW, W = kSparseWaves;
   extern __shared__ float red[];  // [W][G][D + 1], then [W][G][2]
@@ -554,8 +581,9 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
   half8_t qf[4];
   float qpart = 0.f;
   {
-    const _Float16* qrow = a.q + row * a.ld_q + (size_t)(hk * G + min(n, G - 1)) * kHeadDim + 32 * g;
-    const bool live = n < G;
+    const int head = WIDE ? n : n & 7;
+    const _Float16* qrow = a.q + row * a.ld_q + (size_t)(hk * G + min(head, G - 1)) * kHeadDim + 32 * g;
+    const bool live = head < G;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const half8_t raw = *reinterpret_cast<const half8_t*>(qrow + 8 * c);
@@ -567,7 +595,8 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
     }
   }
   const float qsum = sum_over_groups(qpart);
-  SparseState<BITS> s;
+  const uint32_t left_out = n & 8 ? kFirstHalf : 0;
+  SparseState<BITS, WIDE> s;
 #pragma unroll
   for (int db = 0; db < 8; db++) s.o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
 
@@ -590,7 +619,7 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
           load(r[j ^ 1], after);
           const int then = entry(i + 2 * W);
           issue_fence();
-          if (lp >= 0 && lp < table_pages) s.page(r[j], qf, qsum, lp * kPage, L, a.qk_scale, g);
+          if (lp >= 0 && lp < table_pages) s.page(r[j], qf, qsum, lp * kPage, L, a.qk_scale, g, left_out);
           lp = after, after = then;
           i += W;
           more = i < end;
@@ -601,6 +630,12 @@ __global__ __launch_bounds__(64 * kSparseWaves) void sparse_attention_kernel(con
 
   // (logits that are NaN move no reference: without this a query of them alone would count as one that sees nothing)
   if (s.m == -INFINITY && s.l != 0.f) s.m = 0.f;
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int db = 0; db < 8; db++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s.o[db][i] += lane_xor<8>(s.o[db][i]);
+  }
   // join the waves; lane (n, g) holds dims 32 g + 8 i + db of query n
   float* red_ml = red + W * G * (kHeadDim + 1);
   if (n < G) {
@@ -843,7 +878,8 @@ extern "C" int exl3_kv_sparse_attention(const void* q, long long ld_q, const voi
                      plan.parts == 1 ? nullptr : part_o + (size_t)all_heads * plan.parts * kHeadDim,
                      static_cast<_Float16*>(out)};
   const size_t lds = (size_t)kSparseWaves * G * (kHeadDim + 1 + 2) * sizeof(float);
-  auto kern = bits == 8 ? sparse_attention_kernel<8> : sparse_attention_kernel<4>;
+  auto kern = bits == 8 ? (G > 8 ? sparse_attention_kernel<8, true> : sparse_attention_kernel<8, false>)
+                        : (G > 8 ? sparse_attention_kernel<4, true> : sparse_attention_kernel<4, false>);
   kern<<<dim3(plan.parts, num_kv_heads, rows), 64 * kSparseWaves, lds, as_stream(stream)>>>(a);
   EXL3_CHECK_LAUNCH();
   if (plan.parts > 1) {
