@@ -16,15 +16,15 @@
 //
 // sample_chunk_kernel: (chunks, rows) workgroups.  A chunk's largest logit m, its sum of exp((l - m) / t), and counts and sums
 //   in 256 bins an eighth of an octave of w wide (less where the row is flat).  An element's bin is a monotone function of its
-//   logit alone (and of the row's scale), so the chunks'
-//   bins match, and an element of a lower bin comes before every one of a higher.  Elements that the chunk alone shows to be cut
-//   (less than (1 - p) / vocab of its sum, behind its k-th, below m of its largest) stay out of the bins.
+//   logit alone (and of the row's scale), so the chunks' bins match, and an element of a lower bin comes before every one of a
+//   higher.  Elements that the chunk alone shows to be cut (behind its k-th; by up to an octave too few, so that finer bins hardly
+//   leave any of these out: less than (1 - p) / vocab of its sum, below m of its largest) stay out of the bins.
 // sample_border_kernel: a workgroup per row adds the bins up and so knows the bins that each rule's last element is in.
 // sample_list_kernel: (chunks, rows) workgroups list those bins' elements (some hundreds a row) and sum what lies before them.
 // sample_row_kernel: a workgroup per row finds the cut in the list, by histograms of ever smaller ranges; then the chunk, and in
 //   it the element, where the running sum passes the threshold.  Rows of which the border bins hold more than the list takes (most
-//   of the row equal; a top-k of half of 131072 with a top-p) go through the same search over the whole row, in one workgroup
-//   (131072 equal logits, top-p 0.9: 970 us).
+//   of the row equal; a top-k of half of 131072 with a top-p; normal logits of 262144 whose deviation is 0.3 to 1 of t, top-p 0.9)
+//   go through the same search over the whole row, in one workgroup (131072 equal logits, top-p 0.9: 970 us).
 // sample_probs_kernel: (chunks, rows) workgroups write the probabilities.
 //
 // Latency bounds it: each kernel waits for the whole of the one before, and a row's search is a chain of barriers.  In us, chunks,
@@ -287,7 +287,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   x.template get_each<EACH>(first + tid * VEC, THREADS * VEC, whole, l);
   // Each chunk looks at the same 64 elements of the row: one that is flat there has finer bins (by a power of two, so that they still
   // reach over four times the range of these), or its border bins would hold more than the list takes (131072 logits whose
-  // deviation is a tenth of t, top-p 0.9: 38 us for 463; the kernel takes 0.3 us more)
+  // deviation is a tenth of t, top-p 0.9: 38 us for 463; the kernel takes 0.3 us more).  The 256 bins and the list know no vocabulary:
+  // that serves up to 131072 of any deviation, 262144 of some, 2^20 of none below 1.6 t (3.3 ms)
   constexpr int SIDE = 16;  // elements side by side
   const bool probed = a.vocab > kList && wave == 0;
   const float probe = probed ? x.at(lane / SIDE * (a.vocab / (64 / SIDE)) + lane % SIDE) : 0.f;
@@ -317,8 +318,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   const float top = sample_place(m, rules.bin_scale);
   const bool any = m > -INFINITY;
   // Elements of bins past `deep` take no part in any rule.  By weight that holds with bins to spare while places are exact to a
-  // small part of one; exponents stand for logarithms (bins of 8 times floor(log2), up to 7 more than needed), and for top-p a sum
-  // in 32 bits is good enough.
+  // small part of one; exponents stand for logarithms, so `deep` is less than an octave, 8 << finer bins, more than needed (with
+  // finer bins that and what is needed pass the 256 soon, and nothing is left out by weight), and for top-p a sum in 32 bits is
+  // good enough.
   int deep = bins ? kBins - 2 : -1;
   const bool near = any && fabsf(top) < 0x1p16f;
   auto bins_to = [=](double w) { return (8 - 8 * __builtin_amdgcn_frexp_exp(w)) * (1 << finer) + 3; };
