@@ -13,16 +13,18 @@
 // In integers the choice does not depend on any order of summation.
 //
 // page_bounds_kernel: lanes of a (page, kv head) go through its 16 tokens with packed 16-bit minima and maxima.  Bound by the
-//   bytes: 7 sequences of 32k 4-bit tokens, 76 MB, in 17 us (4.4 TB/s).
+//   bytes: 7 sequences of up to 32k 4-bit tokens, 76 MB, in 16.7 us (4.5 TB/s).
 // page_worth_kernel: waves take 16 pages at a time.  16 heads (q8+ | q8-) against 16 x 256 codes are four MFMA 16x16x64 i8; query
-//   rows of one sequence share the codes.  Worths are written as integers that order like them.  Bound by the bounds' bytes
-//   where there are many (16 rows of up to 24k 8-bit tokens 14.9 us), by latency for one row (4.5 us at 32k).
+//   rows of one sequence share the codes.  Worths are written as integers that order like them.  Bound by latency, for one row
+//   (4.5 us at 32k) and for more: 16 rows of up to 24k 8-bit tokens, 26 MB of bounds, take 14.6 us (1.8 TB/s), since a wave has
+//   two groups of 16 pages behind its queries, their rounding and a barrier, one group ahead.
 // page_select_kernel: a workgroup per (row, kv head) keeps the worths in registers, finds the T-th largest by a histogram of its
 //   range and a ranked list of what is left, and writes the pages in ascending order by prefix sums (no atomic decides an
 //   order).  Bound by its steps' latency: 5 us for up to 2048 pages, 10 us for 8192.
 // sparse_attention_kernel: (parts of the list, kv heads, rows) workgroups, waves take pages, one 16-token page is one MFMA
 //   block, the next page is loaded meanwhile; states are joined in LDS, parts by sparse_merge_kernel in order.  Bound by the
-//   scattered pages' bytes: 16 rows x 128 pages of 8 bits, 67 MB, in 17.2 us (3.9 TB/s); 32 rows of 4 bits in 33 us.
+//   scattered pages' bytes: 16 rows x up to 128 pages of 8 bits, 66 MB, in 17.5 us (3.8 TB/s); 32 rows x 256 pages of 4 bits,
+//   134 MB, in 33.7 us (VALU 72 % of the issue).
 #include <math.h>
 
 #include <algorithm>
@@ -506,10 +508,10 @@ __device__ __forceinline__ float without(float x, uint32_t bits) {
 }
 
 // A wave's online softmax of the group's heads over pages.  Groups of up to 8 heads have each head in columns n and n + 8 of the
-// product, with the first halves in the one and the second in the other: one MFMA, as for the first alone (the pair of calls then
-// takes 1.5 % longer; by an MFMA for each, rounded halves, 5 %).  WIDE groups take two.  The reference m lies 11 (base 2) below the
-// largest p * v_scale so far, and moves when a page passes it by 15: probabilities keep fp16's normal range whatever the values'
-// scale.  l sums p itself, at most 2^39 a key.
+// product, with the first halves in the one and the second in the other: one MFMA, as for the first alone (66 MB of 8 bits for
+// groups of 4: 17.0 -> 17.5 us; 134 MB of 4 bits for groups of 5: 32.3 -> 33.7).  WIDE groups take two (the same lengths for
+// groups of 16: 22.2 -> 22.5, 38.1 -> 41.0).  The reference m lies 11 (base 2) below the largest p * v_scale so far, and moves when
+// a page passes it by 15: probabilities keep fp16's normal range whatever the values' scale.  l sums p itself, at most 2^39 a key.
 template <int BITS, bool WIDE>
 struct SparseState {
   float m = -INFINITY, l = 0.f;

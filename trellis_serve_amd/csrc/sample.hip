@@ -23,8 +23,9 @@
 // sample_list_kernel: (chunks, rows) workgroups list those bins' elements (some hundreds a row) and sum what lies before them.
 // sample_row_kernel: a workgroup per row finds the cut in the list, by histograms of ever smaller ranges; then the chunk, and in
 //   it the element, where the running sum passes the threshold.  Rows of which the border bins hold more than the list takes (most
-//   of the row equal; a top-k of half of 131072 with a top-p; normal logits of 262144 whose deviation is 0.3 to 1 of t, top-p 0.9)
-//   go through the same search over the whole row, in one workgroup (131072 equal logits, top-p 0.9: 970 us).
+//   of the row equal; a top-k of half of 131072 with a top-p; normal logits of 262144 whose deviation is 0.3 to 1 of t, top-p 0.9;
+//   a top-p with a top-k whose last element is some 2^-32 of the largest or less, past the bins, as a low t makes it) go through the
+//   same search over the whole row, in one workgroup (131072 equal logits, top-p 0.9: 970 us; such a top-k of 40: 280 us).
 // sample_probs_kernel: (chunks, rows) workgroups write the probabilities.
 //
 // Latency bounds it: each kernel waits for the whole of the one before, and a row's search is a chain of barriers.  In us, chunks,
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunk_kernel(const Sampl
   // Each chunk looks at the same 64 elements of the row: one that is flat there has finer bins (by a power of two, so that they still
   // reach over four times the range of these), or its border bins would hold more than the list takes (131072 logits whose
   // deviation is a tenth of t, top-p 0.9: 38 us for 463; the kernel takes 0.3 us more).  The 256 bins and the list know no vocabulary:
-  // that serves up to 131072 of any deviation, 262144 of some, 2^20 of none below 1.6 t (3.3 ms)
+  // that serves 131072 of every deviation tried from 0.01 t on, 262144 of some, 2^20 of none up to 1.6 t (top-p 0.9: 3.3 ms)
   constexpr int SIDE = 16;  // elements side by side
   const bool probed = a.vocab > kList && wave == 0;
   const float probe = probed ? x.at(lane / SIDE * (a.vocab / (64 / SIDE)) + lane % SIDE) : 0.f;
