@@ -8,15 +8,16 @@
 // when the running sum of need passes the live part: what one sequence gets depends on those before it only through sums, so
 // the whole is two prefix sums and a copy.  Saturating sums of numbers >= 0 are associative, which keeps them in 32 bits.
 //
-// Latency bounds it: 4.8 us of kernel for 8 sequences of one row each, 4.4 + 3.6 us for 1024 sequences of up to 127 rows.  Both scans
+// Latency bounds it: 4.8 us of kernel for 8 sequences of one row each, 4.6 + 3.6 us for 1024 sequences of up to 127 rows.  Both scans
 // of a turn take one barrier each, waves inside by DPP (four scans of two barriers, waves by LDS shuffles: 6.0 and 5.2 us).
 //
 // step_plan_kernel: one workgroup scans the sequences, 1024 at a time, and, where the step is small, fills the rows too.
 // Otherwise step_fill_kernel does: waves of one sequence write its rows, its new table entries and its returned pages.  The
 // ring's state may be updated in place, since only the first kernel reads it.
 // A returned page may go to the place of one that is taken in the same step, where the ring has fewer places than there are pages
-// (live + given back > ring_pages): all that is taken is read before anything is put back.  step_plan_kernel has a barrier
-// between the two; before step_fill_kernel it then writes the taken pages into the table, and the fill reads them there.
+// (live + given back > ring_pages): then all that is taken is read before anything is put back.  step_plan_kernel has a barrier
+// between the two; before step_fill_kernel it writes the taken pages into the table, and the fill reads them there (1024 sequences
+// of up to 127 rows: 35 us, else 7.6).
 #include <algorithm>
 
 #include "exl3_api.hpp"
@@ -90,44 +91,37 @@ __device__ __forceinline__ void plan_scan(int (&v)[N], int (&carry)[N], int (&pa
 
 __device__ __forceinline__ int plan_pages(int tokens) { return (int)(((unsigned)tokens + kPage - 1) / kPage); }
 
-// What the scans say of sequence b
+// What the scans say of sequence b, all asked for at once
 struct PlanSequence {
-  int len, asked, have, base;
+  int len, asked, have, base, count, after, r0, r1;
   int* row;
 };
 __device__ __forceinline__ PlanSequence plan_sequence(const StepPlanArgs& a, int b) {
   const int len = min(max(a.lens[b], 0), a.max_pages * kPage);
-  return PlanSequence{len, a.new_lens[b], plan_pages(len), a.base[b], a.table + (size_t)b * a.max_pages};
+  return PlanSequence{len, a.new_lens[b], plan_pages(len), a.base[b], a.counts[b], a.lens_after[b], a.row_start[b],
+                      a.row_start[b + 1], a.table + (size_t)b * a.max_pages};
 }
 
-// The pages that sequence b takes, into its table row, and its rows; or (b == batch) the rows behind the last sequence.
-// in_table: the taken pages are there
-__device__ __forceinline__ void plan_fill(const StepPlanArgs& a, int b, const PlanSequence& s, int first, int step, bool take,
-                                          bool rows, bool in_table) {
-  if (b == a.batch) {
-    if (!rows) return;
-    for (int r = a.row_start[b] + first; r < a.rows; r += step)
-      a.positions[r] = -1, a.row_lens[r] = 0, a.row_seq[r] = -1, a.slots[r] = -1;
-    return;
-  }
-  if (s.asked < 0) return;
-  const unsigned head = plan_ring(a).head, P = a.ring_pages;
-  auto taken = [&](int j) {  // base + j is below the live pages
-    const unsigned at = head + s.base + j;
-    return a.ring[at < P ? at : at - P];
-  };
-  const int count = a.counts[b];
-  if (take) {
-    const int need = plan_pages(s.len + count) - s.have;
-    for (int j = first; j < need; j += step) s.row[s.have + j] = taken(j);
-  }
-  if (!rows) return;
-  const int r0 = a.row_start[b], n = a.row_start[b + 1] - r0;
-  for (int i = first; i < n; i += step) {
-    const int r = r0 + i, pos = s.len + i, lp = pos / kPage;
-    const bool live = i < count;
+// A page that a sequence takes: base + j is below the live pages
+__device__ __forceinline__ int plan_taken(const StepPlanArgs& a, const PlanRing& ring, const PlanSequence& s, int j) {
+  const unsigned at = (unsigned)ring.head + s.base + j, P = a.ring_pages;
+  return a.ring[at < P ? at : at - P];
+}
+
+// The pages that a sequence takes, into its table row
+__device__ __forceinline__ void plan_take(const StepPlanArgs& a, const PlanRing& ring, const PlanSequence& s, int first, int step) {
+  const int need = s.asked < 0 ? 0 : plan_pages(s.len + s.count) - s.have;
+  for (int j = first; j < need; j += step) s.row[s.have + j] = plan_taken(a, ring, s, j);
+}
+
+// Sequence b's rows.  in_table: the pages that it takes are there
+__device__ __forceinline__ void plan_rows(const StepPlanArgs& a, const PlanRing& ring, const PlanSequence& s, int b, int first,
+                                          int step, bool in_table) {
+  for (int i = first; i < s.r1 - s.r0; i += step) {
+    const int r = s.r0 + i, pos = s.len + i, lp = pos / kPage;
+    const bool live = i < s.count;
     int page = 0;
-    if (live) page = in_table || lp < s.have ? s.row[lp] : taken(lp - s.have);
+    if (live) page = in_table || lp < s.have ? s.row[lp] : plan_taken(a, ring, s, lp - s.have);
     a.positions[r] = live ? pos : -1;
     a.row_lens[r] = live ? pos + 1 : 0;
     a.row_seq[r] = live ? b : -1;
@@ -135,11 +129,15 @@ __device__ __forceinline__ void plan_fill(const StepPlanArgs& a, int b, const Pl
   }
 }
 
-// The pages that sequence b gives up, to the ring's end
-__device__ __forceinline__ void plan_give(const StepPlanArgs& a, int b, const PlanSequence& s, int first, int step) {
-  if (s.asked >= 0) return;
-  const PlanRing ring = plan_ring(a);
-  const int keep = plan_pages(a.lens_after[b]), give = min(s.have - keep, ring.places - s.base);
+// The rows behind the last sequence
+__device__ __forceinline__ void plan_no_rows(const StepPlanArgs& a, int first, int step) {
+  for (int r = a.row_start[a.batch] + first; r < a.rows; r += step)
+    a.positions[r] = -1, a.row_lens[r] = 0, a.row_seq[r] = -1, a.slots[r] = -1;
+}
+
+// The pages that a sequence gives up, to the ring's end
+__device__ __forceinline__ void plan_give(const StepPlanArgs& a, const PlanRing& ring, const PlanSequence& s, int first, int step) {
+  const int keep = plan_pages(s.after), give = s.asked < 0 ? min(s.have - keep, ring.places - s.base) : 0;
   const unsigned to = (unsigned)ring.head + (unsigned)ring.live + (unsigned)s.base;
   for (int j = first; j < give; j += step) a.ring[(to + j) % (unsigned)a.ring_pages] = s.row[keep + j];
 }
@@ -178,9 +176,10 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(const StepPlanA
   }
   __syncthreads();
   const bool early = live + ends[1] > a.ring_pages;
+  const PlanRing ring{head, live, a.ring_pages - (live - popped), early};
   if (threadIdx.x == 0) {
     a.row_start[0] = 0;
-    plan_ring(a) = PlanRing{head, live, a.ring_pages - (live - popped), early};
+    plan_ring(a) = ring;
     const unsigned at = (unsigned)head + (unsigned)popped;
     a.state_out[0] = (int)(at % (unsigned)a.ring_pages);
     a.state_out[1] = min(live - popped + ends[1], a.ring_pages);
@@ -188,21 +187,29 @@ __global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(const StepPlanA
   if (!FILL && !early) return;
   __syncthreads();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int b = wave; b <= a.batch; b += kPlanThreads / 64)
-    plan_fill(a, b, plan_sequence(a, min(b, a.batch - 1)), lane, 64, true, FILL, false);
-  if (!FILL || ends[1] == 0) return;
+  for (int b = wave; b < a.batch; b += kPlanThreads / 64) {
+    const PlanSequence s = plan_sequence(a, b);
+    plan_take(a, ring, s, lane, 64);
+    if (FILL) plan_rows(a, ring, s, b, lane, 64, false);
+    if (FILL && !early) plan_give(a, ring, s, lane, 64);
+  }
+  if (!FILL) return;
+  if (wave == a.batch % (kPlanThreads / 64)) plan_no_rows(a, lane, 64);
+  if (!early) return;
   __syncthreads();
-  for (int b = wave; b < a.batch; b += kPlanThreads / 64) plan_give(a, b, plan_sequence(a, b), lane, 64);
+  for (int b = wave; b < a.batch; b += kPlanThreads / 64) plan_give(a, ring, plan_sequence(a, b), lane, 64);
 }
 
 __global__ __launch_bounds__(256) void step_fill_kernel(const StepPlanArgs a) {
   const long long i = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= (long long)(a.batch + 1) * a.slices) return;
   const int b = (int)(i / a.slices), first = (int)(i % a.slices) * 64 + (threadIdx.x & 63), step = a.slices * 64;
-  const PlanSequence s = plan_sequence(a, min(b, a.batch - 1));
-  const bool early = plan_ring(a).early;
-  plan_fill(a, b, s, first, step, !early, true, early);
-  if (b < a.batch) plan_give(a, b, s, first, step);
+  if (b == a.batch) return plan_no_rows(a, first, step);
+  const PlanRing ring = plan_ring(a);
+  const PlanSequence s = plan_sequence(a, b);
+  if (!ring.early) plan_take(a, ring, s, first, step);
+  plan_rows(a, ring, s, b, first, step, ring.early);
+  plan_give(a, ring, s, first, step);
 }
 
 }  // namespace exl3
