@@ -438,7 +438,8 @@ int exl3_add_norm(const void* x, int x_type, long long ld_x, const void* residua
 /* bounds [num_pages][num_kv_heads][2][row of codes, as k_cache has them]: the largest and the smallest key code of every
  * channel over a page's tokens, made anew for the pages that hold tokens first[b] .. seq_lens[b] - 1 of sequence b (first
  * NULL: 0), of which the last max_new at most.  After exl3_kv_append: first = the lengths before it, seq_lens those after.
- * Pages outside [0, num_pages) are left out. */
+ * Pages outside [0, num_pages) are left out.  batch * num_kv_heads * the pages that max_new tokens may touch (max_pages at most)
+ * stays below 2^28. */
 int exl3_kv_page_bounds(const void* k_cache, int num_pages, const int* page_table, int max_pages, const int* seq_lens,
                         const int* first, int max_new, int batch, int num_kv_heads, int head_dim, int page_size, int bits,
                         void* bounds, void* stream);
